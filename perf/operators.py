@@ -20,9 +20,10 @@ A case is a dict of plain values:
   fresh    "prompt": new tokens of each sequence (at most its length); 0: the whole prompt
 
 A page of a 16-bit cache is [page, kv_heads, dim].  A 4-bit cache holds codes, [kv_heads, page, dim / 2] bytes a
-page, and for each token and group of 64 channels a scale and a minimum in float16, [kv_heads, dim / 64, page, 2];
-an element stands for code * scale + minimum.  The codes of a key: 8 channels a 32-bit word, the even ones in its
-low half.  The codes of values: for 4 tokens and 2 channels a 32-bit word, a byte a token, the even channel low.
+page, and for each token and group of 64 channels a scale and a minimum in float16, [kv_heads, page, dim / 64, 2] for
+keys and [kv_heads, dim / 64, page, 2] for values; an element stands for code * scale + minimum.  A unit of codes is
+a 32-bit word: of a key 8 channels, the even ones in the low half; of values 2 channels of 4 tokens, a byte a token,
+the even channel low, [page / 4, dim / 2] units a head.  The units of two groups lie two and two by turns.
 """
 from __future__ import annotations
 
@@ -163,7 +164,8 @@ def _new_cache(case, pages):
     if case["bits"] == 16:
         return [torch.zeros(pages, page, heads, dim, dtype=DTYPES[case["dtype"]], device=DEV) for _ in range(2)]
     return ([torch.zeros(pages, heads, page, dim // 2, dtype=torch.uint8, device=DEV) for _ in range(2)]
-            + [torch.zeros(pages, heads, dim // GROUP, page, 2, dtype=torch.float16, device=DEV) for _ in range(2)])
+            + [torch.zeros(pages, heads, *shape, 2, dtype=torch.float16, device=DEV)
+               for shape in ((page, dim // GROUP), (dim // GROUP, page))])
 
 
 def _full_cache(inp, case, pages):
@@ -253,6 +255,15 @@ def _quantise(x):
 _SHIFT = [4 * (j // 2) + 16 * (j % 2) for j in range(8)]      # of channel j in a key's word
 
 
+def _by_turns(units, groups):
+    """Units of a row, group after group, in the order a cache holds them: those of two groups two and two."""
+    return units.unflatten(-1, (-1, min(2, groups), units.shape[-1] // groups // 2, 2)).transpose(-3, -2).flatten(-4)
+
+
+def _in_order(units, groups):
+    return units.unflatten(-1, (-1, units.shape[-1] // groups // 2, min(2, groups), 2)).transpose(-3, -2).flatten(-4)
+
+
 def _store(case, cache, slots, k, v):
     """Writes rows to their slots; a negative slot takes none."""
     page, dim = case["page"], case["dim"]
@@ -264,13 +275,13 @@ def _store(case, cache, slots, k, v):
         return
     codes, scales = _quantise(k)
     shift = torch.tensor(_SHIFT, device=DEV)
-    words = (codes.long().unflatten(-1, (-1, 8)) << shift).sum(-1)
+    words = _by_turns((codes.long().unflatten(-1, (-1, 8)) << shift).sum(-1), dim // GROUP)
     cache[0][at, :, row] = ((words[..., None] >> (8 * torch.arange(4, device=DEV))) & 255).flatten(-2).to(torch.uint8)
-    cache[2][at, :, :, row] = scales
+    cache[2][at, :, row] = scales
     codes, scales = _quantise(v)
     pair = codes.unflatten(-1, (-1, 2))
     words = cache[1].view(-1, case["kv_heads"], page // 4, dim // 2, 4)
-    words[at, :, row // 4, :, row % 4] = pair[..., 0] | pair[..., 1] << 4
+    words[at, :, row // 4, :, row % 4] = _by_turns(pair[..., 0] | pair[..., 1] << 4, dim // GROUP)
     cache[3][at, :, :, row] = scales
 
 
@@ -280,12 +291,12 @@ def _load(case, cache, slots):
     at, row = slots // page, slots % page
     if case["bits"] == 16:
         return cache[0][at, row].float(), cache[1][at, row].float()
-    word = cache[0].view(torch.int32).transpose(1, 2)[at, row]
+    word = _in_order(cache[0].view(torch.int32).transpose(1, 2)[at, row], dim // GROUP)
     k = ((word[..., None] >> torch.tensor(_SHIFT, dtype=torch.int32, device=DEV)) & 15).flatten(-2)
     words = cache[1].view(-1, case["kv_heads"], page // 4, dim // 2, 4).permute(0, 2, 4, 1, 3)
-    byte = words[at, row // 4, row % 4]
+    byte = _in_order(words[at, row // 4, row % 4], dim // GROUP)
     v = torch.stack((byte & 15, byte >> 4), -1).flatten(-2)
-    scales = [x.permute(0, 3, 1, 2, 4)[at, row].float() for x in cache[2:]]
+    scales = [cache[2].transpose(1, 2)[at, row].float(), cache[3].permute(0, 3, 1, 2, 4)[at, row].float()]
     return [(c.unflatten(-1, (-1, GROUP)) * s[..., :1] + s[..., 1:]).flatten(-2) for c, s in zip((k, v), scales)]
 
 
@@ -412,16 +423,21 @@ def _slot_rows(case, cache, slots):
     if case["bits"] == 16:
         return [c[at, row].double() for c in cache]
     channel = torch.arange(dim, device=DEV)
+    # Unit u of its group, in a block of one or two groups.
+    def place(u, per_group):
+        if dim == GROUP:
+            return u
+        return channel // (2 * GROUP) * 2 * per_group + u // 2 * 4 + channel // GROUP % 2 * 2 + u % 2
     bit = channel % 8 // 2 * 4 + channel % 2 * 16
-    byte = cache[0][at, :, row][:, :, channel // 8 * 4 + bit // 8]
+    byte = cache[0][at, :, row][:, :, place(channel % GROUP // 8, GROUP // 8) * 4 + bit // 8]
     k = (byte >> (bit % 8).to(torch.uint8)) & 15
-    index = (row // 4)[:, None] * (2 * dim) + channel // 2 * 4 + (row % 4)[:, None]
+    index = (row // 4)[:, None] * (2 * dim) + place(channel % GROUP // 2, GROUP // 2) * 4 + (row % 4)[:, None]
     whole = cache[1].flatten(2)[at]
     byte = torch.gather(whole, 2, index[:, None].expand(-1, whole.shape[1], -1))
     v = (byte >> (channel % 2 * 4).to(torch.uint8)) & 15
     rows = []
-    for code, scales in zip((k, v), cache[2:]):
-        pair = scales[at, :, :, row].double()[:, :, channel // GROUP]
+    for code, pair in zip((k, v), (cache[2][at, :, row], cache[3][at, :, :, row])):
+        pair = pair.double()[:, :, channel // GROUP]
         rows.append(code.double() * pair[..., 0] + pair[..., 1])
     return rows
 
