@@ -1,4 +1,5 @@
-"""ctypes binding of libnanovllm_gemm.so (declared in include/nanovllm_gemm.h).
+"""ctypes binding of libnanovllm_gemm.so (declared in include/nanovllm_gemm.h
+and include/nanovllm_attention.h).
 
 The loader mirrors the reference's ``load_cuda_ops``
 (nanovllm/kernels/_extension.py:36-68) in spirit: one cached load of a
@@ -36,6 +37,17 @@ _INT = ctypes.c_int
 _VP = ctypes.c_void_p
 _F32 = ctypes.c_float
 _U64 = ctypes.c_uint64
+
+
+class KvCacheStruct(ctypes.Structure):
+    """nanovllm_kv_cache of include/nanovllm_attention.h."""
+
+    _fields_ = [(n, _VP) for n in ("k", "v", "k_scales", "v_scales")] + [
+        (n, _I64) for n in ("num_blocks", "block_size", "kv_heads", "head_dim", "k_stride", "v_stride",
+                            "k_scales_stride", "v_scales_stride")] + [("bits", _INT), ("dtype", _INT)]
+
+
+_CACHE = ctypes.POINTER(KvCacheStruct)
 SIGNATURES = {
     "nanovllm_gemm": (_INT, [_VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _INT, _VP]),
     "nanovllm_gemm_with_kernel": (_INT, [_INT, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _INT,
@@ -65,6 +77,11 @@ SIGNATURES = {
     "nanovllm_gemm_add_rmsnorm_workspace_bytes": (_I64, [_I64, _I64, _INT]),
     "nanovllm_gemm_add_rmsnorm_with_kernel": (_INT, [_INT, _VP, _VP, _VP, _F32, _VP, _VP, _VP] + [_I64] * 8
                                               + [_INT, _INT, _INT, _VP, _I64, _VP]),
+    "nanovllm_rope_append": (_INT, [_VP] * 8 + [_CACHE] + [_I64] * 10 + [_VP]),
+    "nanovllm_kv_gather": (_INT, [_CACHE, _VP, _I64, _VP, _VP, _INT, _VP]),
+    "nanovllm_attention_prompt": (_INT, [_VP] * 6 + [_I64] * 12 + [_F32, _INT, _INT, _VP]),
+    "nanovllm_attention_paged": (_INT, [_VP, _CACHE, _VP, _VP, _VP] + [_I64] * 6 + [_F32, _INT, _VP, _I64, _VP]),
+    "nanovllm_attention_paged_workspace_bytes": (_I64, [_CACHE, _I64, _I64, _I64]),
     "nanovllm_gemm_kernel_name": (ctypes.c_char_p, [_INT]),
     "nanovllm_gemm_last_error": (ctypes.c_char_p, []),
     "nanovllm_gemm_last_kernel": (ctypes.c_char_p, []),
@@ -250,3 +267,37 @@ def add_rmsnorm_raw(h_ptr, r_ptr, nw_ptr, eps, w_ptr, c_ptr, res_ptr, m, n, k, l
     rc = (lib.nanovllm_gemm_add_rmsnorm(*args) if kernel is None
           else lib.nanovllm_gemm_add_rmsnorm_with_kernel(kernel, *args))
     check(rc, "nanovllm_gemm_add_rmsnorm")
+
+
+def rope_append_raw(q_ptr, k_ptr, v_ptr, positions_ptr, cos_sin_ptr, slots_ptr, q_out_ptr, k_out_ptr, cache, tokens,
+                    heads, q_row, q_head, k_row, k_head, v_row, v_head, positions_max, rotary, stream) -> None:
+    """Enqueue the rotation and cache append on `stream`; raise on error."""
+    check(load().nanovllm_rope_append(q_ptr, k_ptr, v_ptr, positions_ptr, cos_sin_ptr, slots_ptr, q_out_ptr,
+                                      k_out_ptr, cache, tokens, heads, q_row, q_head, k_row, k_head, v_row, v_head,
+                                      positions_max, rotary, stream), "nanovllm_rope_append")
+
+
+def kv_gather_raw(cache, slots_ptr, rows, k_ptr, v_ptr, dtype, stream) -> None:
+    """Enqueue the read of cached rows on `stream`; raise on error."""
+    check(load().nanovllm_kv_gather(cache, slots_ptr, rows, k_ptr, v_ptr, dtype, stream), "nanovllm_kv_gather")
+
+
+def attention_prompt_raw(q_ptr, k_ptr, v_ptr, cu_q_ptr, cu_k_ptr, out_ptr, batch, q_rows, k_rows, heads, kv_heads,
+                         head_dim, q_row, q_head, k_row, k_head, v_row, v_head, scale, causal, dtype, stream) -> None:
+    """Enqueue attention over packed prompts on `stream`; raise on error."""
+    check(load().nanovllm_attention_prompt(q_ptr, k_ptr, v_ptr, cu_q_ptr, cu_k_ptr, out_ptr, batch, q_rows, k_rows,
+                                           heads, kv_heads, head_dim, q_row, q_head, k_row, k_head, v_row, v_head,
+                                           scale, int(causal), dtype, stream), "nanovllm_attention_prompt")
+
+
+def attention_paged_workspace_bytes(cache, batch, heads, table_blocks) -> int:
+    """Workspace bytes of the paged attention (negative code if invalid)."""
+    return load().nanovllm_attention_paged_workspace_bytes(cache, batch, heads, table_blocks)
+
+
+def attention_paged_raw(q_ptr, cache, tables_ptr, lens_ptr, out_ptr, batch, heads, table_blocks, table_stride, q_row,
+                        q_head, scale, dtype, ws_ptr, ws_bytes, stream) -> None:
+    """Enqueue attention over a paged cache on `stream`; raise on error."""
+    check(load().nanovllm_attention_paged(q_ptr, cache, tables_ptr, lens_ptr, out_ptr, batch, heads, table_blocks,
+                                          table_stride, q_row, q_head, scale, dtype, ws_ptr, ws_bytes, stream),
+          "nanovllm_attention_paged")

@@ -14,8 +14,8 @@ kernel-resource-usage remarks (with a rocprofv3 kernel-stats CSV: per family,
 and for each kernel that run launched).
 
 ``build(sanitize=True, out=path)`` (``build.py --sanitize PATH``) builds a
-copy whose host code in capi.cpp (argument validation, the selection table,
-workspace sizes, error reporting) carries AddressSanitizer and
+copy whose host code in capi.cpp and capi_attention.cpp (argument validation, the
+selection table, workspace sizes, error reporting) carries AddressSanitizer and
 UndefinedBehaviorSanitizer; device code is built as usual.  It is loaded
 through ``NANOVLLM_GEMM_LIB`` with the sanitizer runtime preloaded
 (``sanitizer_runtime()``), for the CPU tests of the C ABI.
@@ -64,6 +64,10 @@ SOURCES = [
     "gemm_gemv.hip",
     "gemm_argmax.hip",
     "gemm_prologue.hip",
+    "capi_attention.cpp",
+    "kv_cache.hip",
+    "attention_prompt.hip",
+    "attention_paged.hip",
 ]
 
 # The microbenchmarks behind `bench.py --probes` and the decode
@@ -82,7 +86,7 @@ TORCH_OPS_LIB_PATH = PKG_DIR / "libnanovllm_torch_ops.so"
 INCLUDE_DIR = PKG_DIR.parent / "include"
 
 
-# Host-only sanitizers for capi.cpp: each -fsanitize= goes to the host pass
+# Host-only sanitizers for the C ABI's sources: each -fsanitize= goes to the host pass
 # alone (-Xarch_host), so no GPU code is instrumented.
 SANITIZE_FLAGS = [
     "-Xarch_host", "-fsanitize=address",
@@ -91,7 +95,7 @@ SANITIZE_FLAGS = [
     "-Xarch_host", "-fno-omit-frame-pointer",
     "-Xarch_host", "-g",
 ]
-SANITIZED_SOURCES = ("capi.cpp",)
+SANITIZED_SOURCES = ("capi.cpp", "capi_attention.cpp")
 
 
 def sanitizer_runtime() -> Path:

@@ -1,0 +1,113 @@
+// What the attention operators share: the paged cache as kernels see it, the
+// places of 4-bit codes, cross-lane moves and the launchers capi_attention.cpp
+// dispatches to.
+#pragma once
+
+#include "../../include/nanovllm_attention.h"
+#include "gemm_common.hpp"
+
+namespace nvg {
+
+// A paged cache (see nanovllm_kv_cache); strides between pages in bytes.
+struct Cache {
+    char *k, *v, *k_scales, *v_scales;
+    int64_t k_stride, v_stride, ks_stride, vs_stride;
+    int64_t slots;        // num_blocks * block_size
+    int32_t num_blocks, block_size, kv_heads;
+};
+
+constexpr int kGroup = 64;   // channels that share a 4-bit scale and minimum
+
+struct AppendArgs {
+    const uint16_t *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // elements
+    const int64_t* positions;
+    const float* cos_sin;
+    const int32_t* slots;
+    uint16_t *q_out, *k_out;
+    int64_t positions_max;
+    int32_t tokens, heads, rotary;
+    Cache cache;
+};
+
+struct GatherArgs {
+    const int32_t* slots;
+    uint16_t *k_out, *v_out;
+    int32_t rows;
+    Cache cache;
+};
+
+struct PromptArgs {
+    const uint16_t *q, *k, *v;
+    const int32_t *cu_q, *cu_k;
+    uint16_t* out;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // elements
+    int32_t batch, q_rows, k_rows, heads, kv_heads, causal;
+    float c;   // scale * log2(e): the softmax runs on base 2
+};
+
+struct PagedArgs {
+    const uint16_t* q;
+    const int32_t *tables, *lens;
+    uint16_t* out;
+    float* partial;
+    int64_t q_row, q_head, table_stride;
+    int32_t batch, heads, table_blocks;
+    float c;
+    Cache cache;
+};
+
+// Word u of group g of a 4-bit row with `groups` groups: its place among the
+// row's words (those of two neighbouring groups take turns two by two).
+template <int GROUPS, int PER_GROUP>
+__device__ __forceinline__ int word_place(int g, int u) {
+    if constexpr (GROUPS == 1) return u;
+    else return (g / 2) * (2 * PER_GROUP) + (u / 2) * 4 + (g % 2) * 2 + u % 2;
+}
+
+// Largest value over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lanes that hold
+// one column of a 16 x 16 product) and over l, l ^ 32 (two, of a 32 x 32 one).
+__device__ __forceinline__ float max_across32(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, uint32_t(r[0])), __builtin_bit_cast(float, uint32_t(r[1])));
+}
+__device__ __forceinline__ float max_across16(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, uint32_t(r[0])), __builtin_bit_cast(float, uint32_t(r[1])));
+}
+__device__ __forceinline__ float sum_across32(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, uint32_t(r[0])) + __builtin_bit_cast(float, uint32_t(r[1]));
+}
+__device__ __forceinline__ float sum_across16(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return __builtin_bit_cast(float, uint32_t(r[0])) + __builtin_bit_cast(float, uint32_t(r[1]));
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The index of a lane-uniform value in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+template <int N, typename F, int I = 0>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, F, I + 1>(static_cast<F&&>(f));
+    }
+}
+
+int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
+int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
+int launch_attention_prompt(const PromptArgs& p, int head_dim, int dtype, hipStream_t s);
+int launch_attention_paged(const PagedArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
+int64_t attention_paged_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  int64_t table_tokens);
+
+void clear_error();
+
+}  // namespace nvg

@@ -579,6 +579,8 @@ int set_error(int code, const char* fmt, ...) {
     return code;
 }
 
+void clear_error() { g_last_error.clear(); }
+
 int check_launch(const char* kernel, int rows, int cols) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(NANOVLLM_GEMM_ELAUNCH, "%s launch failed: %s", kernel, hipGetErrorString(e));

@@ -1,5 +1,6 @@
-// torch_ops.cpp — nanovllm::gemm, gemm_kn and the fused ops (gemm_silu_mul,
-// gemm_argmax, gemm_sample, gemm_gated, gemm_add_rmsnorm) registered from C++.
+// torch_ops.cpp — nanovllm::gemm, gemm_kn, the fused ops (gemm_silu_mul,
+// gemm_argmax, gemm_sample, gemm_gated, gemm_add_rmsnorm) and the attention ops
+// (rope_append, kv_gather, attention_prompt, attention_paged) registered from C++.
 //
 // The registration pattern of nanovllm/csrc/ops.cpp:48-80 (TORCH_LIBRARY
 // block, one CUDA-key implementation per op) over the C ABI of
@@ -9,7 +10,7 @@
 // reference's add op (nanovllm/csrc/add_kernel.cu:49-67).
 //
 // The argument contract and its messages are those of the Python
-// registration (kernels/gemm.py, kernels/prologue.py), so callers see the same
+// registration (kernels/gemm.py, kernels/prologue.py, kernels/attention.py), so callers see the same
 // RuntimeError text from either registration; the schemas are identical.
 // The fake (meta) implementations stay in Python (torch.library.register_fake).
 //
@@ -26,11 +27,13 @@
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
+#include <cstdio>
 #include <optional>
 #include <string>
 #include <tuple>
 #include <vector>
 
+#include "nanovllm_attention.h"
 #include "nanovllm_gemm.h"
 
 namespace {
@@ -339,6 +342,299 @@ std::tuple<at::Tensor, at::Tensor> gemm_add_rmsnorm(const at::Tensor& h, const a
     return {out, res};
 }
 
+// ---------------------------------------------------------------------------
+// The attention ops: kernels/attention.py's contracts, in their order and
+// wording, and their launches.
+// ---------------------------------------------------------------------------
+constexpr int64_t kGroup = 64;
+
+struct CacheTensors {
+    const at::Tensor &k, &v;
+    const std::optional<at::Tensor>&k_scales, &v_scales;
+
+    bool coded() const { return k_scales.has_value(); }
+    int64_t size() const { return k.size(coded() ? 2 : 1); }
+    int64_t heads() const { return k.size(coded() ? 1 : 2); }
+    int64_t dim() const { return coded() ? 2 * k.size(3) : k.size(3); }
+};
+
+bool blocks_contiguous(const at::Tensor& t) {
+    int64_t expected = 1;
+    for (int64_t i = t.dim() - 1; i >= 1; --i) {
+        if (t.size(i) != 1 && t.stride(i) != expected) return false;
+        expected *= t.size(i);
+    }
+    return true;
+}
+
+int64_t block_bytes(const at::Tensor& t) {
+    return (t.size(0) > 1 ? t.stride(0) : t.numel()) * static_cast<int64_t>(t.element_size());
+}
+
+std::string cache_reason(const CacheTensors& c, std::optional<at::ScalarType> dtype) {
+    if (c.k_scales.has_value() != c.v_scales.has_value()) return "k_scales and v_scales must be given together";
+    std::vector<const at::Tensor*> tensors = {&c.k, &c.v};
+    if (!c.coded()) {
+        if (!half_type(c.k) || c.v.scalar_type() != c.k.scalar_type())
+            return "k_cache and v_cache must be float16 or bfloat16 of the same dtype, or uint8 with scales";
+        if (dtype.has_value() && c.k.scalar_type() != *dtype) return "a 16-bit cache must have the dtype of its operands";
+        if (c.k.dim() != 4 || c.v.sizes() != c.k.sizes())
+            return "k_cache and v_cache must be (blocks, block_size, kv_heads, head_dim) tensors of the same shape";
+    } else {
+        const at::Tensor &ks = *c.k_scales, &vs = *c.v_scales;
+        if (c.k.scalar_type() != at::kByte || c.v.scalar_type() != at::kByte)
+            return "k_cache and v_cache must be uint8 with scales";
+        if (ks.scalar_type() != at::kHalf || vs.scalar_type() != at::kHalf)
+            return "k_scales and v_scales must be float16";
+        if (c.k.dim() != 4 || c.v.sizes() != c.k.sizes())
+            return "k_cache and v_cache must be (blocks, kv_heads, block_size, head_dim / 2) tensors of the same shape";
+        const int64_t blocks = c.k.size(0), groups = c.dim() / kGroup;
+        const std::vector<int64_t> want_k = {blocks, c.heads(), c.size(), groups, 2};
+        const std::vector<int64_t> want_v = {blocks, c.heads(), groups, c.size(), 2};
+        if (ks.sizes() != at::IntArrayRef(want_k)) return "k_scales must be (blocks, kv_heads, block_size, head_dim / 64, 2)";
+        if (vs.sizes() != at::IntArrayRef(want_v)) return "v_scales must be (blocks, kv_heads, head_dim / 64, block_size, 2)";
+        tensors.push_back(&ks);
+        tensors.push_back(&vs);
+    }
+    const int64_t dim = c.dim();
+    if (dim != 64 && dim != 128 && dim != 256) return "head_dim must be 64, 128 or 256, got " + std::to_string(dim);
+    if (c.k.size(0) < 1 || c.size() < 1 || c.heads() < 1) return "a cache must have at least one block, token and head";
+    if (c.coded() && c.size() % 16) return "block_size of a 4-bit cache must be a multiple of 16";
+    for (const at::Tensor* t : tensors)
+        if (!blocks_contiguous(*t)) return "the blocks of a cache must be contiguous";
+    for (const at::Tensor* t : tensors)
+        if (!aligned16(*t) || block_bytes(*t) % 16) return "the blocks of a cache must be 16-byte aligned";
+    return {};
+}
+
+// Element stride of dimension i; 0 where it has but one entry.
+int64_t stride_of(const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
+
+std::string rows_reason(const char* name, const at::Tensor& t, at::ScalarType dtype, int64_t heads, int64_t dim,
+                        int64_t rows) {   // heads, rows: any where negative
+    const std::string n = name;
+    if (t.scalar_type() != dtype) return n + " must have the dtype of q";
+    if (t.dim() != 3 || t.size(2) != dim || (heads >= 0 && t.size(1) != heads) || (rows >= 0 && t.size(0) != rows))
+        return n + " must be a (rows, heads, head_dim) tensor that fits the others, got " + tuple_text(t.sizes());
+    if (t.stride(2) != 1) return n + " must have unit stride in its last dimension";
+    if (stride_of(t, 0) % 8 || stride_of(t, 1) % 8) return "the strides of " + n + " must be multiples of 8";
+    if (t.numel() && !aligned16(t)) return n + " must be 16-byte aligned";
+    return {};
+}
+
+std::string index_reason(const char* name, const at::Tensor& t, at::ScalarType dtype, at::IntArrayRef shape) {
+    const std::string n = name;
+    if (t.scalar_type() != dtype) return n + " must be " + dtype_name(dtype);
+    if (t.sizes() != shape) return n + " must have shape " + tuple_text(shape) + ", got " + tuple_text(t.sizes());
+    if (!t.is_contiguous()) return n + " must be contiguous";
+    return {};
+}
+
+std::string device_reason(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && !t->is_cuda()) return "all operands must be CUDA (HIP) tensors";
+    const at::Tensor* first = *tensors.begin();
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->device() != first->device()) return "all operands must be on the same device";
+    return {};
+}
+
+const at::Tensor* optional_of(const std::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+std::string heads_reason(const at::Tensor& q, int64_t kv_heads) {
+    if (q.size(1) < 1 || q.size(1) % kv_heads)
+        return "the heads of q (" + std::to_string(q.size(1)) + ") must be a positive multiple of the " +
+               std::to_string(kv_heads) + " key-value heads";
+    return {};
+}
+
+std::string scale_reason(double scale) {
+    if (scale > 1e-37 && scale < 1e38) return {};
+    char text[64];
+    std::snprintf(text, sizeof(text), "scale must be positive and finite, got %g", scale);
+    return text;
+}
+
+nanovllm_kv_cache cache_struct(const CacheTensors& c, at::ScalarType dtype) {
+    nanovllm_kv_cache s{};
+    s.k = c.k.data_ptr();
+    s.v = c.v.data_ptr();
+    s.num_blocks = c.k.size(0);
+    s.block_size = c.size();
+    s.kv_heads = c.heads();
+    s.head_dim = c.dim();
+    s.k_stride = block_bytes(c.k);
+    s.v_stride = block_bytes(c.v);
+    if (c.coded()) {
+        s.k_scales = c.k_scales->data_ptr();
+        s.v_scales = c.v_scales->data_ptr();
+        s.k_scales_stride = block_bytes(*c.k_scales);
+        s.v_scales_stride = block_bytes(*c.v_scales);
+    }
+    s.bits = c.coded() ? 4 : 16;
+    s.dtype = dtype_code(dtype);
+    return s;
+}
+
+std::string rope_append_reason(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& positions, const at::Tensor& cos_sin, const at::Tensor& slots,
+                               const CacheTensors& c) {
+    std::string r = device_reason({&q, &k, &v, &positions, &cos_sin, &slots, &c.k, &c.v, optional_of(c.k_scales),
+                                   optional_of(c.v_scales)});
+    if (r.empty() && !half_type(q)) r = "q must be float16 or bfloat16";
+    if (r.empty()) r = cache_reason(c, q.scalar_type());
+    if (!r.empty()) return r;
+    const at::ScalarType dt = q.scalar_type();
+    const int64_t heads = c.heads(), dim = c.dim();
+    r = rows_reason("q", q, dt, -1, dim, -1);
+    if (r.empty()) r = heads_reason(q, heads);
+    if (r.empty()) r = rows_reason("k", k, dt, heads, dim, q.size(0));
+    if (r.empty()) r = rows_reason("v", v, dt, heads, dim, q.size(0));
+    if (r.empty()) r = index_reason("positions", positions, at::kLong, {q.size(0)});
+    if (r.empty()) r = index_reason("slots", slots, at::kInt, {q.size(0)});
+    if (!r.empty()) return r;
+    if (cos_sin.scalar_type() != at::kFloat || cos_sin.dim() != 2 || !cos_sin.is_contiguous() || cos_sin.size(0) < 1)
+        return "cos_sin must be a contiguous float32 (positions, rotary_dim) tensor";
+    const int64_t rotary = cos_sin.size(1);
+    if (rotary < 16 || rotary % 16 || rotary > dim)
+        return "rotary_dim (" + std::to_string(rotary) + ") must be a multiple of 16 from 16 to head_dim (" +
+               std::to_string(dim) + ")";
+    return {};
+}
+
+std::tuple<at::Tensor, at::Tensor> rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                               const at::Tensor& positions, const at::Tensor& cos_sin,
+                                               const at::Tensor& slots, const at::Tensor& k_cache,
+                                               const at::Tensor& v_cache, const std::optional<at::Tensor>& k_scales,
+                                               const std::optional<at::Tensor>& v_scales) {
+    const CacheTensors c{k_cache, v_cache, k_scales, v_scales};
+    const std::string reason = rope_append_reason(q, k, v, positions, cos_sin, slots, c);
+    TORCH_CHECK(reason.empty(), "nanovllm::rope_append: ", reason);
+    at::Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+    if (q.size(0) == 0) return {q_out, k_out};
+    const c10::DeviceGuard guard(q.device());
+    const nanovllm_kv_cache cache = cache_struct(c, q.scalar_type());
+    check_rc(nanovllm_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                  static_cast<const int64_t*>(positions.data_ptr()),
+                                  static_cast<const float*>(cos_sin.data_ptr()),
+                                  static_cast<const int32_t*>(slots.data_ptr()), q_out.data_ptr(), k_out.data_ptr(),
+                                  &cache, q.size(0), q.size(1), stride_of(q, 0), stride_of(q, 1), stride_of(k, 0),
+                                  stride_of(k, 1), stride_of(v, 0), stride_of(v, 1), cos_sin.size(0), cos_sin.size(1),
+                                  stream_of(q)),
+             "nanovllm_rope_append");
+    return {q_out, k_out};
+}
+
+std::string kv_gather_reason(const CacheTensors& c, const at::Tensor& slots, std::optional<at::ScalarType> out_dtype) {
+    std::string r = device_reason({&c.k, &c.v, &slots, optional_of(c.k_scales), optional_of(c.v_scales)});
+    if (r.empty()) r = cache_reason(c, std::nullopt);
+    if (!r.empty()) return r;
+    if (!c.coded() && out_dtype.has_value() && *out_dtype != c.k.scalar_type())
+        return "out_dtype of a 16-bit cache must be its dtype";
+    if (c.coded() && !(out_dtype.has_value() && (*out_dtype == at::kHalf || *out_dtype == at::kBFloat16)))
+        return "out_dtype of a 4-bit cache must be float16 or bfloat16";
+    if (slots.dim() != 1) return "slots must be one-dimensional";
+    return index_reason("slots", slots, at::kInt, slots.sizes());
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_gather(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                             const at::Tensor& slots, const std::optional<at::Tensor>& k_scales,
+                                             const std::optional<at::Tensor>& v_scales,
+                                             std::optional<at::ScalarType> out_dtype) {
+    const CacheTensors c{k_cache, v_cache, k_scales, v_scales};
+    const std::string reason = kv_gather_reason(c, slots, out_dtype);
+    TORCH_CHECK(reason.empty(), "nanovllm::kv_gather: ", reason);
+    const at::ScalarType dt = out_dtype.value_or(k_cache.scalar_type());
+    const int64_t rows = slots.size(0);
+    at::Tensor k = at::empty({rows, c.heads(), c.dim()}, k_cache.options().dtype(dt));
+    at::Tensor v = at::empty({rows, c.heads(), c.dim()}, k_cache.options().dtype(dt));
+    if (rows == 0) return {k, v};
+    const c10::DeviceGuard guard(slots.device());
+    const nanovllm_kv_cache cache = cache_struct(c, dt);
+    check_rc(nanovllm_kv_gather(&cache, static_cast<const int32_t*>(slots.data_ptr()), rows, k.data_ptr(),
+                                v.data_ptr(), dtype_code(dt), stream_of(slots)),
+             "nanovllm_kv_gather");
+    return {k, v};
+}
+
+std::string attention_prompt_reason(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                    const at::Tensor& cu_q, const at::Tensor& cu_k, double scale) {
+    std::string r = device_reason({&q, &k, &v, &cu_q, &cu_k});
+    if (!r.empty()) return r;
+    if (!half_type(q)) return "q must be float16 or bfloat16";
+    if (q.dim() != 3 || k.dim() != 3 || (q.size(2) != 64 && q.size(2) != 128 && q.size(2) != 256))
+        return "q and k must be (rows, heads, head_dim) tensors with a head_dim of 64, 128 or 256";
+    if (k.size(1) < 1) return "k must have at least one head";
+    const at::ScalarType dt = q.scalar_type();
+    r = rows_reason("q", q, dt, -1, q.size(2), -1);
+    if (r.empty()) r = heads_reason(q, k.size(1));
+    if (r.empty()) r = rows_reason("k", k, dt, -1, q.size(2), -1);
+    if (r.empty()) r = rows_reason("v", v, dt, k.size(1), q.size(2), k.size(0));
+    if (!r.empty()) return r;
+    if (cu_q.dim() != 1 || cu_q.size(0) < 1) return "cu_seqlens_q must be one-dimensional with at least one offset";
+    r = index_reason("cu_seqlens_q", cu_q, at::kInt, cu_q.sizes());
+    if (r.empty()) r = index_reason("cu_seqlens_k", cu_k, at::kInt, cu_q.sizes());
+    return r.empty() ? scale_reason(scale) : r;
+}
+
+at::Tensor attention_prompt(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                            const at::Tensor& cu_k, double scale, bool causal) {
+    const std::string reason = attention_prompt_reason(q, k, v, cu_q, cu_k, scale);
+    TORCH_CHECK(reason.empty(), "nanovllm::attention_prompt: ", reason);
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    if (q.size(0) == 0) return out;
+    const c10::DeviceGuard guard(q.device());
+    check_rc(nanovllm_attention_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                       static_cast<const int32_t*>(cu_q.data_ptr()),
+                                       static_cast<const int32_t*>(cu_k.data_ptr()), out.data_ptr(),
+                                       cu_q.size(0) - 1, q.size(0), k.size(0), q.size(1), k.size(1), q.size(2),
+                                       stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1),
+                                       stride_of(v, 0), stride_of(v, 1), static_cast<float>(scale), causal,
+                                       dtype_code(q.scalar_type()), stream_of(q)),
+             "nanovllm_attention_prompt");
+    return out;
+}
+
+std::string attention_paged_reason(const at::Tensor& q, const CacheTensors& c, const at::Tensor& tables,
+                                   const at::Tensor& lens, double scale) {
+    std::string r = device_reason({&q, &c.k, &c.v, &tables, &lens, optional_of(c.k_scales), optional_of(c.v_scales)});
+    if (r.empty() && !half_type(q)) r = "q must be float16 or bfloat16";
+    if (r.empty()) r = cache_reason(c, q.scalar_type());
+    if (!r.empty()) return r;
+    r = rows_reason("q", q, q.scalar_type(), -1, c.dim(), -1);
+    if (r.empty()) r = heads_reason(q, c.heads());
+    if (!r.empty()) return r;
+    if (c.size() % 16) return "block_size (" + std::to_string(c.size()) + ") must be a multiple of 16";
+    if (tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != q.size(0))
+        return "block_tables must be an int32 (batch, blocks) tensor";
+    if (tables.size(1) > 1 && tables.stride(1) != 1) return "block_tables must have unit stride in its last dimension";
+    r = index_reason("context_lens", lens, at::kInt, {q.size(0)});
+    return r.empty() ? scale_reason(scale) : r;
+}
+
+at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& tables, const at::Tensor& lens, double scale,
+                           const std::optional<at::Tensor>& k_scales, const std::optional<at::Tensor>& v_scales) {
+    const CacheTensors c{k_cache, v_cache, k_scales, v_scales};
+    const std::string reason = attention_paged_reason(q, c, tables, lens, scale);
+    TORCH_CHECK(reason.empty(), "nanovllm::attention_paged: ", reason);
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    const int64_t batch = q.size(0), blocks = tables.size(1);
+    if (batch == 0) return out;
+    const c10::DeviceGuard guard(q.device());
+    const nanovllm_kv_cache cache = cache_struct(c, q.scalar_type());
+    const int64_t need = nanovllm_attention_paged_workspace_bytes(&cache, batch, q.size(1), blocks);
+    check_rc(need, "nanovllm_attention_paged_workspace_bytes");
+    const at::Tensor ws = bytes_like(q, need > 0 ? need : 1);
+    check_rc(nanovllm_attention_paged(q.data_ptr(), &cache, static_cast<const int32_t*>(tables.data_ptr()),
+                                      static_cast<const int32_t*>(lens.data_ptr()), out.data_ptr(), batch, q.size(1),
+                                      blocks, batch > 1 && blocks > 0 ? tables.stride(0) : blocks, stride_of(q, 0),
+                                      stride_of(q, 1), static_cast<float>(scale), dtype_code(q.scalar_type()),
+                                      ws.data_ptr(), need, stream_of(q)),
+             "nanovllm_attention_paged");
+    return out;
+}
+
 at::Tensor gemm(const at::Tensor& a, const at::Tensor& w, std::optional<at::ScalarType> out_dtype) {
     return launch(a, w, out_dtype, NANOVLLM_GEMM_B_NK);
 }
@@ -361,6 +657,15 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
     m.def("gemm_gated(Tensor a, Tensor gate, Tensor w, ScalarType? out_dtype=None) -> Tensor");
     m.def("gemm_add_rmsnorm(Tensor h, Tensor residual, Tensor norm_weight, Tensor w, float eps, bool silu_mul=False, "
           "ScalarType? out_dtype=None) -> (Tensor, Tensor)");
+    m.def("rope_append(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor cos_sin, Tensor slots, "
+          "Tensor(a6!) k_cache, Tensor(a7!) v_cache, Tensor(a8!)? k_scales, Tensor(a9!)? v_scales) -> "
+          "(Tensor, Tensor)");
+    m.def("kv_gather(Tensor k_cache, Tensor v_cache, Tensor slots, Tensor? k_scales=None, Tensor? v_scales=None, "
+          "ScalarType? out_dtype=None) -> (Tensor, Tensor)");
+    m.def("attention_prompt(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, float scale, "
+          "bool causal=True) -> Tensor");
+    m.def("attention_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, "
+          "float scale, Tensor? k_scales=None, Tensor? v_scales=None) -> Tensor");
 }
 
 namespace {
@@ -373,6 +678,10 @@ void implement(torch::Library& m) {
     m.impl("gemm_sample", &gemm_sample);
     m.impl("gemm_gated", &gemm_gated);
     m.impl("gemm_add_rmsnorm", &gemm_add_rmsnorm);
+    m.impl("rope_append", &rope_append);
+    m.impl("kv_gather", &kv_gather);
+    m.impl("attention_prompt", &attention_prompt);
+    m.impl("attention_paged", &attention_paged);
 }
 
 }  // namespace
@@ -383,9 +692,10 @@ TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) { implement(m); }
 
 TORCH_LIBRARY_IMPL(nanovllm, CPU, m) { implement(m); }
 
-// The fused ops have no backward: asking for one raises, as it does for a
+// The fused ops and the attention ops have no backward: asking for one raises, as it does for a
 // custom_op without an autograd formula.
 TORCH_LIBRARY_IMPL(nanovllm, Autograd, m) {
-    for (const char* op : {"gemm_silu_mul", "gemm_argmax", "gemm_sample", "gemm_gated", "gemm_add_rmsnorm"})
+    for (const char* op : {"gemm_silu_mul", "gemm_argmax", "gemm_sample", "gemm_gated", "gemm_add_rmsnorm", "rope_append",
+                           "kv_gather", "attention_prompt", "attention_paged"})
         m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

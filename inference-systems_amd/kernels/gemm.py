@@ -182,13 +182,13 @@ else:
     _gemm_kn_op.register_fake(_gemm_kn_fake)
 
 
-def register_op(name: str, impl, fake) -> None:
+def register_op(name: str, impl, fake, mutates_args=()) -> None:
     """nanovllm::<name>: its C++ implementation (csrc/torch_ops.cpp) or, with
     the custom_op registration, ``impl`` over ctypes; ``fake`` either way."""
     if REGISTRATION == "torch_library":
         torch.library.register_fake(f"nanovllm::{name}")(fake)
     else:
-        torch.library.custom_op(f"nanovllm::{name}", impl, mutates_args=()).register_fake(fake)
+        torch.library.custom_op(f"nanovllm::{name}", impl, mutates_args=mutates_args).register_fake(fake)
 
 
 def gemm(a: torch.Tensor, w: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:

@@ -1,5 +1,6 @@
 """nano-vLLM layer mirrors whose matmul is the MI355X GEMM (see linear.py,
-gdn_projection.py and mlp.py) and the Qwen3.5 RMSNorm (norm.py)."""
+attention.py, gdn_projection.py and mlp.py) and the Qwen3.5 RMSNorm (norm.py)."""
+from .attention import Qwen35Attention
 from .gdn_projection import GdnInputProjection
 from .linear import (
     ColumnParallelLinear,
@@ -22,6 +23,7 @@ __all__ = [
     "MergedColumnParallelLinear",
     "ParallelLMHead",
     "QKVParallelLinear",
+    "Qwen35Attention",
     "Qwen35MLP",
     "Qwen35RMSNorm",
     "ReplicatedLinear",
