@@ -93,6 +93,13 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // The index of a lane-uniform value in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// A word at a lane-uniform address that nothing writes during the kernel, by a
+// scalar load: it does not wait for the vector loads in flight.
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+    typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
+    return *(constant_ptr)(p);
+}
+
 template <int N, typename F, int I = 0>
 __device__ __forceinline__ void static_for(F&& f) {
     if constexpr (I < N) {
@@ -106,7 +113,7 @@ int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hip
 int launch_attention_prompt(const PromptArgs& p, int head_dim, int dtype, hipStream_t s);
 int launch_attention_paged(const PagedArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
 int64_t attention_paged_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                  int64_t table_tokens);
+                                  int64_t table_tokens, int bits);
 
 void clear_error();
 

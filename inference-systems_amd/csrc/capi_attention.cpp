@@ -71,6 +71,10 @@ int check_cache(const char* op, const nanovllm_kv_cache* c, bool touched) {
                           c->v_scales_stride % 16)))
         return set_error(NANOVLLM_GEMM_EINVAL,
                          "%s: page strides must be multiples of 16 bytes and not smaller than a page", op);
+    // A kernel holds them in 32 bits, in units of 16 bytes.
+    constexpr int64_t most = int64_t(16) * UINT32_MAX;
+    if (c->k_stride > most || c->v_stride > most || (c->bits == 4 && (c->k_scales_stride > most || c->v_scales_stride > most)))
+        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: page strides must be smaller than 64 GiB", op);
     if (!touched) return NANOVLLM_GEMM_OK;
     const int rc = check_pointers(op, {c->k, c->v}, {});
     if (rc != NANOVLLM_GEMM_OK || c->bits == 16) return rc;
@@ -105,7 +109,7 @@ int check_paged(const char* op, const nanovllm_kv_cache* cache, int64_t batch, i
                          op);
     // Units of 128 tokens, and workgroups of the join, are counted in 32 bits.
     const int64_t blocks = cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
-    if (!fits32(batch * blocks) || !fits32(batch * blocks * (table_blocks * cache->block_size / 128 + 1)))
+    if (!fits32(batch * blocks) || !fits32(batch * blocks * (table_blocks * cache->block_size / 128 + 8)))
         return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: batch, heads and table are too large", op);
     return NANOVLLM_GEMM_OK;
 }
@@ -199,7 +203,8 @@ int64_t nanovllm_attention_paged_workspace_bytes(const nanovllm_kv_cache* cache,
     clear_error();
     const int rc = check_paged("attention_paged", cache, batch, heads, table_blocks, false);
     if (rc != NANOVLLM_GEMM_OK) return rc;
-    return attention_paged_workspace(batch, heads, cache->kv_heads, cache->head_dim, table_blocks * cache->block_size);
+    return attention_paged_workspace(batch, heads, cache->kv_heads, cache->head_dim, table_blocks * cache->block_size,
+                                     cache->bits);
 }
 
 int nanovllm_attention_paged(const void* q, const nanovllm_kv_cache* cache, const int32_t* tables, const int32_t* lens,
@@ -223,7 +228,7 @@ int nanovllm_attention_paged(const void* q, const nanovllm_kv_cache* cache, cons
     rc = table_blocks > 0 ? check_pointers(op, {q, out}, {tables, lens}) : check_pointers(op, {q, out}, {lens});
     if (rc != NANOVLLM_GEMM_OK) return rc;
     const int64_t need = attention_paged_workspace(batch, heads, cache->kv_heads, cache->head_dim,
-                                                   table_blocks * cache->block_size);
+                                                   table_blocks * cache->block_size, cache->bits);
     if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
         return set_error(NANOVLLM_GEMM_EINVAL, "attention_paged: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
                          (long long)need, (long long)workspace_bytes);
