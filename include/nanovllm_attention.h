@@ -106,7 +106,8 @@ int nanovllm_kv_gather(const nanovllm_kv_cache* cache, const int32_t* slots, int
  * query sees every key.  out = softmax(scale q k^T) v, fp32 sums, rounded once;
  * a row with no key to attend to is 0, and so are rows behind the last
  * sequence.  q, k, v as in nanovllm_rope_append; out is [q_rows, heads,
- * head_dim], contiguous.
+ * head_dim], contiguous.  Workspace: nanovllm_attention_prompt_workspace_bytes()
+ * bytes, 16-byte aligned scratch.
  */
 int nanovllm_attention_prompt(const void* q, const void* k, const void* v,
                               const int32_t* cu_q, const int32_t* cu_k, void* out,
@@ -114,7 +115,13 @@ int nanovllm_attention_prompt(const void* q, const void* k, const void* v,
                               int64_t heads, int64_t kv_heads, int64_t head_dim,
                               int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                               int64_t v_row, int64_t v_head,
-                              float scale, int causal, int dtype, void* stream);
+                              float scale, int causal, int dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of nanovllm_attention_prompt, or a negative code.  Pure host
+ * function. */
+int64_t nanovllm_attention_prompt_workspace_bytes(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads,
+                                                  int64_t kv_heads, int64_t head_dim, int dtype);
 
 /*
  * Attention of one query token per sequence over its cached tokens: out[b, h]

@@ -79,7 +79,8 @@ SIGNATURES = {
                                               + [_INT, _INT, _INT, _VP, _I64, _VP]),
     "nanovllm_rope_append": (_INT, [_VP] * 8 + [_CACHE] + [_I64] * 10 + [_VP]),
     "nanovllm_kv_gather": (_INT, [_CACHE, _VP, _I64, _VP, _VP, _INT, _VP]),
-    "nanovllm_attention_prompt": (_INT, [_VP] * 6 + [_I64] * 12 + [_F32, _INT, _INT, _VP]),
+    "nanovllm_attention_prompt": (_INT, [_VP] * 6 + [_I64] * 12 + [_F32, _INT, _INT, _VP, _I64, _VP]),
+    "nanovllm_attention_prompt_workspace_bytes": (_I64, [_I64] * 6 + [_INT]),
     "nanovllm_attention_paged": (_INT, [_VP, _CACHE, _VP, _VP, _VP] + [_I64] * 6 + [_F32, _INT, _VP, _I64, _VP]),
     "nanovllm_attention_paged_workspace_bytes": (_I64, [_CACHE, _I64, _I64, _I64]),
     "nanovllm_gemm_kernel_name": (ctypes.c_char_p, [_INT]),
@@ -282,12 +283,19 @@ def kv_gather_raw(cache, slots_ptr, rows, k_ptr, v_ptr, dtype, stream) -> None:
     check(load().nanovllm_kv_gather(cache, slots_ptr, rows, k_ptr, v_ptr, dtype, stream), "nanovllm_kv_gather")
 
 
+def attention_prompt_workspace_bytes(batch, q_rows, k_rows, heads, kv_heads, head_dim, dtype) -> int:
+    """Workspace bytes of the prompt attention (negative code if invalid)."""
+    return load().nanovllm_attention_prompt_workspace_bytes(batch, q_rows, k_rows, heads, kv_heads, head_dim, dtype)
+
+
 def attention_prompt_raw(q_ptr, k_ptr, v_ptr, cu_q_ptr, cu_k_ptr, out_ptr, batch, q_rows, k_rows, heads, kv_heads,
-                         head_dim, q_row, q_head, k_row, k_head, v_row, v_head, scale, causal, dtype, stream) -> None:
+                         head_dim, q_row, q_head, k_row, k_head, v_row, v_head, scale, causal, dtype, ws_ptr, ws_bytes,
+                         stream) -> None:
     """Enqueue attention over packed prompts on `stream`; raise on error."""
     check(load().nanovllm_attention_prompt(q_ptr, k_ptr, v_ptr, cu_q_ptr, cu_k_ptr, out_ptr, batch, q_rows, k_rows,
                                            heads, kv_heads, head_dim, q_row, q_head, k_row, k_head, v_row, v_head,
-                                           scale, int(causal), dtype, stream), "nanovllm_attention_prompt")
+                                           scale, int(causal), dtype, ws_ptr, ws_bytes, stream),
+          "nanovllm_attention_prompt")
 
 
 def attention_paged_workspace_bytes(cache, batch, heads, table_blocks) -> int:

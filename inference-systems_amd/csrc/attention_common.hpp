@@ -100,6 +100,15 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
     return *(constant_ptr)(p);
 }
 
+// dma16 (gemm_common.hpp) from a lane-uniform address and a 32-bit offset per lane.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16_at(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 template <int N, typename F, int I = 0>
 __device__ __forceinline__ void static_for(F&& f) {
     if constexpr (I < N) {
@@ -110,7 +119,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
 int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
-int launch_attention_prompt(const PromptArgs& p, int head_dim, int dtype, hipStream_t s);
+int launch_attention_prompt(const PromptArgs& p, void* workspace, int head_dim, int dtype, hipStream_t s);
+int64_t attention_prompt_workspace(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim);
 int launch_attention_paged(const PagedArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
 int64_t attention_paged_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                   int64_t table_tokens, int bits);

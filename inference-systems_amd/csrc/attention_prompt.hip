@@ -2,7 +2,7 @@
 // lengths.
 //
 // A workgroup takes 128 queries of one head of one sequence, 32 a wave, and
-// walks over the keys in tiles that all waves share in LDS:
+// walks over the keys in tiles of 64 that all waves share in LDS:
 //   S^T[key, query] = K Q^T      32 x 32 x 16 products; accumulator v of lane l
 //                                is key 8 (v / 4) + 4 (l / 32) + v % 4, query l % 32
 //   P = 2^(c S - c max)          online softmax: a query's scores lie in two
@@ -11,6 +11,14 @@
 //                                the accumulators of S^T hold them: P never moves
 // V^T is read from LDS transposed (ds_read_b64_tr_b16), 4 keys of a channel at
 // a time, which is the run of keys a lane's accumulators hold.
+//
+// The work is split over a fixed grid: all (sequence, head, 128 queries) blocks
+// in units of one tile of keys, laid end to end, each workgroup an equal run of
+// units; a block starts with two units that hold no key and stand for what it
+// costs to begin one.  So a causal prompt's long rows and short ones, a few
+// queries against many keys, and sequences of any lengths load the chip evenly.
+// A block whose keys lie in one run is finished there; the parts of others go
+// to a workspace (at most two per workgroup) and a second kernel joins them.
 #include <type_traits>
 
 #include "attention_common.hpp"
@@ -18,38 +26,171 @@
 namespace nvg {
 namespace {
 
-constexpr int kRows = 128;      // queries of a workgroup
+constexpr int kRows = 128;      // queries of a block
+constexpr int kKeys = 64;       // keys of a tile
+constexpr int kBegin = 2;       // units a block costs before its first tile
 constexpr float kLazy = 8.0f;   // sums are rescaled when a maximum grows by more than 2^8
 
-// Tiles of all sequences, 128 queries each, and of the rows behind the last one.
-__device__ __forceinline__ int start_of(const int32_t* cu, int b, int rows) { return min(max(cu[b], 0), rows); }
+struct Split {
+    PromptArgs a;
+    float* partial;
+    int32_t grid;
+    int32_t runs;      // equal runs of units; else a block per workgroup
+};
 
-__device__ __forceinline__ bool find_tile(const PromptArgs& p, int tile, int& seq, int& index) {
+// One sequence: its rows, and the tiles of keys of its blocks.
+struct Sequence {
+    int q0, lq, k0, lk;
+    int blocks;     // of 128 queries
+    int ahead;      // causal: keys of the first block's tiles before its rows, in tiles rounded up
+    int causal;
+
+    // Tiles of keys of block i.
+    __device__ __forceinline__ int tiles(int i) const {
+        if (!causal || i == blocks - 1) return (lk + kKeys - 1) / kKeys;
+        return max(0, (kRows / kKeys) * (i + 1) + ahead);
+    }
+    // Units of the blocks before i < blocks, and of all.  A block has one unit
+    // of keys at least, since one that sees no key has its rows written too.
+    __device__ __forceinline__ int64_t before(int i) const {
+        static_assert(kRows == 2 * kKeys, "the sum below is of 2 (j + 1) + ahead");
+        int64_t sum = int64_t(kBegin) * i;
+        if (!causal) return sum + int64_t(max(1, (lk + kKeys - 1) / kKeys)) * i;
+        const int from = max(0, (1 - ahead + 1) / 2 - 1);      // blocks below see one unit
+        if (i <= from) return sum + i;
+        return sum + from + int64_t(i - from) * ahead + int64_t(i) * (i + 1) - int64_t(from) * (from + 1);
+    }
+    __device__ __forceinline__ int64_t units() const {
+        return blocks == 0 ? 0 : before(blocks - 1) + kBegin + max(1, tiles(blocks - 1));
+    }
+};
+
+// Sequence b of the call, or, behind the last one, the rows that belong to none
+// (they see no key).  Offsets are taken within the operands whatever they hold.
+__device__ __forceinline__ Sequence sequence(const PromptArgs& p, int b) {
+    auto at = [](const int32_t* cu, int i, int rows) { return min(max(cu[i], 0), rows); };
+    Sequence s;
+    s.q0 = at(p.cu_q, b, p.q_rows);
+    const int q1 = b < p.batch ? at(p.cu_q, b + 1, p.q_rows) : p.q_rows;
+    s.k0 = b < p.batch ? at(p.cu_k, b, p.k_rows) : 0;
+    const int k1 = b < p.batch ? at(p.cu_k, b + 1, p.k_rows) : 0;
+    s.lq = max(0, q1 - s.q0);
+    s.lk = max(0, k1 - s.k0);
+    s.blocks = (s.lq + kRows - 1) / kRows;
+    const int more = s.lk - s.lq;
+    s.ahead = more > 0 ? (more + kKeys - 1) / kKeys : -(-more / kKeys);
+    s.causal = p.causal;
+    return s;
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    return int64_t(uint32_t(uniform(int(x)))) | int64_t(uniform(int(x >> 32))) << 32;
+}
+
+// All units: every wave adds them up for itself, 64 sequences at a time.
+__device__ __forceinline__ int64_t all_units(const PromptArgs& p) {
+    const int lane = threadIdx.x & 63;
+    int64_t mine = 0;
+    for (int b = lane; b <= p.batch; b += 64) mine += sequence(p, b).units();
+    return uniform64(wave_sum(mine)) * p.heads;
+}
+
+// A block, and its first unit.
+struct Block {
+    Sequence s;
+    int b, head, index;
+    int64_t first;
+};
+
+// The block that holds a unit below the total.
+__device__ __forceinline__ Block find_block(const PromptArgs& p, int64_t unit) {
+    const int lane = threadIdx.x & 63;
+    int64_t base = 0;
+    Block r{};
+    for (int b0 = 0; b0 <= p.batch; b0 += 64) {
+        const int64_t u = b0 + lane <= p.batch ? sequence(p, b0 + lane).units() * p.heads : 0;
+        int64_t sum = u;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t up = __shfl_up(sum, off);
+            if (lane >= off) sum += up;
+        }
+        const uint64_t past = __ballot(base + sum > unit);
+        if (past) {
+            const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            r.b = uniform(b0 + at);
+            r.first = base + uniform64(__shfl(sum - u, at));
+            break;
+        }
+        base += uniform64(__shfl(sum, 63));
+    }
+    r.s = sequence(p, r.b);
+    const int64_t each = r.s.units();
+    r.head = int((unit - r.first) / each);
+    r.first += r.head * each;
+    // The last block that starts at or before the unit: 64 candidates at a time.
+    int lo = 0, n = r.s.blocks;
+    while (n > 1) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const uint64_t before = __ballot(i < n && r.first + r.s.before(lo + i) <= unit);
+        const int at = (__popcll(static_cast<unsigned long long>(before)) - 1) * step;
+        lo += at;
+        n = min(step, n - at);
+    }
+    r.index = uniform(lo);
+    r.first += r.s.before(r.index);
+    return r;
+}
+
+// Block `index` of all sequences' (of one head), the last of a sequence first,
+// since it sees the most keys; false behind the last block.
+__device__ __forceinline__ bool nth_block(const PromptArgs& p, int index, Block& r) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int b0 = 0; b0 <= p.batch; b0 += 64) {
-        const int b = b0 + lane;
-        int n = 0;
-        if (b <= p.batch) {
-            const int from = start_of(p.cu_q, b, p.q_rows), to = b < p.batch ? start_of(p.cu_q, b + 1, p.q_rows) : p.q_rows;
-            n = max(0, (to - from + kRows - 1) / kRows);
-        }
+        const int n = b0 + lane <= p.batch ? sequence(p, b0 + lane).blocks : 0;
         int sum = n;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int up = __shfl_up(sum, off);
             if (lane >= off) sum += up;
         }
-        const uint64_t past = __ballot(base + sum > tile);
+        const uint64_t past = __ballot(base + sum > index);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            seq = uniform(b0 + at);
-            index = uniform(tile - base - __shfl(sum - n, at));
+            r.b = uniform(b0 + at);
+            r.s = sequence(p, r.b);
+            r.index = r.s.blocks - 1 - (index - base - uniform(__shfl(sum - n, at)));
+            r.first = 0;
             return true;
         }
         base += uniform(__shfl(sum, 63));
     }
     return false;
+}
+
+// The next block in order.
+__device__ __forceinline__ void advance(const PromptArgs& p, Block& r) {
+    r.first += kBegin + max(1, r.s.tiles(r.index));
+    if (++r.index < r.s.blocks) return;
+    r.index = 0;
+    if (++r.head < p.heads) return;
+    r.head = 0;
+    do r.s = sequence(p, ++r.b);
+    while (r.s.blocks == 0 && r.b < p.batch);
+}
+
+// The part of a block a workgroup leaves: rows of fp32 sums, then the rows'
+// maxima and totals of P.
+template <int D>
+__device__ __forceinline__ float* part(const Split& s, int slot) {
+    return s.partial + int64_t(slot) * kRows * (D + 2);
 }
 
 // Place of 16-byte chunk `chunk` of row `row` in a tile: chunks are exchanged
@@ -68,234 +209,432 @@ __device__ __forceinline__ int v_chunk(int row, int chunk) {
 }
 
 template <int DT>
-__device__ __forceinline__ bool finite8(u32x4_t x) {
-    constexpr uint32_t e = DT == NANOVLLM_GEMM_BF16 ? 0x7f80u : 0x7c00u;
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ok = ok && (x[i] & e) != e && ((x[i] >> 16) & e) != e;
-    return ok;
-}
-
-template <int DT>
-__device__ __forceinline__ bool finite1(uint16_t x) {
+__device__ __forceinline__ bool finite1(uint32_t x) {
     constexpr uint32_t e = DT == NANOVLLM_GEMM_BF16 ? 0x7f80u : 0x7c00u;
     return (x & e) != e;
 }
 
-// Values of a masked tile that hold an infinity or a NaN.  Products would carry
+// a . b + c over two 16-bit elements.
+template <int DT>
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    if constexpr (DT == NANOVLLM_GEMM_BF16)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, b), c, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, a), __builtin_bit_cast(f16x2_t, b), c, false);
+}
+
+// Values of a masked tile that hold an infinity or a NaN.  A product would carry
 // it into rows that do not attend to its key (0 x infinity), so such elements
-// are 0 in the products and each row adds its own share here: for every key it
-// attends to, P times the elements that are not finite.  Slow and exact in
-// what spreads; never run on finite values.
+// are 0 in the products and added here, slowly, after all tiles, to the sums in
+// LDS: for every key a row attends to, P times the elements that are not finite.
+// Finite values never come here.  `sums`: the lane's row, of which it has the
+// channels 8 i + 4 half + 0..3.
 template <int DT, int D>
-__device__ __forceinline__ void add_nonfinite(const PromptArgs& p, const uint16_t* qrow, const uint16_t* kbase,
-                                           const uint16_t* vbase, int key0, int key1, int last, int half, float shift,
-                                           f32x16_t (&o)[D / 32]) {
+__device__ __forceinline__ void add_keys(const PromptArgs& p, const uint16_t* qrow, const uint16_t* kbase,
+                                         const uint16_t* vbase, int key0, int key1, int last, int half, float shift,
+                                         float* sums) {
     for (int j = key0; j < key1; ++j) {
-        const uint16_t* vrow = vbase + j * p.v_row;
-        const uint16_t* krow = kbase + j * p.k_row;
+        const uint16_t* vrow = vbase + int64_t(j) * p.v_row;
+        const uint16_t* krow = kbase + int64_t(j) * p.k_row;
+        bool finite = true;
+        for (int ch = 0; ch < D; ch += 2) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(vrow + ch);
+            finite = finite && finite1<DT>(x) && finite1<DT>(x >> 16);
+        }
+        if (finite || j > last) continue;
         float s = 0.0f;
         for (int ch = 0; ch < D; ch += 8) {
             const u32x4_t a = load16(qrow + ch), b = load16(krow + ch);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                s = __builtin_fmaf(half_to_f32<DT>(uint16_t(a[w])), half_to_f32<DT>(uint16_t(b[w])), s);
-                s = __builtin_fmaf(half_to_f32<DT>(uint16_t(a[w] >> 16)), half_to_f32<DT>(uint16_t(b[w] >> 16)), s);
-            }
+            for (int w = 0; w < 4; ++w) s = dot2<DT>(a[w], b[w], s);
         }
         const float pj = exp2_hw(__builtin_fmaf(s, p.c, -shift));
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const uint16_t x = vrow[32 * dt + 8 * (v / 4) + 4 * half + v % 4];
-                if (j <= last && !finite1<DT>(x)) o[dt][v] = __builtin_fmaf(pj, half_to_f32<DT>(x), o[dt][v]);
-            }
+        for (int ch = 4 * half; ch < D; ch += 8)
+            for (int i = ch; i < ch + 4; ++i)
+                if (!finite1<DT>(vrow[i])) sums[i] = __builtin_fmaf(pj, half_to_f32<DT>(vrow[i]), sums[i]);
     }
 }
 
-template <int DT, int D, int BN>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel(const PromptArgs p) {
+template <int DT, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel(const Split s) {
     constexpr int CH = D / 8;                  // 16-byte chunks of a row
     constexpr int KS = D / 16;                 // steps of the contraction over channels
-    constexpr int DTILES = D / 32, NB = BN / 32;
-    constexpr int LOADS = BN * CH / 256;       // 16-byte copies per thread and tile of K, or of V
+    constexpr int DTILES = D / 32, NB = kKeys / 32;
+    constexpr int LOADS = kKeys * CH / 256;    // 16-byte copies per thread and tile of K, or of V
+    constexpr uint32_t PITCH = CH * 16, TILE = kKeys * PITCH;      // bytes of a row and of a tile in LDS
     typedef short v4i16_t __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4i16_t* lds_v4;
-    __shared__ u32x4_t kt[2][BN * CH], vt[2][BN * CH];
+    typedef const __attribute__((address_space(3))) u32x4_t* lds_u4;
+    // Two stages of keys and of values: as many bytes as the block's sums, which
+    // take their place where add_keys runs.
+    __shared__ __attribute__((aligned(1024))) u32x4_t tiles_lds[4][kKeys * CH];
+    static_assert(sizeof(tiles_lds) == kRows * D * sizeof(float), "the sums fill the tiles");
+    u32x4_t (*kt)[kKeys * CH] = tiles_lds, (*vt)[kKeys * CH] = tiles_lds + 2;
 
+    const PromptArgs& p = s.a;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int group = p.heads / p.kv_heads;
-    const int head = int(blockIdx.x) % p.heads, kvh = head / group;
-    int b, index;
-    if (!find_tile(p, int(blockIdx.x) / p.heads, b, index)) return;
+    int wg = blockIdx.x;
+    int64_t unit = 0, end;
+    Block blk{};
+    if (s.runs) {
+        wg = xcd_remap(wg, s.grid);      // neighbouring runs share keys: they go to one XCD
+        const int64_t total = all_units(p), per = (total + s.grid - 1) / s.grid;
+        unit = wg * per;
+        end = unit + per < total ? unit + per : total;
+        if (unit >= end) return;
+        blk = find_block(p, unit);
+    } else {
+        if (!nth_block(p, wg / p.heads, blk)) return;
+        blk.head = wg % p.heads;
+        end = kBegin + max(1, blk.s.tiles(blk.index));
+    }
 
-    const int q0 = start_of(p.cu_q, b, p.q_rows);
-    const int q1 = b < p.batch ? start_of(p.cu_q, b + 1, p.q_rows) : p.q_rows;
-    const int k0 = b < p.batch ? start_of(p.cu_k, b, p.k_rows) : 0;
-    const int k1 = b < p.batch ? start_of(p.cu_k, b + 1, p.k_rows) : 0;
-    const int lq = q1 - q0, lk = max(0, k1 - k0);
-    // The last tiles see the most keys: they come first.
-    const int row0 = ((lq + kRows - 1) / kRows - 1 - index) * kRows;
-    const int row = row0 + 32 * wave + col;                 // this lane's query
-    const int ahead = p.causal ? lk - lq : lk;
-    // Keys a row attends to: 0 .. last.
-    const int last = p.causal ? min(row + ahead, lk - 1) : lk - 1;
-    const int keys = p.causal ? min(lk, max(0, min(row0 + kRows, lq) + ahead)) : lk;
-    const int tiles = (keys + BN - 1) / BN;
-    // Tiles that every row of the workgroup attends to in full.
-    const int full = p.causal ? max(0, min(lk, row0 + ahead + 1)) / BN : lk / BN;
-
-    const uint16_t* qrow = p.q + int64_t(q0 + min(row, lq - 1)) * p.q_row + head * p.q_head;
-    const uint16_t* kbase = p.k + int64_t(k0) * p.k_row + kvh * p.k_head;
-    const uint16_t* vbase = p.v + int64_t(k0) * p.v_row + kvh * p.v_head;
-    u32x4_t q[KS];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) q[i] = load16(qrow + 16 * i + 8 * half);
-
-    // Thread copies of tile `t`: a wave's instruction fills 64 neighbouring
-    // chunks of LDS, each lane from the chunk that belongs there.  Rows behind
-    // the end repeat the last one (their scores are masked).
-    auto copy_tile = [&](int t, int stage) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int base = (i * 4 + wave) * 64, at = base + lane;
-            const int r = at / CH, c = at % CH;
-            const int64_t key = min(t * BN + r, lk - 1);
-            dma16(kbase + key * p.k_row + 8 * k_chunk<D>(r, c), lds_address(&kt[stage][base]));
-            dma16(vbase + key * p.v_row + 8 * v_chunk<D>(r, c), lds_address(&vt[stage][base]));
-        }
-    };
-
-    f32x16_t o[DTILES];
-#pragma unroll
-    for (int i = 0; i < DTILES; ++i) o[i] = f32x16_t{};
-    float m = -__builtin_inff(), l = 0.0f;
-
-    // Addresses of V^T: lane j of 16 points at key j / 4 and channels 4 (j % 4) of
-    // its 16-channel half; rows of a read differ from one another in their two
-    // lowest bits only, which give the chunk exchange.
+    // LDS addresses of a lane's reads, of stage 0.  Chunk exchanges are exclusive
+    // ors, so what step i of a read adds to them is one too.
+    // K: row l % 32, chunk 2 i + l / 32.  V^T: lane j of 16 points at key j / 4 and
+    // channels 4 (j % 4) of its 16-channel half; keys of a read differ from one
+    // another in their two lowest bits only, which give the exchange.
     const int vr = 4 * half + ((lane & 15) >> 2);
     const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint32_t v_off = uint32_t(vr * CH * 16 + (lane & 1) * 8);
+    const uint32_t k_read = lds_address(kt[0]) + col * PITCH + 16 * k_chunk<D>(col, half);
+    const uint32_t v_read = lds_address(vt[0]) + vr * PITCH + 16 * v_chunk<D>(vr, vc) + 8 * (lane & 1);
 
-    if (tiles > 0) copy_tile(0, 0);
-    for (int t = 0; t < tiles; ++t) {
-        const int stage = t & 1;
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (t + 1 < tiles) copy_tile(t + 1, stage ^ 1);
-        const bool masked = t >= full;
-        const u32x4_t* kp = kt[stage];
-        const u32x4_t* vp = vt[stage];
-        f32x16_t sc[NB];
+    // A tile is copied by instructions that fill 64 neighbouring chunks of LDS,
+    // 64 / CH rows, each lane from the chunk that belongs there; the next
+    // instruction of a wave is STEP rows on.  A lane's offsets from the first row:
+    // the exchange of K's chunks may change from one instruction to the next.
+    constexpr int STEP = 4 * 64 / CH;
+    const int r0 = wave * (64 / CH) + lane / CH, c0 = lane % CH;
+    const uint32_t k_bytes = uint32_t(p.k_row) * 2, v_bytes = uint32_t(p.v_row) * 2;
+    const uint32_t k_off[2] = {r0 * k_bytes + 16 * k_chunk<D>(r0, c0), r0 * k_bytes + 16 * k_chunk<D>(r0 + STEP, c0)};
+    const uint32_t v_each = r0 * v_bytes + 16 * v_chunk<D>(r0, c0), v_off[2] = {v_each, v_each};
+
+    for (;; advance(p, blk)) {
+        const int all_tiles = blk.s.tiles(blk.index), units = kBegin + max(1, all_tiles);
+        const int from = int(unit - blk.first), to = int(end - blk.first < units ? end - blk.first : units);
+        unit += to - from;
+        if (to <= kBegin) break;      // the run ends before the block's first tile
+        const int t0 = max(0, from - kBegin), t1 = min(all_tiles, to - kBegin);
+        const bool whole = t0 == 0 && to == units;
+
+        const int lq = blk.s.lq, lk = blk.s.lk, head = blk.head, kvh = head / group;
+        const int row0 = blk.index * kRows, row = row0 + 32 * wave + col;      // row: this lane's query
+        const int ahead = p.causal ? lk - lq : lk;
+        // Keys a row attends to: 0 .. last.
+        const int last = p.causal ? min(row + ahead, lk - 1) : lk - 1;
+        // Tiles that every row of the block attends to in full.
+        const int full = p.causal ? max(0, min(lk, row0 + ahead + 1)) / kKeys : lk / kKeys;
+
+        const uint16_t* qrow = p.q + int64_t(blk.s.q0 + min(row, lq - 1)) * p.q_row + head * p.q_head;
+        const uint16_t* kbase = p.k + int64_t(blk.s.k0) * p.k_row + kvh * p.k_head;
+        const uint16_t* vbase = p.v + int64_t(blk.s.k0) * p.v_row + kvh * p.v_head;
+
+        auto copy = [&](const uint16_t* rows, uint32_t bytes, const uint32_t (&off)[2], uint32_t lds, int t) {
+            const uint32_t to = lds + (t & 1) * TILE + wave * 1024;
+            const char* base = reinterpret_cast<const char*>(rows) + int64_t(t) * kKeys * bytes;
+            const int left = lk - t * kKeys;
+            if (left >= kKeys) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            sc[n] = f32x16_t{};
+                for (int i = 0; i < LOADS; ++i) dma16_at(base + i * STEP * bytes, off[i % 2], to + i * 4096);
+            } else {
+                // Rows behind the end repeat the last one (their scores are masked).
+                // Where that lies before an instruction's first row, the base moves.
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int behind = max(0, i * STEP - (left - 1)), back = max(0, r0 + i * STEP - (left - 1));
+                    dma16_at(base + (i * STEP - behind) * bytes, off[i % 2] - (back - behind) * bytes, to + i * 4096);
+                }
+            }
+        };
+        auto copy_k = [&](int t) { copy(kbase, k_bytes, k_off, lds_address(kt[0]), t); };
+        auto copy_v = [&](int t) { copy(vbase, v_bytes, v_off, lds_address(vt[0]), t); };
+        __syncthreads();      // the last block's tiles have been read
+        if (t0 < t1) {
+            copy_k(t0);
+            copy_v(t0);
+        }
+        u32x4_t q[KS];
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q[i] = load16(qrow + 16 * i + 8 * half);
+
+        f32x16_t o[DTILES];
+#pragma unroll
+        for (int i = 0; i < DTILES; ++i) o[i] = f32x16_t{};
+        float m = -__builtin_inff(), l = 0.0f;
+        uint32_t late = 0;      // masked tiles (3 at most) with values that add_keys adds
+
+        // S^T of tile t, in KS steps; reads run two steps ahead of the products, and
+        // `beside(i)` is what the vector units do in step i.  Steps are kept
+        // apart: the compiler would otherwise issue one kind of work at a time.
+        auto scores = [&](int t, f32x16_t (&sc)[NB], auto&& beside) {
+            const uint32_t k_at = k_read + (t & 1) * TILE;
+            u32x4_t kf[3][NB];
+            auto read = [&](int i) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) kf[i % 3][n] = *(lds_u4)(uintptr_t)((k_at ^ (32 * i)) + 32 * n * PITCH);
+            };
+            read(0);
+            read(1);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) sc[n] = f32x16_t{};
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                const int r = 32 * n + col;
-                sc[n] = mfma_32x32x16<DT>(kp[r * CH + k_chunk<D>(r, 2 * i + half)], q[i], sc[n]);
+                if (i + 2 < KS) read(i + 2);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) sc[n] = mfma_32x32x16<DT>(kf[i % 3][n], q[i], sc[n]);
+                beside(i);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        if (masked) {
+        };
+        // P of two scores, packed, and its sum; `pair` of NB * 8.
+        u32x4_t pk[NB][2];
+        auto weigh = [&](const f32x16_t (&sc)[NB], int pair, float shift) {
+            const int n = pair / 8, w = pair % 8;
+            const uint32_t two = pack2<DT>(exp2_hw(__builtin_fmaf(sc[n][2 * w], p.c, -shift)),
+                                           exp2_hw(__builtin_fmaf(sc[n][2 * w + 1], p.c, -shift)));
+            pk[n][w / 4][w % 4] = two;
+            l = dot2<DT>(two, DT == NANOVLLM_GEMM_BF16 ? 0x3f803f80u : 0x3c003c00u, l);
+        };
+
+        // Tile t, whose scores are in sc; those of the next tile, which only need
+        // the matrix cores, are computed while this one's softmax runs.
+        auto tile = [&](int t, f32x16_t (&sc)[NB], f32x16_t (&ahead_sc)[NB]) {
+            const bool masked = t >= full, more = t + 1 < t1;
+            wait_vmcnt<0>();      // keys of tile t + 1 and values of t
+            __syncthreads();
+            if (more) {
+                if (t + 2 < t1) copy_k(t + 2);
+                copy_v(t + 1);
+            }
+            if (masked) {
+                const int seen = last - t * kKeys - 4 * half;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (32 * n + 8 * (v / 4) + v % 4 > seen) sc[n][v] = -__builtin_inff();
+                // A look at the tile's values: see add_keys.
+                u32x4_t* mine = vt[t & 1] + threadIdx.x;
+                bool clean = true;
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const u32x4_t x = mine[i * 256];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) clean = clean && finite1<DT>(x[w]) && finite1<DT>(x[w] >> 16);
+                }
+                if (__syncthreads_or(!clean)) {
+                    late |= 1u << (t - full);
+                    for (int i = 0; i < LOADS; ++i) {
+                        u32x4_t x = mine[i * 256];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            x[w] &= (finite1<DT>(x[w]) ? 0xffffu : 0u) | (finite1<DT>(x[w] >> 16) ? 0xffff0000u : 0u);
+                        mine[i * 256] = x;
+                    }
+                    __syncthreads();
+                }
+            }
+            float top = sc[0][0];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (t * BN + 32 * n + 8 * (v / 4) + 4 * half + v % 4 > last) sc[n][v] = -__builtin_inff();
-        }
-        float top = sc[0][0];
+                for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[n][v]);
+            top = max_across32(top);
+            // A first score (m is -infinity), or one that outgrows the range P has been given.
+            if (__ballot((top - m) * p.c > kLazy)) {
+                const float higher = fmaxf(m, top);
+                const float down = higher == -__builtin_inff() ? 1.0f : exp2_hw((m - higher) * p.c);
+                m = higher;
+                l *= down;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[n][v]);
-        top = max_across32(top);
-        // A first score (m is -infinity), or one that outgrows the range P has been given.
-        if (__ballot((top - m) * p.c > kLazy)) {
-            const float higher = fmaxf(m, top);
-            const float down = higher == -__builtin_inff() ? 1.0f : exp2_hw((m - higher) * p.c);
-            m = higher;
-            l *= down;
-#pragma unroll
-            for (int i = 0; i < DTILES; ++i) o[i] *= down;
-        }
-        const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
-        u32x4_t pk[NB][2];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                sc[n][v] = exp2_hw(__builtin_fmaf(sc[n][v], p.c, -shift));
-                l += sc[n][v];
+                for (int i = 0; i < DTILES; ++i) o[i] *= down;
             }
+            const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
+            if (more) {
+                scores(t + 1, ahead_sc, [&](int i) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w) pk[n][w / 4][w % 4] = pack2<DT>(sc[n][2 * w], sc[n][2 * w + 1]);
-        }
-        bool clean = true;
-        if (masked) {
-            // A look at the tile's values: see add_nonfinite.
+                    for (int w = i * NB * 8 / KS; w < (i + 1) * NB * 8 / KS; ++w) weigh(sc, w, shift);
+                });
+            } else {
+                // (Hidden, or the compiler would move what both branches share ahead of them.)
+                float alone = shift;
+                asm volatile("" : "+v"(alone));
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) clean = clean && finite8<DT>(vp[i * 256 + threadIdx.x]);
-            clean = !__syncthreads_or(!clean);
-        }
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
+                for (int w = 0; w < NB * 8; ++w) weigh(sc, w, alone);
+            }
+            // Products of 16 keys at a time, the next 16 keys' values read meanwhile.
+            const uint32_t v_at = v_read + (t & 1) * TILE;
+            u32x4_t vf[2][DTILES];
+            auto read = [&](int g) {
 #pragma unroll
                 for (int i = 0; i < DTILES; ++i) {
-                    const uint32_t at = lds_address(vp) + v_off + uint32_t((32 * n + 16 * ks) * CH * 16) +
-                                        uint32_t(v_chunk<D>(vr, 4 * i + vc) * 16);
+                    const uint32_t at = (v_at ^ (64 * i)) + 16 * g * PITCH;
                     const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)at);
-                    const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)(at + 8 * CH * 16));
+                    const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)(at + 8 * PITCH));
                     const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-                    u32x4_t a = {l2[0], l2[1], h2[0], h2[1]};
-                    if (!clean) {
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            if (!finite1<DT>(uint16_t(a[w]))) a[w] &= 0xffff0000u;
-                            if (!finite1<DT>(uint16_t(a[w] >> 16))) a[w] &= 0xffffu;
-                        }
-                    }
-                    o[i] = mfma_32x32x16<DT>(a, pk[n][ks], o[i]);
+                    vf[g % 2][i] = u32x4_t{l2[0], l2[1], h2[0], h2[1]};
                 }
+            };
+            read(0);
+#pragma unroll
+            for (int g = 0; g < 2 * NB; ++g) {
+                if (g + 1 < 2 * NB) read(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < DTILES; ++i) o[i] = mfma_32x32x16<DT>(vf[g % 2][i], pk[g / 2][g % 2], o[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        if (!clean)
-            add_nonfinite<DT, D>(p, qrow, kbase, vbase, t * BN, min(lk, t * BN + BN), last, half, shift, o);
-    }
+        };
+        f32x16_t sc[2][NB];
+        if (t0 < t1) {
+            wait_vmcnt<0>();
+            __syncthreads();
+            if (t0 + 1 < t1) copy_k(t0 + 1);
+            scores(t0, sc[0], [](int) {});
+        }
+        for (int t = t0; t < t1;) {
+            tile(t, sc[0], sc[1]);
+            if (++t < t1) {
+                tile(t, sc[1], sc[0]);
+                ++t;
+            }
+        }
 
-    l = sum_across32(l);
-    if (row >= lq) return;
-    const float inv = last < 0 ? 0.0f : 1.0f / l;     // no key: 0
-    uint16_t* out = p.out + (int64_t(q0 + row) * p.heads + head) * D;
+        l = sum_across32(l);
+        // (Hidden from the compiler, which would keep addresses made of it in
+        // registers over the whole loop.)
+        int oc = col;
+        asm volatile("" : "+v"(oc));
+        const int mine = 32 * wave + oc;      // this lane's row of the block
+        const float inv = last < 0 ? 0.0f : 1.0f / l;     // no key: 0
+        uint16_t* out = p.out + (int64_t(blk.s.q0 + row0 + mine) * p.heads + head) * D;
+        float* slot = part<D>(s, 2 * wg + (t0 == 0 ? 1 : 0));
+        auto store = [&](int ch, f32x4_t x) {
+            if (!whole)
+                *reinterpret_cast<f32x4_t*>(slot + mine * D + ch) = x;
+            else if (row < lq)
+                *reinterpret_cast<u32x2_t*>(out + ch) =
+                    u32x2_t{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+        };
+        if (!whole && half == 0) {
+            slot[kRows * D + mine] = m;
+            slot[kRows * D + kRows + mine] = l;
+        }
+        if (!late) {
 #pragma unroll
-    for (int i = 0; i < DTILES; ++i)
+            for (int i = 0; i < DTILES; ++i)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4)
-            *reinterpret_cast<u32x2_t*>(out + 32 * i + 2 * v + 4 * half) =
-                u32x2_t{pack2<DT>(o[i][v] * inv, o[i][v + 1] * inv), pack2<DT>(o[i][v + 2] * inv, o[i][v + 3] * inv)};
+                for (int v = 0; v < 16; v += 4)
+                    store(32 * i + 2 * v + 4 * half, f32x4_t{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]});
+        } else {
+            __syncthreads();      // the tiles have been read
+            float* sums = reinterpret_cast<float*>(tiles_lds) + mine * D;
+#pragma unroll
+            for (int i = 0; i < DTILES; ++i)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4)
+                    *reinterpret_cast<f32x4_t*>(sums + 32 * i + 2 * v + 4 * half) =
+                        f32x4_t{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]};
+            const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
+            for (int t = full; t < t1; ++t)
+                if (late >> (t - full) & 1)
+                    add_keys<DT, D>(p, qrow, kbase, vbase, t * kKeys, min(lk, t * kKeys + kKeys), last, half, shift, sums);
+            for (int ch = 4 * half; ch < D; ch += 8) store(ch, *reinterpret_cast<const f32x4_t*>(sums + ch));
+        }
+        if (unit >= end) break;
+    }
+}
+
+// Joins the parts of the block that the start of run `blockIdx.x` cuts first:
+// 16 of its rows a workgroup, a row by D / 4 threads.  Parts are added in order.
+constexpr int kJoinRows = 16;
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attention_prompt_join_kernel(const Split s) {
+    constexpr int TPR = D / 4;
+    const PromptArgs& p = s.a;
+    const int wg = int(blockIdx.x) + 1;
+    const int64_t total = all_units(p), per = (total + s.grid - 1) / s.grid, unit = wg * per;
+    if (unit >= total) return;
+    const Block blk = find_block(p, unit);
+    const int64_t keys = blk.first + kBegin;      // the block's first unit with a key
+    const int64_t behind = keys + max(1, blk.s.tiles(blk.index));
+    if (unit <= keys || keys / per != wg - 1) return;
+    const int last_wg = int((behind - 1) / per);
+    const int lq = blk.s.lq, row0 = blk.index * kRows, ahead = p.causal ? blk.s.lk - lq : blk.s.lk;
+    for (int e = threadIdx.x; e < kJoinRows * TPR; e += 256) {
+        const int r = int(blockIdx.y) * kJoinRows + e / TPR, ch = 4 * (e % TPR), row = row0 + r;
+        if (row >= lq) continue;
+        float top = -__builtin_inff();
+        for (int w = wg - 1; w <= last_wg; ++w) top = fmaxf(top, part<D>(s, 2 * w + (w == wg - 1))[kRows * D + r]);
+        float l = 0.0f;
+        f32x4_t o = {0, 0, 0, 0};
+        for (int w = wg - 1; w <= last_wg; ++w) {
+            const float* src = part<D>(s, 2 * w + (w == wg - 1));
+            const float m = src[kRows * D + r];
+            // A part whose maximum is -infinity has nothing, or NaN.
+            const float f = m == -__builtin_inff() ? 1.0f : exp2_hw((m - top) * p.c);
+            l = __builtin_fmaf(f, src[kRows * D + kRows + r], l);
+            o += f * *reinterpret_cast<const f32x4_t*>(src + r * D + ch);
+        }
+        const float inv = (p.causal ? min(row + ahead, blk.s.lk - 1) : blk.s.lk - 1) < 0 ? 0.0f : 1.0f / l;
+        *reinterpret_cast<u32x2_t*>(p.out + (int64_t(blk.s.q0 + row) * p.heads + blk.head) * D + ch) =
+            u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+    }
+}
+
+// Workgroups that the chip runs at once: two a CU, one of head_dim 256.
+int resident(int head_dim) { return head_dim == 256 ? 256 : 512; }
+
+// Blocks there can be: every sequence, and the rows behind the last, round up.
+int64_t most_blocks(int64_t batch, int64_t q_rows, int64_t heads) { return (q_rows / kRows + batch + 1) * heads; }
+
+// Whether blocks are dealt in equal runs, rather than one to a workgroup.
+bool in_runs(int64_t batch, int64_t q_rows, int64_t heads, int head_dim) {
+    return most_blocks(batch, q_rows, heads) < 3 * resident(head_dim);
+}
+
+int64_t grid_of(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int head_dim) {
+    const int64_t blocks = most_blocks(batch, q_rows, heads);
+    if (!in_runs(batch, q_rows, heads, head_dim)) return blocks;
+    const int64_t units = blocks * (kBegin + 1 + k_rows / kKeys), most = resident(head_dim);
+    return units < most ? units : most;
+}
+
+template <int DT, int D>
+int launch(const Split& s, hipStream_t stream) {
+    hipLaunchKernelGGL((attention_prompt_kernel<DT, D>), dim3(s.grid), dim3(256), 0, stream, s);
+    int rc = check_launch("attention_prompt");
+    if (rc != NANOVLLM_GEMM_OK || !s.runs || s.grid == 1) return rc;
+    hipLaunchKernelGGL((attention_prompt_join_kernel<DT, D>), dim3(s.grid - 1, kRows / kJoinRows), dim3(256), 0, stream,
+                       s);
+    return check_launch("attention_prompt_join");
 }
 
 template <int DT>
-int launch_dim(const PromptArgs& p, int head_dim, hipStream_t s) {
-    // Every sequence, and the rows behind the last, round up to a tile of their own.
-    const int64_t tiles = p.q_rows / kRows + p.batch + 1;
-    const int64_t grid = tiles * p.heads;
-    if (grid > INT32_MAX) return set_error(NANOVLLM_GEMM_EINVAL, "attention_prompt: too many rows and heads");
-    const dim3 g(static_cast<uint32_t>(grid)), block(256);
-    if (head_dim == 64) hipLaunchKernelGGL((attention_prompt_kernel<DT, 64, 64>), g, block, 0, s, p);
-    else if (head_dim == 128) hipLaunchKernelGGL((attention_prompt_kernel<DT, 128, 64>), g, block, 0, s, p);
-    else hipLaunchKernelGGL((attention_prompt_kernel<DT, 256, 64>), g, block, 0, s, p);
-    return check_launch("attention_prompt");
+int launch_dim(const Split& s, int head_dim, hipStream_t stream) {
+    return head_dim == 64    ? launch<DT, 64>(s, stream)
+           : head_dim == 128 ? launch<DT, 128>(s, stream)
+                             : launch<DT, 256>(s, stream);
 }
 
 }  // namespace
 
-int launch_attention_prompt(const PromptArgs& p, int head_dim, int dtype, hipStream_t s) {
-    return dtype == NANOVLLM_GEMM_BF16 ? launch_dim<NANOVLLM_GEMM_BF16>(p, head_dim, s)
-                                       : launch_dim<NANOVLLM_GEMM_F16>(p, head_dim, s);
+int64_t attention_prompt_workspace(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim) {
+    const int64_t grid = grid_of(batch, q_rows, k_rows, heads, static_cast<int>(head_dim));
+    if (grid == 1 || !in_runs(batch, q_rows, heads, static_cast<int>(head_dim))) return 0;
+    return 2 * grid * kRows * (head_dim + 2) * 4;
+}
+
+int launch_attention_prompt(const PromptArgs& p, void* workspace, int head_dim, int dtype, hipStream_t s) {
+    const int64_t grid = grid_of(p.batch, p.q_rows, p.k_rows, p.heads, head_dim);
+    if (grid > INT32_MAX) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "attention_prompt: too many rows and heads");
+    const Split split{p, static_cast<float*>(workspace), static_cast<int32_t>(grid),
+                      in_runs(p.batch, p.q_rows, p.heads, head_dim)};
+    return dtype == NANOVLLM_GEMM_BF16 ? launch_dim<NANOVLLM_GEMM_BF16>(split, head_dim, s)
+                                       : launch_dim<NANOVLLM_GEMM_F16>(split, head_dim, s);
 }
 
 }  // namespace nvg

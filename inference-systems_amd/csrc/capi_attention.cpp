@@ -32,6 +32,10 @@ int check_strides(const char* op, const char* name, int64_t row, int64_t head) {
     if (row % 8 || head % 8 || row < 0 || head < 0)
         return set_error(NANOVLLM_GEMM_EINVAL, "%s: strides of %s (%lld, %lld) must be non-negative multiples of 8", op,
                          name, (long long)row, (long long)head);
+    // A tile of 64 rows is addressed with 32 bits.
+    if (row >= int64_t(1) << 24)
+        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: the row stride of %s (%lld) must be below 2^24", op, name,
+                         (long long)row);
     return NANOVLLM_GEMM_OK;
 }
 
@@ -93,6 +97,15 @@ constexpr float kLog2e = 1.44269504088896340736f;
 int check_scale(const char* op, float scale) {
     if (!(scale > 0.0f) || !std::isnormal(scale * kLog2e))
         return set_error(NANOVLLM_GEMM_EINVAL, "%s: scale must be positive, normal and finite", op);
+    return NANOVLLM_GEMM_OK;
+}
+
+int check_prompt(const char* op, int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim, int dtype) {
+    const int rc = check_dims(op, heads, kv_heads, head_dim, dtype);
+    if (rc != NANOVLLM_GEMM_OK) return rc;
+    if (batch < 0 || q_rows < 0 || k_rows < 0 || batch > INT32_MAX / 2 || q_rows > INT32_MAX / 2 || k_rows > INT32_MAX / 2)
+        return set_error(NANOVLLM_GEMM_EINVAL, "%s: batch and rows must be non-negative and below 2^30", op);
     return NANOVLLM_GEMM_OK;
 }
 
@@ -174,27 +187,38 @@ int nanovllm_attention_prompt(const void* q, const void* k, const void* v, const
                               void* out, int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads,
                               int64_t kv_heads, int64_t head_dim, int64_t q_row, int64_t q_head, int64_t k_row,
                               int64_t k_head, int64_t v_row, int64_t v_head, float scale, int causal, int dtype,
-                              void* stream) {
+                              void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace nvg;
     const char* op = "attention_prompt";
     clear_error();
-    int rc = check_dims(op, heads, kv_heads, head_dim, dtype);
+    int rc = check_prompt(op, batch, q_rows, k_rows, heads, kv_heads, head_dim, dtype);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "q", q_row, q_head);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "k", k_row, k_head);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "v", v_row, v_head);
     if (rc == NANOVLLM_GEMM_OK) rc = check_scale(op, scale);
     if (rc != NANOVLLM_GEMM_OK) return rc;
-    if (batch < 0 || q_rows < 0 || k_rows < 0 || batch >= INT32_MAX || q_rows > INT32_MAX / 2 || k_rows > INT32_MAX / 2)
-        return set_error(NANOVLLM_GEMM_EINVAL, "attention_prompt: batch and rows must be non-negative and below 2^30");
     if (q_rows == 0) return NANOVLLM_GEMM_OK;
     rc = k_rows > 0 ? check_pointers(op, {q, k, v, out}, {cu_q, cu_k}) : check_pointers(op, {q, out}, {cu_q, cu_k});
     if (rc != NANOVLLM_GEMM_OK) return rc;
+    const int64_t need = attention_prompt_workspace(batch, q_rows, k_rows, heads, head_dim);
+    if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+        return set_error(NANOVLLM_GEMM_EINVAL, "attention_prompt: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
+                         (long long)need, (long long)workspace_bytes);
     const PromptArgs p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                        static_cast<const uint16_t*>(v), cu_q, cu_k, static_cast<uint16_t*>(out), q_row, q_head, k_row,
                        k_head, v_row, v_head, static_cast<int32_t>(batch), static_cast<int32_t>(q_rows),
                        static_cast<int32_t>(k_rows), static_cast<int32_t>(heads), static_cast<int32_t>(kv_heads),
                        causal != 0, scale * kLog2e};
-    return launch_attention_prompt(p, static_cast<int>(head_dim), dtype, static_cast<hipStream_t>(stream));
+    return launch_attention_prompt(p, workspace, static_cast<int>(head_dim), dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t nanovllm_attention_prompt_workspace_bytes(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads,
+                                                  int64_t kv_heads, int64_t head_dim, int dtype) {
+    using namespace nvg;
+    clear_error();
+    const int rc = check_prompt("attention_prompt", batch, q_rows, k_rows, heads, kv_heads, head_dim, dtype);
+    if (rc != NANOVLLM_GEMM_OK || q_rows == 0) return rc;
+    return attention_prompt_workspace(batch, q_rows, k_rows, heads, head_dim);
 }
 
 int64_t nanovllm_attention_paged_workspace_bytes(const nanovllm_kv_cache* cache, int64_t batch, int64_t heads,

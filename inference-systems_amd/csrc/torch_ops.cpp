@@ -584,13 +584,17 @@ at::Tensor attention_prompt(const at::Tensor& q, const at::Tensor& k, const at::
     at::Tensor out = at::empty(q.sizes(), q.options());
     if (q.size(0) == 0) return out;
     const c10::DeviceGuard guard(q.device());
+    const int64_t need = nanovllm_attention_prompt_workspace_bytes(cu_q.size(0) - 1, q.size(0), k.size(0), q.size(1),
+                                                                   k.size(1), q.size(2), dtype_code(q.scalar_type()));
+    check_rc(need, "nanovllm_attention_prompt_workspace_bytes");
+    const at::Tensor ws = bytes_like(q, need > 0 ? need : 1);
     check_rc(nanovllm_attention_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                        static_cast<const int32_t*>(cu_q.data_ptr()),
                                        static_cast<const int32_t*>(cu_k.data_ptr()), out.data_ptr(),
                                        cu_q.size(0) - 1, q.size(0), k.size(0), q.size(1), k.size(1), q.size(2),
                                        stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1),
                                        stride_of(v, 0), stride_of(v, 1), static_cast<float>(scale), causal,
-                                       dtype_code(q.scalar_type()), stream_of(q)),
+                                       dtype_code(q.scalar_type()), ws.data_ptr(), need, stream_of(q)),
              "nanovllm_attention_prompt");
     return out;
 }

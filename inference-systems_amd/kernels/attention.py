@@ -368,11 +368,14 @@ def _attention_prompt_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     _refuse("attention_prompt", attention_prompt_contract_reason(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if q.shape[0]:
+        sizes = (cu_seqlens_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        need = _lib.attention_prompt_workspace_bytes(*sizes, _CODE[q.dtype])
+        _lib.check(need if need < 0 else _lib.OK, "nanovllm_attention_prompt_workspace_bytes")
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         with torch.cuda.device(q.device):
             _lib.attention_prompt_raw(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(),
-                                      cu_seqlens_k.data_ptr(), out.data_ptr(), cu_seqlens_q.shape[0] - 1, q.shape[0],
-                                      k.shape[0], q.shape[1], k.shape[1], q.shape[2], *_strides(q), *_strides(k),
-                                      *_strides(v), float(scale), causal, _CODE[q.dtype],
+                                      cu_seqlens_k.data_ptr(), out.data_ptr(), *sizes, *_strides(q), *_strides(k),
+                                      *_strides(v), float(scale), causal, _CODE[q.dtype], workspace.data_ptr(), need,
                                       torch.cuda.current_stream(q.device).cuda_stream)
     return out
 

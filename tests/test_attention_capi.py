@@ -37,7 +37,8 @@ def _append(cache=None, **changes):
 
 def _prompt(**changes):
     a = dict(q=P, k=P, v=P, cu_q=P, cu_k=P, out=P, batch=1, q_rows=3, k_rows=3, heads=4, kv_heads=2, head_dim=128,
-             q_row=512, q_head=128, k_row=256, k_head=128, v_row=256, v_head=128, scale=0.1, causal=1, dtype=L.BF16)
+             q_row=512, q_head=128, k_row=256, k_head=128, v_row=256, v_head=128, scale=0.1, causal=1, dtype=L.BF16,
+             workspace=P, workspace_bytes=1 << 30)
     a.update(changes)
     return L.load().nanovllm_attention_prompt(*a.values(), None)
 
@@ -113,7 +114,8 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_prompt, dict(scale=-1.0), L.EINVAL, "scale"),
     (_prompt, dict(batch=-1), L.EINVAL, "batch"),
     (_prompt, dict(q_rows=2 ** 31), L.EINVAL, "rows"),
-    (_prompt, dict(q_rows=2 ** 29, heads=1024), L.EINVAL, "too many"),
+    (_prompt, dict(workspace=None), L.EINVAL, "workspace"),
+    (_prompt, dict(workspace_bytes=100), L.EINVAL, "workspace"),
     (_prompt, dict(k=None), L.EINVAL, "non-null"),
     (_prompt, dict(k_row=3), L.EINVAL, "strides of k"),
     (_prompt, dict(q_rows=0, q=None, out=None), L.OK, ""),
@@ -149,6 +151,17 @@ def test_paged_workspace(lib):
     assert need(_cache(), 1000, 4, 1000) == need(_cache(), 4000, 4, 9000)
     assert need(_cache(bits=4), 1, 4, 16) == one
     assert need(_cache(head_dim=96), 1, 4, 16) == L.EUNSUPPORTED and "head_dim" in L.last_error()
+
+
+def test_prompt_workspace(lib):
+    need = L.attention_prompt_workspace_bytes
+    assert need(1, 0, 0, 4, 2, 128, L.BF16) == 0
+    small = need(1, 5, 5, 1, 1, 128, L.BF16)
+    assert 0 < small < need(1, 500, 500, 4, 2, 128, L.BF16)
+    # Bounded by the grid, whatever the keys; none where every workgroup has a block of its own.
+    assert need(1, 512, 10 ** 4, 32, 8, 128, L.BF16) == need(1, 600, 10 ** 9, 32, 8, 128, L.BF16) < 1 << 27
+    assert need(9, 10 ** 7, 10 ** 9, 64, 8, 128, L.BF16) == 0
+    assert need(1, 5, 5, 3, 2, 128, L.BF16) == L.EINVAL and "multiple" in L.last_error()
 
 
 CHILD = r"""
