@@ -365,28 +365,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
         float m = -__builtin_inff(), l = 0.0f;
         uint32_t late = 0;      // masked tiles (3 at most) with values that add_keys adds
 
-        // S^T of tile t, in KS steps; reads run two steps ahead of the products, and
-        // `beside(i)` is what the vector units do in step i.  Steps are kept
-        // apart: the compiler would otherwise issue one kind of work at a time.
+        // S^T of tile t.  A product occupies the matrix cores for 32 cycles, in which
+        // the wave issues other work only if it stands between two products:
+        // LDS reads, two steps ahead, and `beside(j)`, j of KS * NB.  The compiler,
+        // which would issue one kind of work at a time, is kept to that order.
         auto scores = [&](int t, f32x16_t (&sc)[NB], auto&& beside) {
             const uint32_t k_at = k_read + (t & 1) * TILE;
             u32x4_t kf[3][NB];
-            auto read = [&](int i) {
+            auto read = [&](int i, int n) { kf[i % 3][n] = *(lds_u4)(uintptr_t)((k_at ^ (32 * i)) + 32 * n * PITCH); };
 #pragma unroll
-                for (int n = 0; n < NB; ++n) kf[i % 3][n] = *(lds_u4)(uintptr_t)((k_at ^ (32 * i)) + 32 * n * PITCH);
-            };
-            read(0);
-            read(1);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) read(i, n);
 #pragma unroll
             for (int n = 0; n < NB; ++n) sc[n] = f32x16_t{};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                if (i + 2 < KS) read(i + 2);
+            for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) sc[n] = mfma_32x32x16<DT>(kf[i % 3][n], q[i], sc[n]);
-                beside(i);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                for (int n = 0; n < NB; ++n) {
+                    sc[n] = mfma_32x32x16<DT>(kf[i % 3][n], q[i], sc[n]);
+                    if (i + 2 < KS) read(i + 2, n);
+                    beside(i * NB + n);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         };
         // P of two scores, packed, and its sum; `pair` of NB * 8.
         u32x4_t pk[NB][2];
@@ -398,8 +399,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
             l = dot2<DT>(two, DT == NANOVLLM_GEMM_BF16 ? 0x3f803f80u : 0x3c003c00u, l);
         };
 
-        // Tile t, whose scores are in sc; those of the next tile, which only need
-        // the matrix cores, are computed while this one's softmax runs.
+        // The largest of the scores so far: 32 of them in `steps` steps.
+        float top = -__builtin_inff();
+        auto look = [&](const f32x16_t (&sc)[NB], int step, int steps) {
+#pragma unroll
+            for (int v = step * NB * 16 / steps; v < (step + 1) * NB * 16 / steps; ++v)
+                top = fmaxf(v == 0 ? -__builtin_inff() : top, sc[v / 16][v % 16]);
+        };
+
+        // Tile t, whose scores are in sc and the largest in top; those of the next
+        // tile are computed while this one's softmax runs, and looked through
+        // during its products with the values.
         auto tile = [&](int t, f32x16_t (&sc)[NB], f32x16_t (&ahead_sc)[NB]) {
             const bool masked = t >= full, more = t + 1 < t1;
             wait_vmcnt<0>();      // keys of tile t + 1 and values of t
@@ -435,12 +445,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                     }
                     __syncthreads();
                 }
+                look(sc, 0, 1);
             }
-            float top = sc[0][0];
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[n][v]);
             top = max_across32(top);
             // A first score (m is -infinity), or one that outgrows the range P has been given.
             if (__ballot((top - m) * p.c > kLazy)) {
@@ -452,47 +458,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                 for (int i = 0; i < DTILES; ++i) o[i] *= down;
             }
             const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
+            const uint32_t v_at = v_read + (t & 1) * TILE;
+            u32x4_t vf[2][DTILES];      // values of 16 keys, and of the next 16
+            auto read = [&](int g, int i) {
+                const uint32_t at = (v_at ^ (64 * i)) + 16 * g * PITCH;
+                const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)at);
+                const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)(at + 8 * PITCH));
+                const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+                vf[g % 2][i] = u32x4_t{l2[0], l2[1], h2[0], h2[1]};
+            };
+            constexpr int STEPS = KS * NB;
             if (more) {
-                scores(t + 1, ahead_sc, [&](int i) {
+                scores(t + 1, ahead_sc, [&](int j) {
 #pragma unroll
-                    for (int w = i * NB * 8 / KS; w < (i + 1) * NB * 8 / KS; ++w) weigh(sc, w, shift);
+                    for (int w = j * NB * 8 / STEPS; w < (j + 1) * NB * 8 / STEPS; ++w) weigh(sc, w, shift);
+                    if (j >= STEPS - DTILES) read(0, j - (STEPS - DTILES));
                 });
             } else {
                 // (Hidden, or the compiler would move what both branches share ahead of them.)
                 float alone = shift;
                 asm volatile("" : "+v"(alone));
 #pragma unroll
+                for (int i = 0; i < DTILES; ++i) read(0, i);
+#pragma unroll
                 for (int w = 0; w < NB * 8; ++w) weigh(sc, w, alone);
             }
-            // Products of 16 keys at a time, the next 16 keys' values read meanwhile.
-            const uint32_t v_at = v_read + (t & 1) * TILE;
-            u32x4_t vf[2][DTILES];
-            auto read = [&](int g) {
+#pragma unroll
+            for (int g = 0; g < 2 * NB; ++g)
 #pragma unroll
                 for (int i = 0; i < DTILES; ++i) {
-                    const uint32_t at = (v_at ^ (64 * i)) + 16 * g * PITCH;
-                    const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)at);
-                    const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(uintptr_t)(at + 8 * PITCH));
-                    const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-                    vf[g % 2][i] = u32x4_t{l2[0], l2[1], h2[0], h2[1]};
+                    o[i] = mfma_32x32x16<DT>(vf[g % 2][i], pk[g / 2][g % 2], o[i]);
+                    if (g + 1 < 2 * NB) read(g + 1, i);
+                    look(ahead_sc, g * DTILES + i, 2 * NB * DTILES);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            };
-            read(0);
-#pragma unroll
-            for (int g = 0; g < 2 * NB; ++g) {
-                if (g + 1 < 2 * NB) read(g + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < DTILES; ++i) o[i] = mfma_32x32x16<DT>(vf[g % 2][i], pk[g / 2][g % 2], o[i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
         };
-        f32x16_t sc[2][NB];
+        f32x16_t sc[2][NB] = {};
         if (t0 < t1) {
             wait_vmcnt<0>();
             __syncthreads();
             if (t0 + 1 < t1) copy_k(t0 + 1);
             scores(t0, sc[0], [](int) {});
+            look(sc[0], 0, 1);
         }
         for (int t = t0; t < t1;) {
             tile(t, sc[0], sc[1]);
