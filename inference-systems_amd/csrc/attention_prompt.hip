@@ -83,22 +83,25 @@ __device__ __forceinline__ Sequence sequence(const PromptArgs& p, int b) {
     return s;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
-    return x;
+__device__ __forceinline__ int64_t uniform64(int64_t x, int lane) {
+    return int64_t(uint32_t(__builtin_amdgcn_readlane(int(x), lane))) |
+           int64_t(__builtin_amdgcn_readlane(int(x >> 32), lane)) << 32;
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-    return int64_t(uint32_t(uniform(int(x)))) | int64_t(uniform(int(x >> 32))) << 32;
-}
+// Units of 64 sequences from b0 on, and the sum up to each: a lane a sequence.
+struct Units { int64_t mine, sum; };
 
-// All units: every wave adds them up for itself, 64 sequences at a time.
-__device__ __forceinline__ int64_t all_units(const PromptArgs& p) {
+__device__ __forceinline__ Units units_from(const PromptArgs& p, int b0) {
     const int lane = threadIdx.x & 63;
-    int64_t mine = 0;
-    for (int b = lane; b <= p.batch; b += 64) mine += sequence(p, b).units();
-    return uniform64(wave_sum(mine)) * p.heads;
+    Units u;
+    u.mine = b0 + lane <= p.batch ? sequence(p, b0 + lane).units() : 0;
+    u.sum = u.mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t up = __shfl_up(u.sum, off);
+        if (lane >= off) u.sum += up;
+    }
+    return u;
 }
 
 // A block, and its first unit.
@@ -108,27 +111,31 @@ struct Block {
     int64_t first;
 };
 
+// Units of all sequences and heads; `u`: of the last 64 sequences.
+__device__ __forceinline__ int64_t all_units(const PromptArgs& p, Units& u) {
+    int64_t total = 0;
+    for (int b0 = 0; b0 <= p.batch; b0 += 64) {
+        u = units_from(p, b0);
+        total += uniform64(u.sum, 63);
+    }
+    return total * p.heads;
+}
+
 // The block that holds a unit below the total.
-__device__ __forceinline__ Block find_block(const PromptArgs& p, int64_t unit) {
+__device__ __forceinline__ Block find_block(const PromptArgs& p, Units u, int64_t unit) {
     const int lane = threadIdx.x & 63;
     int64_t base = 0;
     Block r{};
     for (int b0 = 0; b0 <= p.batch; b0 += 64) {
-        const int64_t u = b0 + lane <= p.batch ? sequence(p, b0 + lane).units() * p.heads : 0;
-        int64_t sum = u;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t up = __shfl_up(sum, off);
-            if (lane >= off) sum += up;
-        }
-        const uint64_t past = __ballot(base + sum > unit);
+        if (p.batch >= 64) u = units_from(p, b0);      // else all_units has left them
+        const uint64_t past = __ballot((base + u.sum) * p.heads > unit);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            r.b = uniform(b0 + at);
-            r.first = base + uniform64(__shfl(sum - u, at));
+            r.b = b0 + at;
+            r.first = (base + uniform64(u.sum - u.mine, at)) * p.heads;
             break;
         }
-        base += uniform64(__shfl(sum, 63));
+        base += uniform64(u.sum, 63);
     }
     r.s = sequence(p, r.b);
     const int64_t each = r.s.units();
@@ -143,7 +150,7 @@ __device__ __forceinline__ Block find_block(const PromptArgs& p, int64_t unit) {
         lo += at;
         n = min(step, n - at);
     }
-    r.index = uniform(lo);
+    r.index = lo;
     r.first += r.s.before(r.index);
     return r;
 }
@@ -186,8 +193,8 @@ __device__ __forceinline__ void advance(const PromptArgs& p, Block& r) {
     while (r.s.blocks == 0 && r.b < p.batch);
 }
 
-// The part of a block a workgroup leaves: rows of fp32 sums, then the rows'
-// maxima and totals of P.
+// The part of a block a workgroup leaves: fp32 sums as the waves' lanes hold
+// them, 16 bytes a lane, then the rows' maxima and totals of P.
 template <int D>
 __device__ __forceinline__ float* part(const Split& s, int slot) {
     return s.partial + int64_t(slot) * kRows * (D + 2);
@@ -280,11 +287,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     Block blk{};
     if (s.runs) {
         wg = xcd_remap(wg, s.grid);      // neighbouring runs share keys: they go to one XCD
-        const int64_t total = all_units(p), per = (total + s.grid - 1) / s.grid;
+        Units u;
+        const int64_t total = all_units(p, u), per = (total + s.grid - 1) / s.grid;
         unit = wg * per;
         end = unit + per < total ? unit + per : total;
         if (unit >= end) return;
-        blk = find_block(p, unit);
+        blk = find_block(p, u, unit);
     } else {
         if (!nth_block(p, wg / p.heads, blk)) return;
         blk.head = wg % p.heads;
@@ -518,9 +526,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
         const float inv = last < 0 ? 0.0f : 1.0f / l;     // no key: 0
         uint16_t* out = p.out + (int64_t(blk.s.q0 + row0 + mine) * p.heads + head) * D;
         float* slot = part<D>(s, 2 * wg + (t0 == 0 ? 1 : 0));
-        auto store = [&](int ch, f32x4_t x) {
+        const uint32_t slot_at = 4 * (64 * DTILES * 4 * wave + oc + 32 * half);
+        auto store = [&](int ch, f32x4_t x) {      // channels ch .. ch + 3
             if (!whole)
-                *reinterpret_cast<f32x4_t*>(slot + mine * D + ch) = x;
+                *reinterpret_cast<f32x4_t*>(slot + slot_at + 256 * (ch / 8)) = x;
             else if (row < lq)
                 *reinterpret_cast<u32x2_t*>(out + ch) =
                     u32x2_t{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
@@ -554,42 +563,53 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     }
 }
 
-// Joins the parts of the block that the start of run `blockIdx.x` cuts first:
-// 16 of its rows a workgroup, a row by D / 4 threads.  Parts are added in order.
-constexpr int kJoinRows = 16;
+// Joins the parts of the block that the start of run blockIdx.x + 1 cuts first:
+// a wave takes 32 rows and kJoin channels as the kernel's waves left them.  Parts
+// are added in order.
+constexpr int kJoin = 64;
 
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attention_prompt_join_kernel(const Split s) {
-    constexpr int TPR = D / 4;
     const PromptArgs& p = s.a;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
     const int wg = int(blockIdx.x) + 1;
-    const int64_t total = all_units(p), per = (total + s.grid - 1) / s.grid, unit = wg * per;
+    Units u;
+    const int64_t total = all_units(p, u), per = (total + s.grid - 1) / s.grid, unit = wg * per;
     if (unit >= total) return;
-    const Block blk = find_block(p, unit);
+    const Block blk = find_block(p, u, unit);
     const int64_t keys = blk.first + kBegin;      // the block's first unit with a key
     const int64_t behind = keys + max(1, blk.s.tiles(blk.index));
     if (unit <= keys || keys / per != wg - 1) return;
-    const int last_wg = int((behind - 1) / per);
-    const int lq = blk.s.lq, row0 = blk.index * kRows, ahead = p.causal ? blk.s.lk - lq : blk.s.lk;
-    for (int e = threadIdx.x; e < kJoinRows * TPR; e += 256) {
-        const int r = int(blockIdx.y) * kJoinRows + e / TPR, ch = 4 * (e % TPR), row = row0 + r;
-        if (row >= lq) continue;
-        float top = -__builtin_inff();
-        for (int w = wg - 1; w <= last_wg; ++w) top = fmaxf(top, part<D>(s, 2 * w + (w == wg - 1))[kRows * D + r]);
-        float l = 0.0f;
-        f32x4_t o = {0, 0, 0, 0};
-        for (int w = wg - 1; w <= last_wg; ++w) {
-            const float* src = part<D>(s, 2 * w + (w == wg - 1));
-            const float m = src[kRows * D + r];
-            // A part whose maximum is -infinity has nothing, or NaN.
-            const float f = m == -__builtin_inff() ? 1.0f : exp2_hw((m - top) * p.c);
-            l = __builtin_fmaf(f, src[kRows * D + kRows + r], l);
-            o += f * *reinterpret_cast<const f32x4_t*>(src + r * D + ch);
-        }
-        const float inv = (p.causal ? min(row + ahead, blk.s.lk - 1) : blk.s.lk - 1) < 0 ? 0.0f : 1.0f / l;
-        *reinterpret_cast<u32x2_t*>(p.out + (int64_t(blk.s.q0 + row) * p.heads + blk.head) * D + ch) =
-            u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+    const int first = wg - 1, last_wg = int((behind - 1) / per);
+    const int mine = 32 * wave + (lane & 31), row = blk.index * kRows + mine;
+    const int ahead = p.causal ? blk.s.lk - blk.s.lq : blk.s.lk;
+    const float* src0 = part<D>(s, 0);
+    auto source = [&](int w) { return src0 + int64_t(2 * w + (w == first)) * kRows * (D + 2); };
+    const uint32_t at = 4 * (64 * (D / 8) * wave + 64 * (kJoin / 8) * int(blockIdx.y) + lane);
+    float m = -__builtin_inff(), l = 0.0f;
+    f32x4_t o[kJoin / 8] = {};
+    for (int w = first; w <= last_wg; ++w) {
+        const float* src = source(w);
+        f32x4_t x[kJoin / 8];
+#pragma unroll
+        for (int i = 0; i < kJoin / 8; ++i) x[i] = *reinterpret_cast<const f32x4_t*>(src + at + 256 * i);
+        const float mw = src[kRows * D + mine], lw = src[kRows * D + kRows + mine];
+        // A part whose maximum is -infinity has nothing, or NaN.
+        const float top = fmaxf(m, mw);
+        const float f = mw == -__builtin_inff() ? 1.0f : exp2_hw((mw - top) * p.c);
+        const float down = m == -__builtin_inff() ? 1.0f : exp2_hw((m - top) * p.c);
+        m = top;
+        l = __builtin_fmaf(l, down, f * lw);
+#pragma unroll
+        for (int i = 0; i < kJoin / 8; ++i) o[i] = o[i] * down + x[i] * f;
     }
+    if (row >= blk.s.lq) return;
+    const float inv = (p.causal ? min(row + ahead, blk.s.lk - 1) : blk.s.lk - 1) < 0 ? 0.0f : 1.0f / l;
+    uint16_t* out = p.out + (int64_t(blk.s.q0 + row) * p.heads + blk.head) * D + kJoin * int(blockIdx.y) + 4 * half;
+#pragma unroll
+    for (int i = 0; i < kJoin / 8; ++i)
+        *reinterpret_cast<u32x2_t*>(out + 8 * i) =
+            u32x2_t{pack2<DT>(o[i][0] * inv, o[i][1] * inv), pack2<DT>(o[i][2] * inv, o[i][3] * inv)};
 }
 
 // Workgroups that the chip runs at once: two a CU, one of head_dim 256.
@@ -615,8 +635,7 @@ int launch(const Split& s, hipStream_t stream) {
     hipLaunchKernelGGL((attention_prompt_kernel<DT, D>), dim3(s.grid), dim3(256), 0, stream, s);
     int rc = check_launch("attention_prompt");
     if (rc != NANOVLLM_GEMM_OK || !s.runs || s.grid == 1) return rc;
-    hipLaunchKernelGGL((attention_prompt_join_kernel<DT, D>), dim3(s.grid - 1, kRows / kJoinRows), dim3(256), 0, stream,
-                       s);
+    hipLaunchKernelGGL((attention_prompt_join_kernel<DT, D>), dim3(s.grid - 1, D / kJoin), dim3(256), 0, stream, s);
     return check_launch("attention_prompt_join");
 }
 
