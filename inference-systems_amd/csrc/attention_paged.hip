@@ -67,17 +67,6 @@ __device__ __forceinline__ int units_of(int len, int cap) {
     return kBegin + max(1, (n + kUnit - 1) / kUnit);
 }
 
-// Sum over lanes 0 .. l of a wave.
-__device__ __forceinline__ int prefix_sum(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);    // 1, 2, 4, 8 lanes up in rows of 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);    // lane 15 of a row into the next
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);    // lane 31 into the upper half
-    return x;
-}
-
 // The units of all pairs, per sequence in a lane: every wave adds them up for
 // itself, 64 sequences at a time.
 struct Units { int total, len, mine, sum; };    // all of them; of sequence `lane` of the last 64: its length, units,

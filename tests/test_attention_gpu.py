@@ -187,6 +187,38 @@ def test_kv_gather(bits, size, dtype, dim, kv):
                 assert torch.equal(got[i, h].cpu(), w), (i, s, h)
 
 
+@pytest.mark.parametrize("bits,size", [(16, 23), (4, 48)])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim,tokens", [(64, 4500), (128, 2301), (256, 2070)])
+def test_rope_append_of_many_tokens(bits, size, dtype, dim, tokens):
+    """A call of prompts (several heads and rows of values to a team) writes bit for bit what calls of at most 50 tokens
+    write: sequences that begin at any slot of a page, rows that are kept nowhere, odd counts of heads."""
+    _say("many tokens", bits, size, dtype, dim, tokens)
+    gen, heads, kv = _gen(dim + bits), 10, 5
+    rows = torch.randn((tokens, heads + 2 * kv, dim), generator=gen).to(dtype).to(DEV)
+    q, k, v = rows.split([heads, kv, kv], 1)
+    table = K.rope_table(1000, 32, device=DEV)
+    positions = torch.randint(0, 1000, (tokens,), generator=gen).to(DEV)
+    blocks = tokens // size + 20
+    slots = torch.arange(tokens) + torch.repeat_interleave(torch.randint(0, 7, (tokens // 90 + 1,), generator=gen).cumsum(0),
+                                                           90)[:tokens]
+    slots[500:530] = slots[500:530].flip(0)
+    slots[torch.randint(0, tokens, (9,), generator=gen)] = -1
+    assert int(slots.max()) < blocks * size
+    slots = slots.to(torch.int32).to(DEV)
+    whole = _noisy_cache(blocks, size, kv, dim, bits, dtype, gen)
+    parts = K.KVCache(*[None if x is None else x.clone() for x in whole])
+    outs = K.rope_append(q, k, v, positions, table, slots, *whole)
+    at = 0
+    while at < tokens:
+        n = at + int(torch.randint(1, 51, (1,), generator=gen))
+        piece = K.rope_append(q[at:n], k[at:n], v[at:n], positions[at:n], table, slots[at:n], *parts)
+        assert all(torch.equal(a[at:n], b) for a, b in zip(outs, piece)), at
+        at = n
+    for a, b in zip(whole, parts):
+        assert a is b is None or torch.equal(_bits(a), _bits(b))
+
+
 def test_appended_rows_read_back():
     """A cache written in pieces reads back as written at once, through blocks that are slices of a larger allocation."""
     _say("read back")
@@ -319,6 +351,58 @@ def test_attention_prompt_many_sequences():
     q, k, v = (torch.randn((sum(lens), h, 64), generator=gen).to(BF16).to(DEV) for h in (4, 2, 2))
     got = K.attention_prompt(q, k, v, _cu(lens), _cu(lens), 0.125)
     _check_prompt(got, q, k, v, lens, lens, 0.125, True, "many")
+
+
+@pytest.mark.parametrize("dim,heads,kv,lq,lk", [(64, 2, 1, 130, 5000), (128, 3, 3, 515, 2500), (256, 2, 2, 300, 3400)])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_attention_prompt_long_keys(dim, heads, kv, lq, lk, causal):
+    """Few blocks of queries against many keys: a block's keys are taken by many workgroups and joined."""
+    _say("long keys", dim, lq, lk, causal)
+    gen = _gen(lk)
+    q, k, v = (torch.randn((n, h, dim), generator=gen).to(BF16).to(DEV) for n, h in ((lq, heads), (lk, kv), (lk, kv)))
+    got = K.attention_prompt(q, k, v, _cu([lq]), _cu([lk]), dim ** -0.5, causal)
+    _check_prompt(got, q, k, v, [lq], [lk], dim ** -0.5, causal, "long keys")
+
+
+# Enough blocks that each has a workgroup of its own.
+MANY = [(64, 4, 2, 400), (128, 4, 1, 400), (256, 2, 2, 400)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim,heads,kv,count", MANY)
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_attention_prompt_many_blocks(dtype, dim, heads, kv, count, causal):
+    _say("many blocks", dtype, dim, causal)
+    gen = _gen(dim + count)
+    lq = torch.randint(0, 7, (count,), generator=gen).tolist()
+    lk = [n + int(x) for n, x in zip(lq, torch.randint(0, 9, (count,), generator=gen))]
+    lq[10], lk[10], lq[200], lk[200], lq[399], lk[399] = 300, 300, 140, 700, 150, 70
+    q, k, v = (torch.randn((sum(n), h, dim), generator=gen).to(dtype).to(DEV) for n, h in ((lq, heads), (lk, kv), (lk, kv)))
+    spare = torch.ones((200, heads, dim), dtype=dtype, device=DEV)      # rows behind the last sequence
+    got = K.attention_prompt(torch.cat((q, spare)), k, v, _cu(lq), _cu(lk), dim ** -0.5, causal)
+    assert not got[sum(lq):].any()
+    _check_prompt(got, q, k, v, lq, lk, dim ** -0.5, causal, "many blocks")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim,heads,kv,count", MANY)
+def test_attention_prompt_many_blocks_keep_to_what_a_row_sees(dtype, dim, heads, kv, count):
+    """As test_attention_prompt_keeps_to_what_a_row_sees, a workgroup a block."""
+    _say("many blocks, masked places", dtype, dim)
+    gen = _gen(dim)
+    lens = [70, 45] + [1] * count
+    n = sum(lens)
+    q, k, v = (torch.randn((n, h, dim), generator=gen).to(dtype) for h in (heads, kv, kv))
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_v[30, 0, 3], bad_v[90], bad_k[60], bad_v[200], bad_k[201] = torch.nan, -torch.inf, torch.nan, torch.inf, torch.nan
+    got, want = (K.attention_prompt(q.to(DEV), a.to(DEV), b.to(DEV), _cu(lens), _cu(lens), dim ** -0.5).cpu()
+                 for a, b in ((bad_k, bad_v), (k, v)))
+    assert not torch.isnan(want).any()
+    same = torch.ones(n, heads, dim, dtype=torch.bool)
+    same[30:70, :heads // kv, 3] = same[60:70] = same[90:115] = same[200:202] = False
+    assert torch.equal(got[same], want[same])
+    assert torch.isnan(got[30:70, :heads // kv, 3]).all() and torch.isnan(got[60:70]).all()
+    assert (got[90:115] == -torch.inf).all() and (got[200] == torch.inf).all() and torch.isnan(got[201]).all()
 
 
 # ---------------------------------------------------------------------------
@@ -497,6 +581,29 @@ def test_graph_replays_follow_their_inputs():
         torch.cuda.synchronize()
         assert torch.equal(outs[i % 2], want), i
         assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(cache, twin)), i
+
+
+@pytest.mark.parametrize("heads,batch", [(4, 3), (8, 250)])
+def test_prompt_graph_replays_follow_their_offsets(heads, batch):
+    """attention_prompt captured once (equal runs of keys; a workgroup a block) and replayed with other rows and
+    offsets, eager calls in between, as it answers eagerly."""
+    _say("prompt graph", heads, batch)
+    gen, rows, dim = _gen(batch), 900, 128
+    q, k, v = (torch.zeros((rows, h, dim), dtype=BF16, device=DEV) for h in (heads, 2, 2))
+    cu = torch.zeros(batch + 1, dtype=torch.int32, device=DEV)
+    K.attention_prompt(q, k, v, cu, cu, 0.09)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.attention_prompt(q, k, v, cu, cu, 0.09)
+    for i in range(5):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=gen).to(BF16))
+        cu[1:].copy_(torch.randint(0, rows + 1, (batch,), generator=gen).sort().values.to(torch.int32))
+        want = K.attention_prompt(q, k, v, cu, cu, 0.09)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
 
 
 def test_calls_on_another_stream():
