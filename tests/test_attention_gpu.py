@@ -496,6 +496,18 @@ def test_attention_paged_long_and_many(bits):
     _check_paged(got, q, cache, slots, lens, 0.125, "long")
 
 
+@pytest.mark.parametrize("dim,kv", [(64, 16), (128, 8), (256, 8)])
+def test_attention_paged_more_work_than_the_chip_holds(dim, kv):
+    """16-bit pages, units enough that half of the workgroups take them all."""
+    _say("paged much", dim)
+    gen = _gen(dim)
+    lens = [900, 0, 1, 128, 129] + torch.randint(1, 900, (20,), generator=gen).tolist()
+    assert kv * sum(3 + max(1, -(-n // 128)) for n in lens) >= 2 * (1024 if dim == 64 else 512)
+    q, cache, tables, slots = _paged_case(lens, 16, 2 * kv, kv, dim, 16, BF16, gen)
+    got = K.attention_paged(q, cache.k, cache.v, tables, _i32(lens), dim ** -0.5)
+    _check_paged(got, q, cache, slots, lens, dim ** -0.5, "much")
+
+
 @pytest.mark.parametrize("magnitude", [1e-3, 300.0, 20000.0])
 def test_attention_paged_4bit_values_of_every_size(magnitude):
     """Scales for which the probabilities keep their factor of 2^10, and larger ones for which they cannot."""
