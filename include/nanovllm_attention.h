@@ -25,8 +25,9 @@ extern "C" {
 
 /*
  * A paged cache of keys and values.  Slot s is row s % block_size of page
- * s / block_size.  Strides between pages are in bytes, a multiple of 16;
- * pointers are 16-byte aligned; head_dim is 64, 128 or 256.
+ * s / block_size; there are fewer than 2^31.  Strides between pages are in
+ * bytes, a multiple of 16 below 64 GiB, pages smaller than 2 GiB; pointers are
+ * 16-byte aligned; head_dim is 64, 128 or 256.
  *
  * bits == 16: a page of k, and of v, is [block_size, kv_heads, head_dim]
  * elements of dtype (the layout of store_kvcache); the scales are null.
@@ -67,7 +68,7 @@ typedef struct nanovllm_kv_cache {
  * Rotates queries and keys and appends keys and values to the cache.  q is
  * [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim], of dtype,
  * element (t, h, c) at t * row stride + h * head stride + c (strides in
- * elements, multiples of 8).  With x1, x2 the two halves of the first
+ * elements, multiples of 8, that of rows below 2^24).  With x1, x2 the two halves of the first
  * `rotary` channels (a multiple of 16, at most head_dim),
  *     y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin,
  * in fp32, rounded once; the other channels stay.  Row p of cos_sin
@@ -101,13 +102,14 @@ int nanovllm_kv_gather(const nanovllm_kv_cache* cache, const int32_t* slots, int
 /*
  * Attention of packed sequences, heads in groups of heads / kv_heads that
  * share keys and values.  Sequence b holds queries cu_q[b] .. cu_q[b + 1] and
- * keys cu_k[b] .. cu_k[b + 1] (batch + 1 offsets each, not decreasing); its row
- * i attends to key j where causal is 0 or j <= i + (keys - queries), so the last
- * query sees every key.  out = softmax(scale q k^T) v, fp32 sums, rounded once;
- * a row with no key to attend to is 0, and so are rows behind the last
- * sequence.  q, k, v as in nanovllm_rope_append; out is [q_rows, heads,
- * head_dim], contiguous.  Workspace: nanovllm_attention_prompt_workspace_bytes()
- * bytes, 16-byte aligned scratch.
+ * keys cu_k[b] .. cu_k[b + 1] (batch + 1 offsets each, not decreasing, the
+ * first of cu_q 0); its row i attends to key j where causal is 0 or
+ * j <= i + (keys - queries), so the last query sees every key.
+ * out = softmax(scale q k^T) v, fp32 sums, rounded once; a row with no key to
+ * attend to is 0, and so are rows behind the last sequence.  q, k, v as in
+ * nanovllm_rope_append; out is [q_rows, heads, head_dim], contiguous.
+ * Workspace: nanovllm_attention_prompt_workspace_bytes() bytes, 16-byte
+ * aligned scratch.
  */
 int nanovllm_attention_prompt(const void* q, const void* k, const void* v,
                               const int32_t* cu_q, const int32_t* cu_k, void* out,

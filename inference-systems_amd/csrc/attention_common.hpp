@@ -16,6 +16,8 @@ struct Cache {
     int32_t num_blocks, block_size, kv_heads;
 };
 
+// A launch has fewer than 2^32 threads, here of 256 a workgroup.
+constexpr int64_t kMostGroups = (int64_t(1) << 24) - 1;
 constexpr int kGroup = 64;   // channels that share a 4-bit scale and minimum
 
 struct AppendArgs {

@@ -120,9 +120,9 @@ int check_paged(const char* op, const nanovllm_kv_cache* cache, int64_t batch, i
     if (!fits32(batch) || !fits32(table_blocks) || !fits32(table_blocks * cache->block_size))
         return set_error(NANOVLLM_GEMM_EINVAL, "%s: batch and table must be non-negative and hold fewer than 2^31 tokens",
                          op);
-    // Units of 128 tokens, and workgroups of the join, are counted in 32 bits.
+    // Units of 128 tokens are counted in 32 bits; the join has a workgroup or more for each pair.
     const int64_t blocks = cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
-    if (!fits32(batch * blocks) || !fits32(batch * blocks * (table_blocks * cache->block_size / 128 + 8)))
+    if (batch * blocks > kMostGroups || !fits32(batch * blocks * (table_blocks * cache->block_size / 128 + 8)))
         return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: batch, heads and table are too large", op);
     return NANOVLLM_GEMM_OK;
 }

@@ -363,7 +363,9 @@ int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, h
         sp.v_rows = int64_t(p.tokens) * kvh >= 64 * kFull / 8 ? 64 : teams;
         sp.v_groups = (p.tokens + sp.v_rows - 1) / sp.v_rows * kvh;
     }
-    const dim3 grid(static_cast<uint32_t>(runs * sp.parts + sp.v_groups));
+    const int64_t groups = runs * sp.parts + sp.v_groups;
+    if (groups > kMostGroups) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "rope_append: too many tokens and heads");
+    const dim3 grid(static_cast<uint32_t>(groups));
     return pick(dtype, head_dim, bits, [&](auto dt, auto d, auto b) {
         if (each == 4)
             hipLaunchKernelGGL((rope_append_kernel<dt.value, d.value, b.value, 4>), grid, dim3(kThreads), 0, s, sp);
@@ -375,7 +377,9 @@ int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, h
 
 int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s) {
     const int64_t rows = int64_t(p.rows) * 2 * p.cache.kv_heads, per = kThreads / (head_dim / 8);
-    const dim3 grid(static_cast<uint32_t>((rows + per - 1) / per));
+    const int64_t groups = (rows + per - 1) / per;
+    if (groups > kMostGroups) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "kv_gather: too many rows and heads");
+    const dim3 grid(static_cast<uint32_t>(groups));
     return pick(dtype, head_dim, bits, [&](auto dt, auto d, auto b) {
         hipLaunchKernelGGL((kv_gather_kernel<dt.value, d.value, b.value>), grid, dim3(kThreads), 0, s, p);
         return check_launch("kv_gather");

@@ -19,7 +19,8 @@ nanovllm/layers/attention.py, nanovllm/layers/rotary_embedding.py).
 
     attention_prompt(q[Tq, H, D], k[Tk, KV, D], v, cu_seqlens_q, cu_seqlens_k,
                      scale, causal=True) -> out[Tq, H, D]
-        Attention of packed sequences; query i of a sequence sees keys up to
+        Attention of packed sequences: int32 offsets of their rows, from 0 and
+        not decreasing.  Query i of a sequence sees keys up to
         i + (its keys - its queries).  A row with no key to see is 0, and so
         are rows behind the last sequence.
 
@@ -32,7 +33,8 @@ nanovllm/layers/attention.py, nanovllm/layers/rotary_embedding.py).
 
 Types: float16 or bfloat16, D of 64, 128 or 256, H a multiple of KV.  q, k and
 v may be strided views (a column range of one projection) with unit stride in
-the last dimension.  ``positions`` is int64, the other index tensors int32,
+the last dimension, and strides that are multiples of 8, that of rows below
+2^24.  ``positions`` is int64, the other index tensors int32,
 ``cos_sin`` float32.
 
 A paged cache (``new_kv_cache``) holds 16-bit elements, [blocks, block_size,

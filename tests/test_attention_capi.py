@@ -69,6 +69,8 @@ BAD_CACHES = [
     (dict(k_stride=16 * 2 * 128 * 2 - 16), L.EINVAL, "strides"),
     (dict(v_stride=16 * 2 * 128 * 2 + 8), L.EINVAL, "strides"),
     (dict(bits=4, v_scales_stride=0), L.EINVAL, "strides"),
+    (dict(k_stride=2 ** 36), L.EUNSUPPORTED, "64 GiB"),
+    (dict(bits=4, v_scales_stride=2 ** 40), L.EUNSUPPORTED, "64 GiB"),
     (dict(k=None), L.EINVAL, "non-null"),
     (dict(v=P + 8), L.EINVAL, "16-byte aligned"),
     (dict(bits=4, k_scales=None), L.EINVAL, "non-null"),
@@ -92,6 +94,8 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_append, dict(q_row=4), L.EINVAL, "strides of q"),
     (_append, dict(k_head=-8), L.EINVAL, "strides of k"),
     (_append, dict(v_row=12), L.EINVAL, "strides of v"),
+    (_append, dict(q_row=2 ** 24), L.EUNSUPPORTED, "2^24"),
+    (_append, dict(tokens=2 ** 27), L.EUNSUPPORTED, "too many"),
     (_append, dict(rotary=0), L.EINVAL, "rotary"),
     (_append, dict(rotary=24), L.EINVAL, "rotary"),
     (_append, dict(rotary=144), L.EINVAL, "rotary"),
@@ -101,6 +105,7 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_append, dict(tokens=0, q=None), L.OK, ""),
     (_gather, dict(rows=-1), L.EINVAL, "rows"),
     (_gather, dict(rows=2 ** 30), L.EINVAL, "2^31"),
+    (_gather, dict(rows=2 ** 28), L.EUNSUPPORTED, "too many"),
     (_gather, dict(dtype=L.F16), L.EUNSUPPORTED, "own dtype"),
     (_gather, dict(slots=None), L.EINVAL, "non-null"),
     (_gather, dict(rows=0, k_out=None), L.OK, ""),
@@ -116,6 +121,8 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_prompt, dict(q_rows=2 ** 31), L.EINVAL, "rows"),
     (_prompt, dict(workspace=None), L.EINVAL, "workspace"),
     (_prompt, dict(workspace_bytes=100), L.EINVAL, "workspace"),
+    (_prompt, dict(k_row=2 ** 24), L.EUNSUPPORTED, "2^24"),
+    (_prompt, dict(batch=2 ** 22), L.EUNSUPPORTED, "too many"),
     (_prompt, dict(k=None), L.EINVAL, "non-null"),
     (_prompt, dict(k_row=3), L.EINVAL, "strides of k"),
     (_prompt, dict(q_rows=0, q=None, out=None), L.OK, ""),
@@ -123,6 +130,7 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_paged, dict(batch=-1), L.EINVAL, "batch"),
     (_paged, dict(batch=2 ** 31), L.EINVAL, "batch"),
     (_paged, dict(table_blocks=2 ** 28), L.EINVAL, "2^31"),
+    (_paged, dict(batch=2 ** 23, table_blocks=1, table_stride=1), L.EUNSUPPORTED, "too large"),
     (_paged, dict(batch=2 ** 20, table_blocks=2 ** 20, table_stride=2 ** 20), L.EUNSUPPORTED, "too large"),
     (_paged, dict(table_stride=19), L.EINVAL, "table_stride"),
     (_paged, dict(workspace=None), L.EINVAL, "workspace"),
