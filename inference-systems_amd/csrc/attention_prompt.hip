@@ -19,6 +19,12 @@
 // queries against many keys, and sequences of any lengths load the chip evenly.
 // A block whose keys lie in one run is finished there; the parts of others go
 // to a workspace (at most two per workgroup) and a second kernel joins them.
+//
+// Bound by the matrix cores, which run at the chip's power limit: on MI355X 16384
+// tokens of 8 heads of 256 take 1121-1145 us, 960-980 TFLOP/s (a large library
+// product 1265; the products alone 807 us); a chunk of 512 behind 8188 cached
+// tokens, 32 heads of 128, 85-88 us, 12 of them in the join; 2048 tokens of 8
+// heads of 256 48 us, 18 of them for the traffic of 35 MB of parts.
 #include <type_traits>
 
 #include "attention_common.hpp"
