@@ -7,8 +7,10 @@
 // neighbouring lanes.  Measured on MI355X (a large copy: 5.1 TB/s): 8000 tokens
 // of 16 + 2 x 4 heads of 128 into a 4-bit cache 23 us for 101 MB, 4.4 TB/s (a row
 // a team, with its own cosines and divisions: 49 us); 20000 tokens of 8 + 2 x 2
-// heads of 256, 16 bits, 45 us; one token 2.6 us.  20000 rows of 4 + 4 heads of
-// 128 gathered from 16-bit pages 13 us, partly from the last-level cache.
+// heads of 256, 16 bits, 45 us; one token 2.6 us.  Rows of 4 + 4 heads of 128
+// gathered: 20000 from 16-bit pages 13 us, partly from the last-level cache, 8000
+// and 20000 from 4-bit ones 6.6 and 13.2 us (values by a team a row, three of four
+// of them idle: 9.2 and 19.1 us).
 #include <type_traits>
 
 #include "attention_common.hpp"
@@ -145,22 +147,29 @@ struct AppendSplit {
     int32_t v_groups;       // 4 bits: workgroups of values
 };
 
-// 4-bit values of up to 64 rows of one head.  Lane l of every wave looks at row
-// l; the rows that have a share are then listed, so that no team waits for
-// those that another takes with its own.
+// Rows first .. first + n - 1 (64 at most) that have a share of the values: how
+// many, and in lane i of every wave the i-th of them and its share << 8.  Lane l
+// looks at row l.  So no team waits for rows that another takes with its own.
+__device__ __forceinline__ int list_shares(const int32_t* slots, int first, int n, int rows, int most, int& listed) {
+    const int lane = threadIdx.x & 63;
+    int share = 0;
+    if (lane < n) {
+        const int slot = slots[first + lane];
+        if (slot >= 0 && slot < most) share = row_share(slots, first + lane, rows, slot);
+    }
+    const uint64_t taken = __ballot(share != 0);
+    const int count = __popcll(taken), rank = __popcll(taken & ((uint64_t(1) << lane) - 1));
+    listed = __builtin_amdgcn_ds_permute(4 * (share != 0 ? rank : count + lane - rank), lane | share << 8);
+    return count;
+}
+
+// 4-bit values of up to 64 rows of one head.
 template <int DT, int D>
 __device__ __forceinline__ void append_values(const AppendArgs& p, int first, int rows, int h) {
     constexpr int CH = D / 8, GROUPS = D / kGroup, TEAMS = kThreads / CH;
-    const int c = threadIdx.x % CH, g = c / 8, lane = threadIdx.x & 63;
-    rows = min(rows, p.tokens - first);
-    int share = 0;
-    if (lane < rows) {
-        const int slot = p.slots[first + lane];
-        if (slot >= 0 && slot < p.cache.slots) share = row_share(p.slots, first + lane, p.tokens, slot);
-    }
-    const uint64_t taken = __ballot(share != 0), below = taken & ((uint64_t(1) << lane) - 1);
-    const int count = __popcll(taken), rank = __popcll(below);
-    const int listed = __builtin_amdgcn_ds_permute(4 * (share != 0 ? rank : count + lane - rank), lane | share << 8);
+    const int c = threadIdx.x % CH, g = c / 8;
+    int listed;
+    const int count = list_shares(p.slots, first, min(rows, p.tokens - first), p.tokens, p.cache.slots, listed);
     for (int i = threadIdx.x / CH; i - int(threadIdx.x / CH) < count; i += TEAMS) {      // all lanes stay for the shuffles
         const int what = __shfl(listed, min(i, count - 1));
         const int t = first + (what & 255), four = (what >> 8) == 4;
@@ -279,14 +288,64 @@ __device__ __forceinline__ u32x4_t dequantise8(uint32_t scale, F&& code) {
     return narrow8<DT>(f);
 }
 
+// 4-bit values of up to 64 rows of one head, and zeros for those outside the cache.
+template <int DT, int D>
+__device__ __forceinline__ void gather_values(const GatherArgs& p, int first, int rows, int h) {
+    constexpr int CH = D / 8, GROUPS = D / kGroup, TEAMS = kThreads / CH;
+    const int c = threadIdx.x % CH, g = c / 8, team = threadIdx.x / CH, kvh = p.cache.kv_heads;
+    rows = min(rows, p.rows - first);
+    auto out = [&](int n) { return reinterpret_cast<u32x4_t*>(p.v_out + (int64_t(n) * kvh + h) * D + 8 * c); };
+    int listed;
+    const int count = list_shares(p.slots, first, rows, p.rows, p.cache.slots, listed);
+    for (int i = team; i - team < count; i += TEAMS) {      // all lanes stay for the shuffle
+        const int what = __shfl(listed, min(i, count - 1));
+        if (i >= count) continue;
+        const int n = first + (what & 255), slot = p.slots[n];
+        const uint32_t page = uint32_t(slot) / uint32_t(p.cache.block_size), at = slot - page * p.cache.block_size;
+        const char* words = p.cache.v + page * p.cache.v_stride +
+                            (int64_t(h) * p.cache.block_size + (at & ~3u)) * (D / 2);
+        const char* scales = p.cache.v_scales + page * p.cache.vs_stride +
+                             4 * ((int64_t(h) * GROUPS + g) * p.cache.block_size + at);
+        u32x2_t w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            w[e] = *reinterpret_cast<const u32x2_t*>(words + 4 * word_place<GROUPS, 32>(g, 4 * (c % 8) + 2 * e));
+        auto token = [&](uint32_t scale, int j) {
+            return dequantise8<DT>(scale, [&](int x) { return (w[x / 4][(x / 2) % 2] >> (8 * j + 4 * (x % 2))) & 15u; });
+        };
+        if ((what >> 8) == 4) {
+            const u32x4_t sc = load16(scales);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *out(n + j) = token(sc[j], j);
+        } else {
+            *out(n) = token(*reinterpret_cast<const uint32_t*>(scales), at & 3);
+        }
+    }
+    for (int i = team; i < rows; i += TEAMS) {
+        const int slot = p.slots[first + i];
+        if (slot < 0 || slot >= p.cache.slots) *out(first + i) = u32x4_t{0, 0, 0, 0};
+    }
+}
+
+// Keys of a 4-bit cache, keys and values of a 16-bit one: a team a row.
 template <int DT, int D, int BITS>
-__global__ __launch_bounds__(kThreads) void kv_gather_kernel(const GatherArgs p) {
+__global__ __launch_bounds__(kThreads) void kv_gather_kernel(const GatherArgs p, int v_rows, int v_groups) {
     constexpr int CH = D / 8, GROUPS = D / kGroup;
     const int c = threadIdx.x % CH, kvh = p.cache.kv_heads;
-    const int64_t row = int64_t(blockIdx.x) * (kThreads / CH) + threadIdx.x / CH;
-    if (row >= int64_t(p.rows) * 2 * kvh) return;
-    const int n = int(uint32_t(row) / uint32_t(2 * kvh));
-    int h = int(row - int64_t(n) * 2 * kvh);
+    int block = blockIdx.x;
+    if constexpr (BITS == 4) {
+        if (block < v_groups) {
+            const int run = block / kvh;
+            gather_values<DT, D>(p, run * v_rows, v_rows, block - run * kvh);
+            return;
+        }
+        block -= v_groups;
+    }
+    const int heads = BITS == 4 ? kvh : 2 * kvh;
+    const int64_t row = int64_t(block) * (kThreads / CH) + threadIdx.x / CH;
+    if (row >= int64_t(p.rows) * heads) return;
+    const int n = int(uint32_t(row) / uint32_t(heads));
+    int h = int(row - int64_t(n) * heads);
     const bool value = h >= kvh;
     if (value) h -= kvh;
     uint16_t* out = (value ? p.v_out : p.k_out) + (int64_t(n) * kvh + h) * D + 8 * c;
@@ -301,36 +360,13 @@ __global__ __launch_bounds__(kThreads) void kv_gather_kernel(const GatherArgs p)
         *reinterpret_cast<u32x4_t*>(out) = load16(src + ((int64_t(at) * kvh + h) * D + 8 * c) * 2);
     } else {
         const int g = c / 8;
-        if (!value) {
-            const int64_t line = int64_t(h) * p.cache.block_size + at;
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(
-                p.cache.k + page * p.cache.k_stride + line * (D / 2) + 4 * word_place<GROUPS, 8>(g, c % 8));
-            const uint32_t scale = *reinterpret_cast<const uint32_t*>(
-                p.cache.k_scales + page * p.cache.ks_stride + 4 * (line * GROUPS + g));
-            *reinterpret_cast<u32x4_t*>(out) =
-                dequantise8<DT>(scale, [&](int j) { return (word >> (4 * (j / 2) + 16 * (j % 2))) & 15u; });
-            return;
-        }
-        const int share = row_share(p.slots, n, p.rows, slot);
-        if (share == 0) return;
-        const char* words = p.cache.v + page * p.cache.v_stride +
-                            (int64_t(h) * p.cache.block_size + (at & ~3u)) * (D / 2);
-        const char* scales = p.cache.v_scales + page * p.cache.vs_stride +
-                             4 * ((int64_t(h) * GROUPS + g) * p.cache.block_size + at);
-        u32x2_t w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-            w[e] = *reinterpret_cast<const u32x2_t*>(words + 4 * word_place<GROUPS, 32>(g, 4 * (c % 8) + 2 * e));
-        auto token = [&](uint32_t scale, int i) {
-            return dequantise8<DT>(scale, [&](int j) { return (w[j / 4][(j / 2) % 2] >> (8 * i + 4 * (j % 2))) & 15u; });
-        };
-        if (share == 4) {
-            const u32x4_t sc = load16(scales);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4_t*>(out + int64_t(i) * kvh * D) = token(sc[i], i);
-        } else {
-            *reinterpret_cast<u32x4_t*>(out) = token(*reinterpret_cast<const uint32_t*>(scales), at & 3);
-        }
+        const int64_t line = int64_t(h) * p.cache.block_size + at;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(
+            p.cache.k + page * p.cache.k_stride + line * (D / 2) + 4 * word_place<GROUPS, 8>(g, c % 8));
+        const uint32_t scale = *reinterpret_cast<const uint32_t*>(
+            p.cache.k_scales + page * p.cache.ks_stride + 4 * (line * GROUPS + g));
+        *reinterpret_cast<u32x4_t*>(out) =
+            dequantise8<DT>(scale, [&](int j) { return (word >> (4 * (j / 2) + 16 * (j % 2))) & 15u; });
     }
 }
 
@@ -348,6 +384,12 @@ int pick(int dtype, int head_dim, int bits, F&& f) {
                                        : with_dim(std::integral_constant<int, NANOVLLM_GEMM_F16>{});
 }
 
+// 4 bits: rows of a workgroup of values.  64 where enough workgroups are left: 8000
+// tokens of 4 heads of 128 are appended in 23.1 us, 24.1 with 16.
+int value_rows(int rows, int kv_heads, int teams) {
+    return int64_t(rows) * kv_heads >= 64 * kFull / 8 ? 64 : teams;
+}
+
 }  // namespace
 
 int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, hipStream_t s) {
@@ -355,12 +397,11 @@ int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, h
     const int64_t heads = p.heads + int64_t(bits == 4 ? 1 : 2) * kvh, runs = (p.tokens + teams - 1) / teams;
     // Four heads to a team where enough workgroups are left: at 16 + 4 heads of 128, 4 bits, 64 tokens take 3.4 us
     // with one head and 5.8 with four, 1500 8.7 and 9.2, 3500 13.3 and 12.6; at 8 + 4 heads of 256, 16 bits, 300
-    // tokens 3.7 and 4.5, 1000 5.6 and 5.5, 2500 9.3 and 8.5, 20000 61 and 45.  Rows of values likewise: 64 of them
-    // for 16 took 8000 tokens from 24.1 to 23.1 us.
+    // tokens 3.7 and 4.5, 1000 5.6 and 5.5, 2500 9.3 and 8.5, 20000 61 and 45.
     const int each = runs * heads >= 2 * kFull ? 4 : 1;
     AppendSplit sp{p, int32_t((heads + each - 1) / each), 0, 0};
     if (bits == 4) {
-        sp.v_rows = int64_t(p.tokens) * kvh >= 64 * kFull / 8 ? 64 : teams;
+        sp.v_rows = value_rows(p.tokens, kvh, teams);
         sp.v_groups = (p.tokens + sp.v_rows - 1) / sp.v_rows * kvh;
     }
     const int64_t groups = runs * sp.parts + sp.v_groups;
@@ -376,12 +417,16 @@ int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, h
 }
 
 int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s) {
-    const int64_t rows = int64_t(p.rows) * 2 * p.cache.kv_heads, per = kThreads / (head_dim / 8);
-    const int64_t groups = (rows + per - 1) / per;
+    const int kvh = p.cache.kv_heads, teams = kThreads / (head_dim / 8);
+    const int64_t rows = int64_t(p.rows) * (bits == 4 ? 1 : 2) * kvh;
+    const int v_rows = value_rows(p.rows, kvh, teams);
+    const int64_t v_groups = bits == 4 ? (int64_t(p.rows) + v_rows - 1) / v_rows * kvh : 0;
+    const int64_t groups = (rows + teams - 1) / teams + v_groups;
     if (groups > kMostGroups) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "kv_gather: too many rows and heads");
     const dim3 grid(static_cast<uint32_t>(groups));
     return pick(dtype, head_dim, bits, [&](auto dt, auto d, auto b) {
-        hipLaunchKernelGGL((kv_gather_kernel<dt.value, d.value, b.value>), grid, dim3(kThreads), 0, s, p);
+        hipLaunchKernelGGL((kv_gather_kernel<dt.value, d.value, b.value>), grid, dim3(kThreads), 0, s, p, v_rows,
+                           static_cast<int>(v_groups));
         return check_launch("kv_gather");
     });
 }

@@ -219,6 +219,32 @@ def test_rope_append_of_many_tokens(bits, size, dtype, dim, tokens):
         assert a is b is None or torch.equal(_bits(a), _bits(b))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim,rows", [(64, 3300), (128, 2801), (256, 2760)])
+def test_kv_gather_of_many_rows(dtype, dim, rows):
+    """A long 4-bit gather (64 rows of values to a workgroup) reads bit for bit what calls of at most 50 rows read:
+    runs that begin at any slot, slots outside the cache, the same slot twice."""
+    _say("many rows", dtype, dim, rows)
+    gen, kv, size = _gen(dim + rows), 3, 48
+    blocks = rows // size + 4
+    cache = _noisy_cache(blocks, size, kv, dim, 4, dtype, gen)
+    slots = torch.arange(rows) + torch.repeat_interleave(torch.randint(0, 4, (rows // 90 + 1,), generator=gen).cumsum(0),
+                                                         90)[:rows]
+    slots[500:530] = slots[500:530].flip(0)
+    slots[1000:1100] = torch.randint(0, blocks * size, (100,), generator=gen)
+    slots[40:44] = slots[44:48]
+    slots[torch.randint(0, rows, (9,), generator=gen)] = -1
+    slots[2000], slots[rows - 1] = blocks * size, 2 ** 31 - 1
+    slots = slots.to(torch.int32).to(DEV)
+    k, v = K.kv_gather(cache.k, cache.v, slots, cache.k_scales, cache.v_scales, out_dtype=dtype)
+    at = 0
+    while at < rows:
+        n = at + int(torch.randint(1, 51, (1,), generator=gen))
+        pk, pv = K.kv_gather(cache.k, cache.v, slots[at:n], cache.k_scales, cache.v_scales, out_dtype=dtype)
+        assert torch.equal(_bits(k[at:n]), _bits(pk)) and torch.equal(_bits(v[at:n]), _bits(pv)), at
+        at = n
+
+
 def test_appended_rows_read_back():
     """A cache written in pieces reads back as written at once, through blocks that are slices of a larger allocation."""
     _say("read back")
