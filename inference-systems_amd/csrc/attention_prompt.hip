@@ -12,13 +12,14 @@
 // V^T is read from LDS transposed (ds_read_b64_tr_b16), 4 keys of a channel at
 // a time, which is the run of keys a lane's accumulators hold.
 //
-// The work is split over a fixed grid: all (sequence, head, 128 queries) blocks
-// in units of one tile of keys, laid end to end, each workgroup an equal run of
-// units; a block starts with six units that hold no key and stand for what it
-// costs to begin one.  So a causal prompt's long rows and short ones, a few
-// queries against many keys, and sequences of any lengths load the chip evenly.
-// A block whose keys lie in one run is finished there; the parts of others go
-// to a workspace (at most two per workgroup) and a second kernel joins them.
+// Short blocks, and many, have a workgroup each.  The others (see in_runs) are
+// split over a fixed grid: all (sequence, head, 128 queries) blocks in units of
+// one tile of keys, laid end to end, each workgroup an equal run of units; a
+// block starts with six units that hold no key and stand for what it costs to
+// begin one.  So a causal prompt's long rows and short ones, a few queries
+// against many keys, and sequences of any lengths load the chip evenly.  A block
+// whose keys lie in one run is finished there; the parts of others go to a
+// workspace (at most two per workgroup) and a second kernel joins them.
 //
 // Bound by the matrix cores, which run at the chip's power limit: on MI355X 16384
 // tokens of 8 heads of 256 take 1121-1145 us, 960-980 TFLOP/s (a large library
@@ -627,14 +628,27 @@ int resident(int head_dim) { return head_dim == 256 ? 256 : 512; }
 // Blocks there can be: every sequence, and the rows behind the last, round up.
 int64_t most_blocks(int64_t batch, int64_t q_rows, int64_t heads) { return (q_rows / kRows + batch + 1) * heads; }
 
-// Whether blocks are dealt in equal runs, rather than one to a workgroup.
-bool in_runs(int64_t batch, int64_t q_rows, int64_t heads, int head_dim) {
-    return most_blocks(batch, q_rows, heads) < 3 * resident(head_dim);
+// Whether blocks are dealt in equal runs, rather than one to a workgroup.  Not where
+// there are three or more for every place on the chip (24 ragged prompts: 123 us a
+// block a workgroup, 153 + 16 in runs).  Else runs save what the longest block has
+// over the average place, and cost the parts and the join, as much as `worth` tiles.
+// Of several sequences only the sum of keys is known here, so the longest is taken
+// for all of it and the average for nothing.  A block a workgroup / in runs, us:
+// 8 heads of 256, 300 tokens 19.9 / 24.2, 500 27.0 / 29.3, 700 31.2 / 30.8, 1000 42.4 /
+// 33.2; 32 of them, 800 36.5 / 50.9; 100 tokens behind 400 26.3 / 23.5; 8 heads of 128,
+// 300 12.7 / 18.3, 1200 27.1 / 30.3, 1500 33.4 / 32.7; 32 of them, 1900 48.3 / 58.4; 16
+// heads of 64, 300 9.7 / 16.6, 1500 24.8 / 29.4.
+bool in_runs(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int head_dim) {
+    const int64_t blocks = most_blocks(batch, q_rows, heads), worth = head_dim == 256 ? 7 : 18;
+    if (blocks >= 3 * resident(head_dim)) return false;
+    const int64_t longest = (k_rows + kKeys - 1) / kKeys, before = q_rows / kRows;
+    const int64_t average = batch > 1 ? 0 : heads * (before + 1) * (longest > before ? longest - before : 0);
+    return (longest - worth) * resident(head_dim) > average;
 }
 
 int64_t grid_of(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int head_dim) {
     const int64_t blocks = most_blocks(batch, q_rows, heads);
-    if (!in_runs(batch, q_rows, heads, head_dim)) return blocks;
+    if (!in_runs(batch, q_rows, k_rows, heads, head_dim)) return blocks;
     const int64_t units = blocks * (kBegin + 1 + k_rows / kKeys), most = resident(head_dim);
     return units < most ? units : most;
 }
@@ -659,7 +673,7 @@ int launch_dim(const Split& s, int head_dim, hipStream_t stream) {
 
 int64_t attention_prompt_workspace(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim) {
     const int64_t grid = grid_of(batch, q_rows, k_rows, heads, static_cast<int>(head_dim));
-    if (grid == 1 || !in_runs(batch, q_rows, heads, static_cast<int>(head_dim))) return 0;
+    if (grid == 1 || !in_runs(batch, q_rows, k_rows, heads, static_cast<int>(head_dim))) return 0;
     return 2 * grid * kRows * (head_dim + 2) * 4;
 }
 
@@ -668,7 +682,7 @@ int launch_attention_prompt(const PromptArgs& p, void* workspace, int head_dim, 
     if (grid > kMostGroups)
         return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "attention_prompt: too many sequences, rows and heads");
     const Split split{p, static_cast<float*>(workspace), static_cast<int32_t>(grid),
-                      in_runs(p.batch, p.q_rows, p.heads, head_dim)};
+                      in_runs(p.batch, p.q_rows, p.k_rows, p.heads, head_dim)};
     return dtype == NANOVLLM_GEMM_BF16 ? launch_dim<NANOVLLM_GEMM_BF16>(split, head_dim, s)
                                        : launch_dim<NANOVLLM_GEMM_F16>(split, head_dim, s);
 }

@@ -119,8 +119,8 @@ def test_bad_caches_are_refused(lib, fields, code, message):
     (_prompt, dict(scale=-1.0), L.EINVAL, "scale"),
     (_prompt, dict(batch=-1), L.EINVAL, "batch"),
     (_prompt, dict(q_rows=2 ** 31), L.EINVAL, "rows"),
-    (_prompt, dict(workspace=None), L.EINVAL, "workspace"),
-    (_prompt, dict(workspace_bytes=100), L.EINVAL, "workspace"),
+    (_prompt, dict(k_rows=5000, workspace=None), L.EINVAL, "workspace"),
+    (_prompt, dict(k_rows=5000, workspace_bytes=100), L.EINVAL, "workspace"),
     (_prompt, dict(k_row=2 ** 24), L.EUNSUPPORTED, "2^24"),
     (_prompt, dict(batch=2 ** 22), L.EUNSUPPORTED, "too many"),
     (_prompt, dict(k=None), L.EINVAL, "non-null"),
@@ -164,9 +164,10 @@ def test_paged_workspace(lib):
 def test_prompt_workspace(lib):
     need = L.attention_prompt_workspace_bytes
     assert need(1, 0, 0, 4, 2, 128, L.BF16) == 0
-    small = need(1, 5, 5, 1, 1, 128, L.BF16)
-    assert 0 < small < need(1, 500, 500, 4, 2, 128, L.BF16)
-    # Bounded by the grid, whatever the keys; none where every workgroup has a block of its own.
+    small = need(1, 5, 2000, 1, 1, 128, L.BF16)
+    assert 0 < small < need(1, 500, 3000, 4, 2, 128, L.BF16)
+    # Bounded by the grid, whatever the keys; none where every workgroup has a block of its own: few keys, many blocks.
+    assert need(1, 500, 500, 4, 2, 128, L.BF16) == need(3, 900, 900, 4, 2, 64, L.BF16) == 0
     assert need(1, 512, 10 ** 4, 32, 8, 128, L.BF16) == need(1, 600, 10 ** 9, 32, 8, 128, L.BF16) < 1 << 27
     assert need(9, 10 ** 7, 10 ** 9, 64, 8, 128, L.BF16) == 0
     assert need(1, 5, 5, 3, 2, 128, L.BF16) == L.EINVAL and "multiple" in L.last_error()

@@ -379,6 +379,53 @@ def test_attention_prompt_many_sequences():
     _check_prompt(got, q, k, v, lens, lens, 0.125, True, "many")
 
 
+# Keys enough that blocks are cut into equal runs.
+RUNS = [
+    ([5, 130, 31, 0, 900], [5, 130, 31, 0, 1200]),
+    ([1, 7, 129], [40, 200, 1300]),
+    ([20, 0, 3, 140, 1], [3, 9, 0, 70, 1400]),
+    ([1], [1250]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 4), (128, 6, 2), (256, 8, 1)])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("lengths", RUNS, ids=lambda x: "-".join(map(str, x[0])))
+def test_attention_prompt_in_runs(dtype, dim, heads, kv, causal, lengths):
+    lq, lk = lengths
+    _say("prompt in runs", dtype, dim, heads, kv, causal, lengths)
+    gen = _gen(sum(lk) + dim)
+    q, k, v = (torch.randn((sum(n), h, dim), generator=gen).to(dtype).to(DEV) for n, h in ((lq, heads), (lk, kv), (lk, kv)))
+    got = K.attention_prompt(q, k, v, _cu(lq), _cu(lk), dim ** -0.5, causal)
+    _check_prompt(got, q, k, v, lq, lk, dim ** -0.5, causal, "runs")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_prompt_in_runs_keeps_to_what_a_row_sees(dtype, dim):
+    """As test_attention_prompt_keeps_to_what_a_row_sees, blocks cut into runs; growing scores rescale the sums."""
+    _say("runs, masked places", dtype, dim)
+    gen = _gen(dim)
+    lens = [70, 45, 1, 1300]
+    n = sum(lens)
+    q, k, v = (torch.randn((n, 2, dim), generator=gen) for _ in range(3))
+    k[116:] *= torch.linspace(0.01, 6.0, 1300)[:, None, None]
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_v[30, 0, 3], bad_v[90], bad_k[60], bad_v[800, 1], bad_k[1000, 0] = torch.nan, -torch.inf, torch.nan, torch.inf, torch.nan
+    got, want = (K.attention_prompt(q.to(DEV), a.to(DEV), b.to(DEV), _cu(lens), _cu(lens), dim ** -0.5).cpu()
+                 for a, b in ((bad_k, bad_v), (k, v)))
+    _check_prompt(want, q, k, v, lens, lens, dim ** -0.5, True, "runs")
+    same = torch.ones(n, 2, dim, dtype=torch.bool)
+    same[30:70, 0, 3] = same[60:70] = same[90:115] = same[800:, 1] = same[1000:, 0] = False
+    assert torch.equal(got[same], want[same])
+    assert torch.isnan(got[30:70, 0, 3]).all() and torch.isnan(got[60:70]).all()
+    assert (got[90:115] == -torch.inf).all() and torch.isnan(got[1000:, 0]).all()
+    # Where its P is 0, by rounding, an infinity makes a NaN.
+    assert (torch.isnan(got[800:, 1]) | (got[800:, 1] == torch.inf)).all()
+
+
 @pytest.mark.parametrize("dim,heads,kv,lq,lk", [(64, 2, 1, 130, 5000), (128, 3, 3, 515, 2500), (256, 2, 2, 300, 3400)])
 @pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
 def test_attention_prompt_long_keys(dim, heads, kv, lq, lk, causal):
@@ -626,7 +673,7 @@ def test_prompt_graph_replays_follow_their_offsets(heads, batch):
     """attention_prompt captured once (equal runs of keys; a workgroup a block) and replayed with other rows and
     offsets, eager calls in between, as it answers eagerly."""
     _say("prompt graph", heads, batch)
-    gen, rows, dim = _gen(batch), 900, 128
+    gen, rows, dim = _gen(batch), 1900, 128
     q, k, v = (torch.zeros((rows, h, dim), dtype=BF16, device=DEV) for h in (heads, 2, 2))
     cu = torch.zeros(batch + 1, dtype=torch.int32, device=DEV)
     K.attention_prompt(q, k, v, cu, cu, 0.09)
