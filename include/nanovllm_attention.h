@@ -129,9 +129,10 @@ int64_t nanovllm_attention_prompt_workspace_bytes(int64_t batch, int64_t q_rows,
  * Attention of one query token per sequence over its cached tokens: out[b, h]
  * = softmax(scale q[b, h] k^T) v over the first lens[b] tokens of pages
  * tables[b, 0 .. table_blocks) (row stride table_stride, in entries).  Page
- * sizes are multiples of 16.  No token: 0.  A page number outside the cache,
- * or a length behind the table, makes the sequence's output NaN.  q is
- * [batch, heads, head_dim] with strides as above, out contiguous.  Workspace:
+ * sizes are multiples of 16, and a table holds at most 2^31 - 1024 tokens.  No
+ * token: 0.  A page number outside the cache, or a length behind the table,
+ * makes the sequence's output NaN.  q is [batch, heads, head_dim] with strides
+ * as above, out contiguous.  Workspace:
  * nanovllm_attention_paged_workspace_bytes() bytes, 16-byte aligned scratch.
  */
 int nanovllm_attention_paged(const void* q, const nanovllm_kv_cache* cache,

@@ -117,9 +117,11 @@ int check_paged(const char* op, const nanovllm_kv_cache* cache, int64_t batch, i
     if (cache->block_size % 16)
         return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: block_size (%lld) must be a multiple of 16", op,
                          (long long)cache->block_size);
-    if (!fits32(batch) || !fits32(table_blocks) || !fits32(table_blocks * cache->block_size))
-        return set_error(NANOVLLM_GEMM_EINVAL, "%s: batch and table must be non-negative and hold fewer than 2^31 tokens",
-                         op);
+    // Tokens are counted in 32 bits, and the kernel looks two units of 128 and half a tile past a sequence's end.
+    constexpr int64_t most = INT32_MAX - 1023;
+    if (!fits32(batch) || !fits32(table_blocks) || table_blocks * cache->block_size > most)
+        return set_error(NANOVLLM_GEMM_EINVAL,
+                         "%s: batch and table must be non-negative, and a table hold at most 2^31 - 1024 tokens", op);
     // Units of 128 tokens are counted in 32 bits; the join has a workgroup or more for each pair.
     const int64_t blocks = cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
     if (batch * blocks > kMostGroups || !fits32(batch * blocks * (table_blocks * cache->block_size / 128 + 8)))
