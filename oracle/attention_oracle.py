@@ -129,3 +129,52 @@ def tolerance(out, absolute, big, dtype, dim: int, *, p_half_step: float):
     half_step = torch.finfo(dtype).eps / 2
     w = 2 * (dim + 16) * 2.0 ** -24 * big + 2.0 ** -20
     return half_step * out.abs() + (p_half_step + w) * (absolute + out.abs()) * (1 + half_step) + 1e-30
+
+
+def read_rows(cache, slots):
+    """Rows of a 4-bit cache of numpy arrays, for slots [n]: (codes, scales, minima) of keys and of values, float64
+    [n, heads, dim] each."""
+    k, v, ks, vs = cache
+    size, dim = k.shape[2], 2 * k.shape[3]
+    block, at = np.divmod(np.asarray(slots, dtype=np.int64), size)
+    c = np.arange(dim)
+    word = np.ascontiguousarray(k[block, :, at]).view(np.uint32)
+    word = word[..., [word_place(dim, x, 8, x % GROUP // 8) for x in c]]
+    code_k = (word >> (4 * (c % 8 // 2) + 16 * (c % 2)).astype(np.uint32)) & 15
+    byte = v.reshape(*v.shape[:2], size // 4, dim // 2, 4)[block, :, at // 4, :, at % 4]
+    byte = byte[..., [word_place(dim, x, 32, x % GROUP // 2) for x in c]]
+    code_v = (byte >> (4 * (c % 2)).astype(np.uint8)) & 15
+    pairs = [p.astype(np.float64)[:, :, c // GROUP] for p in (ks[block, :, at], vs[block, :, :, at])]
+    return [[torch.from_numpy(x) for x in (code.astype(np.float64), p[..., 0], p[..., 1])]
+            for code, p in zip((code_k, code_v), pairs)]
+
+
+def attend_4bit(q, keys, values, scale, dtype, tiles: int):
+    """One query row float64 [1, heads, dim] over 4-bit rows (`read_rows`): (out, how far a correct kernel may be off).
+
+    With key c s + m, a kernel may sum products on 16 + c and take m - 16 s apart, in fp32: a product goes through
+    the 64 sums of its group and 16 further roundings, each of half a last place (2^-24) of what is added up.  An error
+    e of a score changes its weight by a factor 1 + e, of which the total has the mean.  2^-20: base-2 exponentials and
+    the scaling.
+    With value (c - 7.5) s + (m + 7.5 s) and weight p: p s, p and m + 7.5 s are rounded to float16 (2^-11 each, or
+    2^-25 in its subnormal range: of p and p s held 2^10 fold where all scales are at most 32), the total of the
+    rounded p divides.  Sums of (64 + c) p s and of 64 + 7.5 times the p s run over `tiles` tiles of 32 tokens: 32
+    and 8 additions a tile and 8 to join lanes, of at most one last place (2^-23) of (64 + 15) p s.  Then one rounding
+    to dtype.  1 + 2^-6: products of these errors."""
+    (ck, sk, mk), (cv, sv, mv) = keys, values
+    group = q.shape[1] // ck.shape[1]
+    out, w, _ = attend(q, ck * sk + mk, cv * sv + mv, scale)
+    heads = lambda x: x.repeat_interleave(group, 1)      # noqa: E731
+    spread = lambda x: torch.einsum("hij,jhd->ihd", w, heads(x))      # noqa: E731
+    score = torch.einsum("ihd,jhd->hij", q.abs(), heads((16 + ck) * sk + (mk - 16 * sk).abs())) * scale
+    error = w * (80 * 2.0 ** -24 * score + 2.0 ** -20)
+    value = (cv * sv + mv).abs()
+    n, around, middle = ck.shape[0], (cv - 7.5).abs() * sv, (mv + 7.5 * sv).abs()
+    half = 2.0 ** -11
+    least = 2.0 ** -35 if bool((sv <= 32).all()) else 2.0 ** -25
+    off = half * (spread(around) + 2 * spread(middle) + out.abs())
+    off = off + torch.einsum("hij,jhd->ihd", error, heads(value)) + error.sum(-1).T[..., None] * out.abs()
+    off = off + least * (7.5 * n + heads(middle).sum(0, keepdim=True) + n * out.abs()) + 2.0 ** -25
+    off = off + (40 * tiles + 8) * 2.0 ** -23 * 79 * spread(sv)
+    off = off * (1 + 2.0 ** -6)
+    return out, off + torch.finfo(dtype).eps / 2 * (out.abs() + off)

@@ -1,4 +1,5 @@
-"""A 4-bit cache byte for byte."""
+"""A 4-bit cache byte for byte, and attention over it within a bound derived
+from its scales: the bound itself on the CPU, the kernels on the GPU."""
 from __future__ import annotations
 
 import numpy as np
@@ -108,3 +109,87 @@ def test_append_leaves_every_other_byte(dtype, dim, kv, size, tokens, kind):
     """Written rows by the oracle, every other byte as it was: words that four tokens share among them."""
     _say("every byte", dtype, dim, kv, size, tokens, kind)
     _append_and_compare("cuda:0", "hip", dtype, dim, kv, size, tokens, kind)
+
+
+# ---------------------------------------------------------------------------
+# attention_paged over 4-bit pages
+# ---------------------------------------------------------------------------
+# (lengths, page, heads, kv_heads, dim, magnitude of the values)
+PAGED = [(lens, size, heads, kv, dim, 1.0)
+         for lens, size, heads, kv in (([1, 15, 16, 17], 16, 4, 4), ([31, 32, 33, 127, 128, 129], 48, 8, 2),
+                                       ([257, 1000], 256, 5, 1), ([700], 32, 40, 2))
+         for dim in (64, 128, 256)]
+PAGED += [([300, 40], 16, 4, 2, 128, m) for m in (1e-3, 300.0, 20000.0)]      # scales above 32 in the last two
+PAGED += [([9000] + [1 + 7 * i % 60 for i in range(140)], 16, 4, 2, 64, 1.0)]
+PAGED_IDS = [f"{len(p[0])}x{p[0][0]}-{p[4]}-{p[5]:g}" for p in PAGED]
+
+
+def _paged_case(lens, size, heads, kv, dim, magnitude, dtype, device, backend):
+    gen = _gen(sum(lens) + dim)
+    need = [-(-n // size) for n in lens]
+    blocks = sum(need) + 2
+    order = torch.randperm(blocks, generator=gen).tolist()
+    tables, slots, at = torch.full((len(lens), max(need)), -1, dtype=torch.int32), [], 0
+    for b, n in enumerate(lens):
+        pages = order[at:at + need[b]]
+        tables[b, :need[b]] = torch.tensor(pages, dtype=torch.int32)
+        slots.append([pages[t // size] * size + t % size for t in range(n)])
+        at += need[b]
+    q = torch.randn((len(lens), heads, dim), generator=gen).to(dtype)
+    total = sum(lens)
+    k = (torch.randn((total, kv, dim), generator=gen) + torch.randn((kv, dim), generator=gen)).to(dtype)
+    v = (torch.randn((total, kv, dim), generator=gen) * magnitude).to(dtype)
+    cache = K.KVCache(*[t.to(device) for t in _noisy(K.new_kv_cache(blocks, size, kv, dim, bits=4), gen)])
+    _append(k.to(device), v.to(device), _i32([s for x in slots for s in x], device), cache, backend)
+    return q.to(device), cache, tables.to(device), slots
+
+
+def _tiles(lens, kv, heads):
+    """Most tiles of 32 tokens that one wave adds up: a pair (sequence, key-value head, 16 query heads) has a unit per
+    128 tokens and 3 to begin, a unit is one tile of each of 4 waves, and 512 workgroups or more share them evenly."""
+    units = sum(3 + -(-n // 128) for n in lens) * kv * -(-heads // kv // 16)
+    return min(-(-max(lens) // 128), -(-units // 512))
+
+
+def _bounds(q, cache, slots, lens, scale):
+    """out and tolerance [batch, heads, dim]."""
+    kv, now, rows = cache.k.shape[1], _numpy(cache), []
+    for b, mine in enumerate(slots):
+        keys, values = orc.read_rows(now, mine)
+        rows.append(orc.attend_4bit(q[b:b + 1].cpu().double(), keys, values, scale, q.dtype,
+                                    _tiles(lens, kv, q.shape[1])))
+    return [torch.cat(x) for x in zip(*rows)]
+
+
+def _outside(got, out, tol):
+    return ~((got.cpu().double() - out).abs() <= tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("case", PAGED, ids=PAGED_IDS)
+def test_the_bound_rejects_what_is_wrong(dtype, case):
+    """Zeros leave the bound in nearly all elements, outputs 3% off in a fifth or more (small sums of large parts may be
+    that far off); what the torch backend computes in 32 bits does not."""
+    lens, heads, dim = case[0], case[2], case[4]
+    q, cache, tables, slots = _paged_case(*case, dtype, "cpu", "torch")
+    out, tol = _bounds(q, cache, slots, lens, dim ** -0.5)
+    got = K.paged_attention(q, cache, tables, _i32(lens, "cpu"), dim ** -0.5, backend="torch")
+    assert not _outside(got, out, tol).any()
+    assert _outside(torch.zeros_like(out), out, tol).float().mean() > 0.95
+    assert _outside(out * 1.03, out, tol).float().mean() > 0.2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("case", PAGED, ids=PAGED_IDS)
+def test_paged_4bit_within_the_bound(dtype, case):
+    lens, dim = case[0], case[4]
+    _say("paged 4 bit", dtype, case[1:], lens[:6])
+    q, cache, tables, slots = _paged_case(*case, dtype, "cuda:0", "hip")
+    out, tol = _bounds(q, cache, slots, lens, dim ** -0.5)
+    got = K.attention_paged(q, cache.k, cache.v, tables, _i32(lens, "cuda:0"), dim ** -0.5, cache.k_scales,
+                            cache.v_scales)
+    bad = _outside(got, out, tol)
+    worst = ((got.cpu().double() - out).abs() / tol).max()
+    _say("largest share of the bound", float(worst))
+    assert not bad.any(), (int(bad.sum()), float(worst))
