@@ -464,6 +464,11 @@ __global__ __launch_bounds__(256, D == 256 && BITS == 16 ? 1 : 2) void attention
                               fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
             top = max_across32(max_across16(top));
             if constexpr (BITS == 4) {
+                if (ragged) {   // scales behind the end may be anything, and are not the sequence's
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (t + 16 * h + 4 * quad + (col / NB) % 4 >= t_end) tile.vb[h] = 0;
+                }
                 // 2^10 p s has to fit fp16.  Where a scale is too large for that,
                 // this and the following tiles go without the factor.
                 const float big = fmaxf(f16_to_f32(uint16_t(tile.vb[0])), f16_to_f32(uint16_t(tile.vb[1])));
@@ -527,11 +532,6 @@ __global__ __launch_bounds__(256, D == 256 && BITS == 16 ? 1 : 2) void attention
                         o[nb][e] = mfma_16x16x32<PT>(a, pk, o[nb][e]);
                     }
             } else {
-                if (ragged) {   // scales behind the end may be NaN
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (t + 16 * h + 4 * quad + (col / NB) % 4 >= t_end) tile.vb[h] = 0;
-                }
                 // Tokens of an operand in the order 0 2 1 3 of each four.  The four
                 // of group l % 16 lie NB lanes apart in vb.
                 u32x4_t pk, am;

@@ -2,6 +2,8 @@
 from its scales: the bound itself on the CPU, the kernels on the GPU."""
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -193,3 +195,36 @@ def test_paged_4bit_within_the_bound(dtype, case):
     worst = ((got.cpu().double() - out).abs() / tol).max()
     _say("largest share of the bound", float(worst))
     assert not bad.any(), (int(bad.sum()), float(worst))
+
+
+def _one_large_score(n, down, dim, dtype, device):
+    """q, keys, values, scale: key 0 scores `down` powers of two above all others, and its value is 0."""
+    q, k = torch.ones((1, 1, dim)), torch.zeros((n, 1, dim))
+    k[0] = 1.0
+    v = torch.linspace(0.5, 1.5, dim).expand(n, 1, dim).clone()
+    v[0] = 0.0
+    return *(x.to(dtype).to(device) for x in (q, k, v)), down * math.log(2) / dim
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,page", [(5, 16), (20, 16), (45, 32), (140, 48)])
+def test_paged_4bit_depends_on_its_own_scales_only(dim, n, page):
+    """What scales hold behind a sequence's end, and in pages it has none of, changes no bit of its output.  (Its
+    weights, 2^-17 of the largest, would lose bits if such a scale took the factor off that P is held with.)"""
+    _say("own scales", dim, n, page)
+    q, k, v, scale = _one_large_score(n, 17.3, dim, F16, "cuda:0")
+    blocks = -(-n // page)
+    pages = list(range(1, blocks + 1))
+    slots = _i32([pages[t // page] * page + t % page for t in range(n)], "cuda:0")
+    outs = []
+    for left in (0.0, 33.0, 1000.0, 60000.0, torch.inf, torch.nan):
+        cache = K.new_kv_cache(blocks + 2, page, 1, dim, bits=4, device="cuda:0")
+        cache.v_scales.fill_(left)
+        cache.k_scales.fill_(left)
+        _append(k, v, slots, cache, "hip")
+        outs.append(K.attention_paged(q, cache.k, cache.v, _i32([pages + [0]], "cuda:0"), _i32([n], "cuda:0"), scale,
+                                      cache.k_scales, cache.v_scales))
+    assert not torch.isnan(outs[0]).any() and outs[0].any()
+    for x in outs[1:]:
+        assert torch.equal(x, outs[0])
