@@ -79,9 +79,10 @@ typedef struct nanovllm_kv_cache {
  * of one call are distinct.  A position outside the table turns by NaN.
  *
  * 4 bits: a group x of 64 channels of a row, clamped to float16's finite range,
- * is kept as minimum m = f16(min x), scale s = f16((max x - min x) / 15) and
- * codes clamp(rint((x - m) / s), 0, 15), 0 where s is 0.  A NaN in the group
- * makes all of it NaN.
+ * is kept as minimum m = f16(min x), scale s = f16((max x - min x) / 15), or
+ * the float16 below it where 15 s + m passes 65504, and codes
+ * clamp(rint((x - m) / s), 0, 15), 0 where s is 0.  So what a code stands for is
+ * in float16's finite range too.  A NaN in the group makes all of it NaN.
  */
 int nanovllm_rope_append(const void* q, const void* k, const void* v,
                          const int64_t* positions, const float* cos_sin, const int32_t* slots,

@@ -105,8 +105,13 @@ __device__ __forceinline__ Coded quantise8(u32x4_t raw) {
         nan |= __shfl_xor(nan, off);
     }
     if (nan) lo = hi = __builtin_nanf("");
-    const _Float16 s16 = static_cast<_Float16>((hi - lo) / 15.0f), m16 = static_cast<_Float16>(lo);
-    const float s = static_cast<float>(s16), m = static_cast<float>(m16);
+    _Float16 s16 = static_cast<_Float16>((hi - lo) / 15.0f);
+    const _Float16 m16 = static_cast<_Float16>(lo);
+    const float m = static_cast<float>(m16);
+    // A scale rounded up may carry code 15 past float16's range (15 s is exact, so the sum is rounded once).
+    if (15.0f * static_cast<float>(s16) + m > 65504.0f)
+        s16 = __builtin_bit_cast(_Float16, static_cast<uint16_t>(__builtin_bit_cast(uint16_t, s16) - 1));
+    const float s = static_cast<float>(s16);
     const float y = 1.0f / s;
     Coded r;
 #pragma unroll

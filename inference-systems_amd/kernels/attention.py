@@ -472,6 +472,8 @@ def _quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     g = x.float().clamp(-65504.0, 65504.0).unflatten(-1, (-1, GROUP))
     low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
     s, m = ((high - low) / 15).half(), low.half()
+    # Code 15 stays in float16's range: the scale below one that was rounded up past it.
+    s = torch.where(15 * s.float() + m.float() > 65504.0, (s.view(torch.int16) - 1).view(torch.float16), s)
     codes = ((g - m.float()) / s.float()).round().clamp(0, 15)
     codes = torch.where(s > 0, codes, 0.0).to(torch.int32)
     return codes.flatten(-2), torch.cat((s, m), -1)

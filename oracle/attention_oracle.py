@@ -39,6 +39,8 @@ def code_row(row: np.ndarray):
             continue
         s = np.float16((g.max() - g.min()) / np.float32(15))
         m = np.float16(g.min())
+        if 15.0 * float(s) + float(m) > 65504.0:      # a finite row stays finite: code 15 in float16's range
+            s = np.nextafter(s, np.float16(0))
         if s > 0:
             q = np.rint((g - np.float32(m)) / np.float32(s))
             codes += [int(v) for v in np.clip(q, 0, 15)]

@@ -228,3 +228,60 @@ def test_paged_4bit_depends_on_its_own_scales_only(dim, n, page):
     assert not torch.isnan(outs[0]).any() and outs[0].any()
     for x in outs[1:]:
         assert torch.equal(x, outs[0])
+
+
+# ---------------------------------------------------------------------------
+# The ends of float16's range
+# ---------------------------------------------------------------------------
+def _extreme_rows(dim, dtype):
+    """Groups whose top code is at, or near, the largest float16."""
+    top, at = 65504.0, torch.arange(dim)
+    ranges = [(-top, top), (0.0, top), (-top, 0.0), (top, top), (-top, -top), (60000.0, top), (-3000.0, top),
+              (-50000.0, 65000.0), (-20000.0, 65472.0), (-65472.0, 65472.0), (torch.finfo(dtype).min, torch.finfo(dtype).max)]
+    rows = [torch.where(at % 3 == 0, hi, torch.where(at % 3 == 1, lo, (lo + hi) / 2)) for lo, hi in ranges[:-1]]
+    lo, hi = ranges[-1]
+    rows.append(torch.where(at % 2 == 0, torch.full((dim,), hi), torch.full((dim,), lo)))
+    rows.append(torch.where(at % 2 == 0, torch.inf, -torch.inf) * torch.ones(dim))
+    return torch.stack(rows)[:, None].to(dtype)
+
+
+def _finite_rows_stay_finite(device, backend, dtype, dim):
+    rows = _extreme_rows(dim, dtype)
+    n = rows.shape[0]
+    slots = [(5 * t + 3) % 32 for t in range(n)]
+    cache = K.new_kv_cache(2, 16, 1, dim, bits=4, device=device)
+    want = _numpy(K.new_kv_cache(2, 16, 1, dim, bits=4))
+    x = rows.to(device)
+    still = torch.cat((torch.ones(1, 16), torch.zeros(1, 16)), 1)
+    keys = torch.where(torch.isinf(rows), 0.0, rows)      # an infinity turns by 0 x infinity
+    K.rope_append_kv(keys.to(device), keys.to(device), x, torch.zeros(n, dtype=torch.int64, device=device),
+                     still.to(device), _i32(slots, device), cache, backend=backend)
+    turned = orc.rotate(keys, [0] * n, still)
+    for t, s in enumerate(slots):
+        orc.write_row(want, s, 0, turned[t, 0].float().numpy(), rows[t, 0].float().numpy())
+    for a, b in zip(_numpy(cache), want):
+        assert np.array_equal(a, b)
+    _, (code, step, low) = orc.read_rows(want, slots)
+    stands_for = code * step + low
+    assert float(stands_for.abs().max()) <= 65504.0
+    # Half of a code's step, and what rounding the scale down adds at code 15.
+    off = (stands_for - rows.double().clamp(-65504, 65504)).abs()
+    assert (off <= 0.5 * step + 15 * 8 + 16).all()
+    for out_dtype in (F16, BF16):
+        for got in K.gather_kv(cache, _i32(slots, device), out_dtype, backend=backend):
+            assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim", [64, 256])
+def test_torch_backend_keeps_finite_rows_finite(dtype, dim):
+    _finite_rows_stay_finite("cpu", "torch", dtype, dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_finite_rows_stay_finite(dtype, dim):
+    """Rows are clamped to float16's range so that they stay finite; what their codes stand for stays in it too."""
+    _say("ends of the range", dtype, dim)
+    _finite_rows_stay_finite("cuda:0", "hip", dtype, dim)
