@@ -37,7 +37,16 @@ constexpr int kRows = 128;      // queries of a block
 constexpr int kKeys = 64;       // keys of a tile
 constexpr int kBegin = 6;       // units a block costs before its first tile, and by its masked ones (2, 4, 6:
                                 // 43.0, 42.1, 40.6 us for 2048 tokens, 79 -> 77 for a chunk of 512)
-constexpr float kLazy = 8.0f;   // sums are rescaled when a maximum grows by more than 2^8
+
+// Sums are rescaled when a maximum grows by more than 2^kLazy, and P is held
+// 2^kBoost fold, which cancels in O / l; together they fit the type.  Without the
+// factor float16 loses weights below 2^-25 next to 1, which count where there are
+// many: 131072 keys 2^-25.4 below another one came out 2.4e-3 off, with it 4.7e-4
+// (half a step of the output: 4.9e-4).  By (kLazy, kBoost), float16: 16384 tokens
+// of 8 heads of 256 (8, 0) 1181 us, (8, 7) 1181, (3, 12) 1184, (0, 15) 1238; 24
+// ragged prompts 117, 118, 118, 123.
+template <int DT> constexpr float kLazy = DT == NANOVLLM_GEMM_F16 ? 3.0f : 8.0f;
+template <int DT> constexpr float kBoost = DT == NANOVLLM_GEMM_F16 ? 12.0f : 0.0f;
 
 struct Split {
     PromptArgs a;
@@ -467,7 +476,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
             }
             top = max_across32(top);
             // A first score (m is -infinity), or one that outgrows the range P has been given.
-            if (__ballot((top - m) * p.c > kLazy)) {
+            if (__ballot((top - m) * p.c > kLazy<DT>)) {
                 const float higher = fmaxf(m, top);
                 const float down = higher == -__builtin_inff() ? 1.0f : exp2_hw((m - higher) * p.c);
                 m = higher;
@@ -475,7 +484,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
 #pragma unroll
                 for (int i = 0; i < DTILES; ++i) o[i] *= down;
             }
-            const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
+            const float shift = (m == -__builtin_inff() ? 0.0f : m * p.c) - kBoost<DT>;
             const uint32_t v_at = v_read + (t & 1) * TILE;
             u32x4_t vf[2][DTILES];      // values of 16 keys, and of the next 16
             auto read = [&](int g, int i) {
@@ -563,7 +572,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                 for (int v = 0; v < 16; v += 4)
                     *reinterpret_cast<f32x4_t*>(sums + 32 * i + 2 * v + 4 * half) =
                         f32x4_t{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]};
-            const float shift = m == -__builtin_inff() ? 0.0f : m * p.c;
+            const float shift = (m == -__builtin_inff() ? 0.0f : m * p.c) - kBoost<DT>;
             for (int t = full; t < t1; ++t)
                 if (late >> (t - full) & 1)
                     add_keys<DT, D>(p, qrow, kbase, vbase, t * kKeys, min(lk, t * kKeys + kKeys), last, half, shift, sums);
