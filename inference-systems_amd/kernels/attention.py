@@ -568,11 +568,15 @@ def _torch_attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal=T
 
 def _torch_attention_paged(q, k_cache, v_cache, block_tables, context_lens, scale, k_scales=None, v_scales=None):
     cache = KVCache(k_cache, v_cache, k_scales, v_scales)
-    size = _geometry(k_cache, k_scales)[1]
+    blocks, size, _, _ = _geometry(k_cache, k_scales)
     out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     for b, n in enumerate(context_lens.tolist()):
-        at = torch.arange(n, device=q.device)
-        k, v = _torch_rows(cache, block_tables[b].long()[at // size] * size + at % size)
+        pages = block_tables[b, :-(-max(n, 0) // size)].long()
+        if n > block_tables.shape[1] * size or ((pages < 0) | (pages >= blocks)).any():
+            out[b] = torch.nan
+            continue
+        at = torch.arange(max(n, 0), device=q.device)
+        k, v = _torch_rows(cache, pages[at // size] * size + at % size)
         out[b] = _torch_attend(q[b:b + 1].float(), k, v, scale, None)[0].to(q.dtype)
     return out
 

@@ -1,0 +1,67 @@
+"""The plain torch backend keeps the contracts of the ops: what pages, lengths,
+masks and infinities give is the same on either backend (on the GPU, both)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import PKG
+
+K = PKG.kernels
+BF16, F16 = torch.bfloat16, torch.float16
+BACKENDS = [pytest.param(("cpu", "torch"), id="torch"),
+            pytest.param(("cuda:0", "torch"), id="torch-gpu", marks=pytest.mark.gpu),
+            pytest.param(("cuda:0", "hip"), id="hip", marks=pytest.mark.gpu)]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _i32(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def _filled(bits, device, gen, blocks=6, size=16, heads=2, dim=64):
+    """A cache whose every slot holds a row of random keys and values."""
+    cache = K.new_kv_cache(blocks, size, heads, dim, bits=bits, device=device)
+    k, v = (torch.randn((blocks * size, heads, dim), generator=gen).to(BF16).to(device) for _ in range(2))
+    table = torch.cat((torch.ones(1, 16), torch.zeros(1, 16)), 1).to(device)
+    K.rope_append_kv(k, k, v, torch.zeros(blocks * size, dtype=torch.int64, device=device), table,
+                     torch.arange(blocks * size, dtype=torch.int32, device=device), cache, backend="torch")
+    return cache
+
+
+@pytest.mark.parametrize("where", BACKENDS)
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_bad_pages_and_lengths(where, bits):
+    """A page outside the cache or a length behind the table makes that sequence NaN and no other, whatever the entries
+    behind a sequence's end hold; no token gives 0, a negative length too."""
+    device, backend = where
+    print("bad pages", device, backend, bits, flush=True)
+    gen = _gen(bits)
+    cache = _filled(bits, device, gen)
+    q = torch.randn((8, 4, 64), generator=gen).to(BF16).to(device)
+    good = [[0, 1, 2], [3, 4, 5], [5, 0, 3], [1, 2, 4], [4, 3, 2], [2, 1, 0], [0, 2, 4], [1, 3, 5]]
+    lens = [33, 48, 17, 40, 16, 48, 5, 30]
+    want = K.paged_attention(q, cache, _i32(good, device), _i32(lens, device), 0.125, backend=backend)
+    bad = [row[:] for row in good]
+    bad[0][2], bad[1][0], bad[2][1] = -1, 6, 2 ** 31 - 1      # inside the length
+    bad[4][1], bad[4][2], bad[6][1] = -7, 6, 10 ** 9          # behind it
+    lens[3], lens[5], lens[7] = 49, 0, -3
+    got = K.paged_attention(q, cache, _i32(bad, device), _i32(lens, device), 0.125, backend=backend)
+    assert not torch.isnan(want).any()
+    assert torch.isnan(got[:4]).all()
+    assert torch.equal(got[[4, 6]], want[[4, 6]])
+    assert not got[[5, 7]].any()
+
+
+@pytest.mark.parametrize("where", BACKENDS)
+def test_paged_empty_table(where):
+    device, backend = where
+    print("empty table", device, backend, flush=True)
+    cache = _filled(16, device, _gen(1))
+    q = torch.ones((3, 2, 64), dtype=BF16, device=device)
+    table = torch.empty((3, 0), dtype=torch.int32, device=device)
+    got = K.paged_attention(q, cache, table, _i32([0, 1, -2 ** 31], device), 0.125, backend=backend)
+    assert torch.isnan(got[1]).all() and not got[[0, 2]].any()
