@@ -554,7 +554,13 @@ def _torch_attend(q, k, v, scale, first):
     top = s.amax(-1, keepdim=True) if k.shape[1] else s.new_zeros((*s.shape[:2], 1))
     p = torch.exp(s - torch.where(top == -torch.inf, 0.0, top))
     total = p.sum(-1, keepdim=True)
-    return (torch.matmul(p, v) / torch.where(total == 0, 1.0, total)).transpose(0, 1)
+    # Values that are not finite only reach the rows that see them (a product would: 0 x infinity).
+    finite = torch.isfinite(v)
+    o = torch.matmul(p, torch.where(finite, v, 0.0))
+    for j in (~finite).any(-1).any(0).nonzero().flatten().tolist():
+        rows = slice(0 if first is None else max(0, j - first), None)
+        o[:, rows] += p[:, rows, j:j + 1] * torch.where(finite[:, j], 0.0, v[:, j])[:, None]
+    return (o / torch.where(total == 0, 1.0, total)).transpose(0, 1)
 
 
 def _torch_attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal=True):

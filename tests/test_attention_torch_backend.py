@@ -65,3 +65,31 @@ def test_paged_empty_table(where):
     table = torch.empty((3, 0), dtype=torch.int32, device=device)
     got = K.paged_attention(q, cache, table, _i32([0, 1, -2 ** 31], device), 0.125, backend=backend)
     assert torch.isnan(got[1]).all() and not got[[0, 2]].any()
+
+
+@pytest.mark.parametrize("where", BACKENDS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_keeps_to_what_a_row_sees(where, causal):
+    """NaN and infinities in keys and values that a row does not see change nothing in it."""
+    device, backend = where
+    print("masked places", device, backend, causal, flush=True)
+    gen = _gen(7)
+    lens, spare = [70, 45, 1], 20
+    n = sum(lens)
+    q, k, v = (torch.randn((n + spare, 2, 64), generator=gen).to(BF16) for _ in range(3))
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_v[30, 0, 3], bad_v[33, 1, 5], bad_v[90] = torch.nan, torch.inf, -torch.inf
+    bad_k[60], bad_k[n:], bad_v[n:] = torch.nan, torch.nan, torch.inf
+    cu = _i32([0, 70, 115, 116], device)
+    want, got = (K.prompt_attention(*(x.to(device) for x in (q, *kv)), cu, cu, 0.125, causal, backend=backend).cpu()
+                 for kv in ((k, v), (bad_k, bad_v)))
+    first = lambda i, a: i if causal else a      # noqa: E731
+    same = torch.ones(n + spare, 2, 64, dtype=torch.bool)
+    same[first(30, 0):70, 0, 3] = same[first(33, 0):70, 1, 5] = False
+    same[first(60, 0):70] = same[first(90, 70):115] = False
+    assert not torch.isnan(want).any() and not want[n:].any()
+    assert torch.equal(got[same], want[same])
+    assert torch.isnan(got[first(30, 0):70, 0, 3]).all() and torch.isnan(got[first(60, 0):70]).all()
+    assert (got[first(90, 70):115] == -torch.inf).all()
+    if causal:
+        assert (got[33:60, 1, 5] == torch.inf).all()
