@@ -547,20 +547,21 @@ def _torch_attend(q, k, v, scale, first):
     """fp32 q [m, heads, dim] over k, v [n, kv_heads, dim]; row i sees keys up to first + i (None: all)."""
     group = q.shape[1] // k.shape[1]
     k, v = (x.repeat_interleave(group, 1).transpose(0, 1).contiguous() for x in (k, v))
+    m, n = q.shape[0], k.shape[1]
+    last = torch.full((m,), n - 1, device=q.device) if first is None else first + torch.arange(m, device=q.device)
+    hidden = torch.arange(n, device=q.device) > last[:, None]
     s = torch.matmul(q.transpose(0, 1).contiguous(), k.transpose(1, 2).contiguous()) * scale
-    if first is not None:
-        hidden = torch.arange(k.shape[1], device=q.device) > first + torch.arange(q.shape[0], device=q.device)[:, None]
-        s = s.masked_fill(hidden, -torch.inf)
-    top = s.amax(-1, keepdim=True) if k.shape[1] else s.new_zeros((*s.shape[:2], 1))
+    s = s.masked_fill(hidden, -torch.inf)
+    top = s.amax(-1, keepdim=True) if n else s.new_zeros((*s.shape[:2], 1))
     p = torch.exp(s - torch.where(top == -torch.inf, 0.0, top))
-    total = p.sum(-1, keepdim=True)
     # Values that are not finite only reach the rows that see them (a product would: 0 x infinity).
     finite = torch.isfinite(v)
     o = torch.matmul(p, torch.where(finite, v, 0.0))
     for j in (~finite).any(-1).any(0).nonzero().flatten().tolist():
         rows = slice(0 if first is None else max(0, j - first), None)
         o[:, rows] += p[:, rows, j:j + 1] * torch.where(finite[:, j], 0.0, v[:, j])[:, None]
-    return (o / torch.where(total == 0, 1.0, total)).transpose(0, 1)
+    # A row that sees no key is 0; one whose every score is -infinity is 0 / 0.
+    return (o / torch.where(hidden.all(-1)[:, None], 1.0, p.sum(-1, keepdim=True))).transpose(0, 1)
 
 
 def _torch_attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal=True):

@@ -93,3 +93,28 @@ def test_prompt_keeps_to_what_a_row_sees(where, causal):
     assert (got[first(90, 70):115] == -torch.inf).all()
     if causal:
         assert (got[33:60, 1, 5] == torch.inf).all()
+
+
+@pytest.mark.parametrize("where", BACKENDS)
+def test_scores_that_are_not_finite(where):
+    """A score of -infinity drops its key; rows whose every score is -infinity, or one with +infinity, are NaN; a row
+    with no key to see is 0."""
+    device, backend = where
+    print("infinite scores", device, backend, flush=True)
+    gen = _gen(5)
+    q, k, v = (torch.randn((40, 1, 64), generator=gen).to(BF16) for _ in range(3))
+    q[:, 0, 0], k[:, 0, 0] = 1.0, 0.0
+    k[3, 0, 0], k[0, 0, 0], k[35, 0, 0] = -torch.inf, -torch.inf, torch.inf
+    cu = _i32([0, 40], device)
+    got = K.prompt_attention(*(x.to(device) for x in (q, k, v)), cu, cu, 0.125, backend=backend).cpu()
+    assert torch.isnan(got[0]).all() and torch.isnan(got[35:]).all() and not torch.isnan(got[1:35]).any()
+    # More queries than keys: the first three rows see none, the fourth one of -infinity only.
+    cu_k = _i32([0, 37], device)
+    got = K.prompt_attention(*(x.to(device) for x in (q, k[:37], v[:37])), cu, cu_k, 0.125, backend=backend).cpu()
+    assert not got[:3].any() and torch.isnan(got[3]).all() and not torch.isnan(got[4:38]).any()
+    # The same over pages.
+    cache = K.new_kv_cache(4, 16, 1, 64, device=device)
+    cache.k.view(-1, 1, 64)[:40], cache.v.view(-1, 1, 64)[:40] = k.to(device), v.to(device)
+    table, lens = _i32([[0, 1, 2, 3]] * 3, device), _i32([1, 35, 36], device)
+    got = K.paged_attention(q[:3].to(device), cache, table, lens, 0.125, backend=backend).cpu()
+    assert torch.isnan(got[0]).all() and not torch.isnan(got[1]).any() and torch.isnan(got[2]).all()
