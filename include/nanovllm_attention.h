@@ -92,6 +92,10 @@ int nanovllm_rope_append(const void* q, const void* k, const void* v,
                          int64_t v_row, int64_t v_head,
                          int64_t positions_max, int64_t rotary, void* stream);
 
+/* Whether nanovllm_rope_append takes a call of these sizes: OK, or the code it
+ * would return.  Pure host function; the cache's pointers are not looked at. */
+int nanovllm_rope_append_check(const nanovllm_kv_cache* cache, int64_t tokens, int64_t heads);
+
 /*
  * Rows of the cache as packed keys and values: k_out and v_out [rows,
  * kv_heads, head_dim] of dtype (the cache's in 16 bits) hold row slots[i] of
@@ -99,6 +103,9 @@ int nanovllm_rope_append(const void* q, const void* k, const void* v,
  */
 int nanovllm_kv_gather(const nanovllm_kv_cache* cache, const int32_t* slots, int64_t rows,
                        void* k_out, void* v_out, int dtype, void* stream);
+
+/* Whether nanovllm_kv_gather takes a call of these sizes, as above. */
+int nanovllm_kv_gather_check(const nanovllm_kv_cache* cache, int64_t rows);
 
 /*
  * Attention of packed sequences, heads in groups of heads / kv_heads that
@@ -121,8 +128,8 @@ int nanovllm_attention_prompt(const void* q, const void* k, const void* v,
                               float scale, int causal, int dtype,
                               void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of nanovllm_attention_prompt, or a negative code.  Pure host
- * function. */
+/* Workspace bytes of nanovllm_attention_prompt, or the negative code that it
+ * returns for a call of these sizes.  Pure host function. */
 int64_t nanovllm_attention_prompt_workspace_bytes(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads,
                                                   int64_t kv_heads, int64_t head_dim, int dtype);
 
@@ -142,8 +149,8 @@ int nanovllm_attention_paged(const void* q, const nanovllm_kv_cache* cache,
                              int64_t q_row, int64_t q_head, float scale, int dtype,
                              void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of nanovllm_attention_paged, or a negative code.  Pure host
- * function. */
+/* Workspace bytes of nanovllm_attention_paged, or the negative code that it
+ * returns for a call of these sizes.  Pure host function. */
 int64_t nanovllm_attention_paged_workspace_bytes(const nanovllm_kv_cache* cache, int64_t batch, int64_t heads,
                                                  int64_t table_blocks);
 

@@ -78,6 +78,8 @@ SIGNATURES = {
     "nanovllm_gemm_add_rmsnorm_with_kernel": (_INT, [_INT, _VP, _VP, _VP, _F32, _VP, _VP, _VP] + [_I64] * 8
                                               + [_INT, _INT, _INT, _VP, _I64, _VP]),
     "nanovllm_rope_append": (_INT, [_VP] * 8 + [_CACHE] + [_I64] * 10 + [_VP]),
+    "nanovllm_rope_append_check": (_INT, [_CACHE, _I64, _I64]),
+    "nanovllm_kv_gather_check": (_INT, [_CACHE, _I64]),
     "nanovllm_kv_gather": (_INT, [_CACHE, _VP, _I64, _VP, _VP, _INT, _VP]),
     "nanovllm_attention_prompt": (_INT, [_VP] * 6 + [_I64] * 12 + [_F32, _INT, _INT, _VP, _I64, _VP]),
     "nanovllm_attention_prompt_workspace_bytes": (_I64, [_I64] * 6 + [_INT]),
@@ -276,6 +278,16 @@ def rope_append_raw(q_ptr, k_ptr, v_ptr, positions_ptr, cos_sin_ptr, slots_ptr, 
     check(load().nanovllm_rope_append(q_ptr, k_ptr, v_ptr, positions_ptr, cos_sin_ptr, slots_ptr, q_out_ptr,
                                       k_out_ptr, cache, tokens, heads, q_row, q_head, k_row, k_head, v_row, v_head,
                                       positions_max, rotary, stream), "nanovllm_rope_append")
+
+
+def rope_append_check(cache, tokens, heads) -> int:
+    """OK, or the code with which the rotation and cache append refuses these sizes."""
+    return load().nanovllm_rope_append_check(cache, tokens, heads)
+
+
+def kv_gather_check(cache, rows) -> int:
+    """OK, or the code with which the read of cached rows refuses these sizes."""
+    return load().nanovllm_kv_gather_check(cache, rows)
 
 
 def kv_gather_raw(cache, slots_ptr, rows, k_ptr, v_ptr, dtype, stream) -> None:

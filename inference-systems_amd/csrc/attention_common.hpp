@@ -130,6 +130,11 @@ __device__ __forceinline__ void static_for(F&& f) {
     }
 }
 
+// Workgroups of a launch: kMostGroups at most, which the C ABI checks.
+int64_t rope_append_groups(int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim, int bits);
+int64_t kv_gather_groups(int64_t rows, int64_t kv_heads, int head_dim, int bits);
+int64_t attention_prompt_groups(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim);
+
 int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
 int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s);
 int launch_attention_prompt(const PromptArgs& p, void* workspace, int head_dim, int dtype, hipStream_t s);

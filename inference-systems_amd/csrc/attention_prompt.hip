@@ -680,6 +680,10 @@ int launch_dim(const Split& s, int head_dim, hipStream_t stream) {
 
 }  // namespace
 
+int64_t attention_prompt_groups(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim) {
+    return grid_of(batch, q_rows, k_rows, heads, static_cast<int>(head_dim));
+}
+
 int64_t attention_prompt_workspace(int64_t batch, int64_t q_rows, int64_t k_rows, int64_t heads, int64_t head_dim) {
     const int64_t grid = grid_of(batch, q_rows, k_rows, heads, static_cast<int>(head_dim));
     if (grid == 1 || !in_runs(batch, q_rows, k_rows, heads, static_cast<int>(head_dim))) return 0;
@@ -688,8 +692,6 @@ int64_t attention_prompt_workspace(int64_t batch, int64_t q_rows, int64_t k_rows
 
 int launch_attention_prompt(const PromptArgs& p, void* workspace, int head_dim, int dtype, hipStream_t s) {
     const int64_t grid = grid_of(p.batch, p.q_rows, p.k_rows, p.heads, head_dim);
-    if (grid > kMostGroups)
-        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "attention_prompt: too many sequences, rows and heads");
     const Split split{p, static_cast<float*>(workspace), static_cast<int32_t>(grid),
                       in_runs(p.batch, p.q_rows, p.k_rows, p.heads, head_dim)};
     return dtype == NANOVLLM_GEMM_BF16 ? launch_dim<NANOVLLM_GEMM_BF16>(split, head_dim, s)

@@ -106,6 +106,29 @@ int check_prompt(const char* op, int64_t batch, int64_t q_rows, int64_t k_rows, 
     if (rc != NANOVLLM_GEMM_OK) return rc;
     if (batch < 0 || q_rows < 0 || k_rows < 0 || batch > INT32_MAX / 2 || q_rows > INT32_MAX / 2 || k_rows > INT32_MAX / 2)
         return set_error(NANOVLLM_GEMM_EINVAL, "%s: batch and rows must be non-negative and below 2^30", op);
+    if (q_rows > 0 && attention_prompt_groups(batch, q_rows, k_rows, heads, head_dim) > kMostGroups)
+        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: too many sequences, rows and heads", op);
+    return NANOVLLM_GEMM_OK;
+}
+
+int check_append(const char* op, const nanovllm_kv_cache* cache, int64_t tokens, int64_t heads, bool touched) {
+    int rc = check_cache(op, cache, touched);
+    if (rc == NANOVLLM_GEMM_OK) rc = check_dims(op, heads, cache->kv_heads, cache->head_dim, cache->dtype);
+    if (rc != NANOVLLM_GEMM_OK) return rc;
+    if (tokens < 0 || !fits32(tokens) || tokens * (heads + 2 * cache->kv_heads) > INT32_MAX)
+        return set_error(NANOVLLM_GEMM_EINVAL, "%s: tokens must be non-negative, and tokens times heads below 2^31", op);
+    if (rope_append_groups(tokens, heads, cache->kv_heads, static_cast<int>(cache->head_dim), cache->bits) > kMostGroups)
+        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: too many tokens and heads", op);
+    return NANOVLLM_GEMM_OK;
+}
+
+int check_gather(const char* op, const nanovllm_kv_cache* cache, int64_t rows, bool touched) {
+    const int rc = check_cache(op, cache, touched);
+    if (rc != NANOVLLM_GEMM_OK) return rc;
+    if (rows < 0 || !fits32(rows) || rows * 2 * cache->kv_heads > INT32_MAX)
+        return set_error(NANOVLLM_GEMM_EINVAL, "%s: rows must be non-negative, and rows times heads below 2^31", op);
+    if (kv_gather_groups(rows, cache->kv_heads, static_cast<int>(cache->head_dim), cache->bits) > kMostGroups)
+        return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "%s: too many rows and heads", op);
     return NANOVLLM_GEMM_OK;
 }
 
@@ -141,14 +164,11 @@ int nanovllm_rope_append(const void* q, const void* k, const void* v, const int6
     using namespace nvg;
     const char* op = "rope_append";
     clear_error();
-    int rc = check_cache(op, cache, tokens > 0);
-    if (rc == NANOVLLM_GEMM_OK) rc = check_dims(op, heads, cache->kv_heads, cache->head_dim, cache->dtype);
+    int rc = check_append(op, cache, tokens, heads, tokens > 0);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "q", q_row, q_head);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "k", k_row, k_head);
     if (rc == NANOVLLM_GEMM_OK) rc = check_strides(op, "v", v_row, v_head);
     if (rc != NANOVLLM_GEMM_OK) return rc;
-    if (tokens < 0 || !fits32(tokens) || tokens * (heads + 2 * cache->kv_heads) > INT32_MAX)
-        return set_error(NANOVLLM_GEMM_EINVAL, "rope_append: tokens must be non-negative, and tokens times heads below 2^31");
     if (rotary < 16 || rotary % 16 || rotary > cache->head_dim)
         return set_error(NANOVLLM_GEMM_EINVAL, "rope_append: rotary (%lld) must be a multiple of 16 from 16 to head_dim",
                          (long long)rotary);
@@ -170,19 +190,27 @@ int nanovllm_kv_gather(const nanovllm_kv_cache* cache, const int32_t* slots, int
     using namespace nvg;
     const char* op = "kv_gather";
     clear_error();
-    int rc = check_cache(op, cache, rows > 0);
+    int rc = check_gather(op, cache, rows, rows > 0);
     if (rc != NANOVLLM_GEMM_OK) return rc;
     if (!is_half(dtype) || (cache->bits == 16 && dtype != cache->dtype))
         return set_error(NANOVLLM_GEMM_EUNSUPPORTED,
                          "kv_gather: rows are f16 or bf16, those of a 16-bit cache in its own dtype");
-    if (rows < 0 || !fits32(rows) || rows * 2 * cache->kv_heads > INT32_MAX)
-        return set_error(NANOVLLM_GEMM_EINVAL, "kv_gather: rows must be non-negative, and rows times heads below 2^31");
     if (rows == 0) return NANOVLLM_GEMM_OK;
     rc = check_pointers(op, {k_out, v_out}, {slots});
     if (rc != NANOVLLM_GEMM_OK) return rc;
     const GatherArgs p{slots, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out),
                        static_cast<int32_t>(rows), kernel_cache(*cache)};
     return launch_kv_gather(p, static_cast<int>(cache->head_dim), cache->bits, dtype, static_cast<hipStream_t>(stream));
+}
+
+int nanovllm_rope_append_check(const nanovllm_kv_cache* cache, int64_t tokens, int64_t heads) {
+    nvg::clear_error();
+    return nvg::check_append("rope_append", cache, tokens, heads, false);
+}
+
+int nanovllm_kv_gather_check(const nanovllm_kv_cache* cache, int64_t rows) {
+    nvg::clear_error();
+    return nvg::check_gather("kv_gather", cache, rows, false);
 }
 
 int nanovllm_attention_prompt(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,

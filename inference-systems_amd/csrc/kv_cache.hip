@@ -391,27 +391,57 @@ int pick(int dtype, int head_dim, int bits, F&& f) {
 
 // 4 bits: rows of a workgroup of values.  64 where enough workgroups are left: 8000
 // tokens of 4 heads of 128 are appended in 23.1 us, 24.1 with 16.
-int value_rows(int rows, int kv_heads, int teams) {
-    return int64_t(rows) * kv_heads >= 64 * kFull / 8 ? 64 : teams;
+int value_rows(int64_t rows, int64_t kv_heads, int teams) {
+    return rows * kv_heads >= 64 * kFull / 8 ? 64 : teams;
 }
+
+// The workgroups of an append, see AppendSplit.
+struct AppendGrid {
+    int each, v_rows;
+    int64_t parts, v_groups, all;
+
+    AppendGrid(int64_t tokens, int64_t q_heads, int64_t kv_heads, int head_dim, int bits) {
+        const int teams = kThreads / (head_dim / 8);
+        const int64_t heads = q_heads + (bits == 4 ? 1 : 2) * kv_heads, runs = (tokens + teams - 1) / teams;
+        // Four heads to a team where enough workgroups are left: at 16 + 4 heads of 128, 4 bits, 64 tokens take 3.4 us
+        // with one head and 5.8 with four, 1500 8.7 and 9.2, 3500 13.3 and 12.6; at 8 + 4 heads of 256, 16 bits, 300
+        // tokens 3.7 and 4.5, 1000 5.6 and 5.5, 2500 9.3 and 8.5, 20000 61 and 45.
+        each = runs * heads >= 2 * kFull ? 4 : 1;
+        parts = (heads + each - 1) / each;
+        v_rows = bits == 4 ? value_rows(tokens, kv_heads, teams) : 0;
+        v_groups = bits == 4 ? (tokens + v_rows - 1) / v_rows * kv_heads : 0;
+        all = runs * parts + v_groups;
+    }
+};
+
+// The workgroups of a gather.
+struct GatherGrid {
+    int v_rows;
+    int64_t v_groups, all;
+
+    GatherGrid(int64_t rows, int64_t kv_heads, int head_dim, int bits) {
+        const int teams = kThreads / (head_dim / 8);
+        v_rows = value_rows(rows, kv_heads, teams);
+        v_groups = bits == 4 ? (rows + v_rows - 1) / v_rows * kv_heads : 0;
+        all = (rows * (bits == 4 ? 1 : 2) * kv_heads + teams - 1) / teams + v_groups;
+    }
+};
 
 }  // namespace
 
+int64_t rope_append_groups(int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim, int bits) {
+    return AppendGrid(tokens, heads, kv_heads, head_dim, bits).all;
+}
+
+int64_t kv_gather_groups(int64_t rows, int64_t kv_heads, int head_dim, int bits) {
+    return GatherGrid(rows, kv_heads, head_dim, bits).all;
+}
+
 int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, hipStream_t s) {
-    const int kvh = p.cache.kv_heads, teams = kThreads / (head_dim / 8);
-    const int64_t heads = p.heads + int64_t(bits == 4 ? 1 : 2) * kvh, runs = (p.tokens + teams - 1) / teams;
-    // Four heads to a team where enough workgroups are left: at 16 + 4 heads of 128, 4 bits, 64 tokens take 3.4 us
-    // with one head and 5.8 with four, 1500 8.7 and 9.2, 3500 13.3 and 12.6; at 8 + 4 heads of 256, 16 bits, 300
-    // tokens 3.7 and 4.5, 1000 5.6 and 5.5, 2500 9.3 and 8.5, 20000 61 and 45.
-    const int each = runs * heads >= 2 * kFull ? 4 : 1;
-    AppendSplit sp{p, int32_t((heads + each - 1) / each), 0, 0};
-    if (bits == 4) {
-        sp.v_rows = value_rows(p.tokens, kvh, teams);
-        sp.v_groups = (p.tokens + sp.v_rows - 1) / sp.v_rows * kvh;
-    }
-    const int64_t groups = runs * sp.parts + sp.v_groups;
-    if (groups > kMostGroups) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "rope_append: too many tokens and heads");
-    const dim3 grid(static_cast<uint32_t>(groups));
+    const AppendGrid g(p.tokens, p.heads, p.cache.kv_heads, head_dim, bits);
+    const AppendSplit sp{p, static_cast<int32_t>(g.parts), g.v_rows, static_cast<int32_t>(g.v_groups)};
+    const int each = g.each;
+    const dim3 grid(static_cast<uint32_t>(g.all));
     return pick(dtype, head_dim, bits, [&](auto dt, auto d, auto b) {
         if (each == 4)
             hipLaunchKernelGGL((rope_append_kernel<dt.value, d.value, b.value, 4>), grid, dim3(kThreads), 0, s, sp);
@@ -422,16 +452,11 @@ int launch_rope_append(const AppendArgs& p, int head_dim, int bits, int dtype, h
 }
 
 int launch_kv_gather(const GatherArgs& p, int head_dim, int bits, int dtype, hipStream_t s) {
-    const int kvh = p.cache.kv_heads, teams = kThreads / (head_dim / 8);
-    const int64_t rows = int64_t(p.rows) * (bits == 4 ? 1 : 2) * kvh;
-    const int v_rows = value_rows(p.rows, kvh, teams);
-    const int64_t v_groups = bits == 4 ? (int64_t(p.rows) + v_rows - 1) / v_rows * kvh : 0;
-    const int64_t groups = (rows + teams - 1) / teams + v_groups;
-    if (groups > kMostGroups) return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "kv_gather: too many rows and heads");
-    const dim3 grid(static_cast<uint32_t>(groups));
+    const GatherGrid g(p.rows, p.cache.kv_heads, head_dim, bits);
+    const dim3 grid(static_cast<uint32_t>(g.all));
     return pick(dtype, head_dim, bits, [&](auto dt, auto d, auto b) {
-        hipLaunchKernelGGL((kv_gather_kernel<dt.value, d.value, b.value>), grid, dim3(kThreads), 0, s, p, v_rows,
-                           static_cast<int>(v_groups));
+        hipLaunchKernelGGL((kv_gather_kernel<dt.value, d.value, b.value>), grid, dim3(kThreads), 0, s, p, g.v_rows,
+                           static_cast<int>(g.v_groups));
         return check_launch("kv_gather");
     });
 }

@@ -347,6 +347,7 @@ std::tuple<at::Tensor, at::Tensor> gemm_add_rmsnorm(const at::Tensor& h, const a
 // wording, and their launches.
 // ---------------------------------------------------------------------------
 constexpr int64_t kGroup = 64;
+constexpr int64_t kRowStrides = int64_t(1) << 24;
 
 struct CacheTensors {
     const at::Tensor &k, &v;
@@ -418,6 +419,7 @@ std::string rows_reason(const char* name, const at::Tensor& t, at::ScalarType dt
         return n + " must be a (rows, heads, head_dim) tensor that fits the others, got " + tuple_text(t.sizes());
     if (t.stride(2) != 1) return n + " must have unit stride in its last dimension";
     if (stride_of(t, 0) % 8 || stride_of(t, 1) % 8) return "the strides of " + n + " must be multiples of 8";
+    if (stride_of(t, 0) >= kRowStrides) return "the row stride of " + n + " must be below 2^24";
     if (t.numel() && !aligned16(t)) return n + " must be 16-byte aligned";
     return {};
 }
@@ -476,6 +478,13 @@ nanovllm_kv_cache cache_struct(const CacheTensors& c, at::ScalarType dtype) {
     return s;
 }
 
+// The library's words for sizes it refuses (rc of its check or workspace function).
+std::string sizes_reason(const char* op, int64_t rc) {
+    if (rc >= 0) return {};
+    const std::string said = nanovllm_gemm_last_error(), prefix = std::string(op) + ": ";
+    return said.rfind(prefix, 0) == 0 ? said.substr(prefix.size()) : said;
+}
+
 std::string rope_append_reason(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                const at::Tensor& positions, const at::Tensor& cos_sin, const at::Tensor& slots,
                                const CacheTensors& c) {
@@ -499,7 +508,8 @@ std::string rope_append_reason(const at::Tensor& q, const at::Tensor& k, const a
     if (rotary < 16 || rotary % 16 || rotary > dim)
         return "rotary_dim (" + std::to_string(rotary) + ") must be a multiple of 16 from 16 to head_dim (" +
                std::to_string(dim) + ")";
-    return {};
+    const nanovllm_kv_cache cache = cache_struct(c, dt);
+    return sizes_reason("rope_append", nanovllm_rope_append_check(&cache, q.size(0), q.size(1)));
 }
 
 std::tuple<at::Tensor, at::Tensor> rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -534,7 +544,10 @@ std::string kv_gather_reason(const CacheTensors& c, const at::Tensor& slots, std
     if (c.coded() && !(out_dtype.has_value() && (*out_dtype == at::kHalf || *out_dtype == at::kBFloat16)))
         return "out_dtype of a 4-bit cache must be float16 or bfloat16";
     if (slots.dim() != 1) return "slots must be one-dimensional";
-    return index_reason("slots", slots, at::kInt, slots.sizes());
+    r = index_reason("slots", slots, at::kInt, slots.sizes());
+    if (!r.empty()) return r;
+    const nanovllm_kv_cache cache = cache_struct(c, out_dtype.value_or(c.k.scalar_type()));
+    return sizes_reason("kv_gather", nanovllm_kv_gather_check(&cache, slots.size(0)));
 }
 
 std::tuple<at::Tensor, at::Tensor> kv_gather(const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -574,7 +587,11 @@ std::string attention_prompt_reason(const at::Tensor& q, const at::Tensor& k, co
     if (cu_q.dim() != 1 || cu_q.size(0) < 1) return "cu_seqlens_q must be one-dimensional with at least one offset";
     r = index_reason("cu_seqlens_q", cu_q, at::kInt, cu_q.sizes());
     if (r.empty()) r = index_reason("cu_seqlens_k", cu_k, at::kInt, cu_q.sizes());
-    return r.empty() ? scale_reason(scale) : r;
+    if (r.empty()) r = scale_reason(scale);
+    if (!r.empty()) return r;
+    return sizes_reason("attention_prompt",
+                        nanovllm_attention_prompt_workspace_bytes(cu_q.size(0) - 1, q.size(0), k.size(0), q.size(1),
+                                                                  k.size(1), q.size(2), dtype_code(dt)));
 }
 
 at::Tensor attention_prompt(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
@@ -599,6 +616,9 @@ at::Tensor attention_prompt(const at::Tensor& q, const at::Tensor& k, const at::
     return out;
 }
 
+// Entries between rows of a block table.
+int64_t table_stride(const at::Tensor& t) { return t.size(0) > 1 && t.size(1) > 0 ? t.stride(0) : t.size(1); }
+
 std::string attention_paged_reason(const at::Tensor& q, const CacheTensors& c, const at::Tensor& tables,
                                    const at::Tensor& lens, double scale) {
     std::string r = device_reason({&q, &c.k, &c.v, &tables, &lens, optional_of(c.k_scales), optional_of(c.v_scales)});
@@ -612,8 +632,13 @@ std::string attention_paged_reason(const at::Tensor& q, const CacheTensors& c, c
     if (tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != q.size(0))
         return "block_tables must be an int32 (batch, blocks) tensor";
     if (tables.size(1) > 1 && tables.stride(1) != 1) return "block_tables must have unit stride in its last dimension";
+    if (table_stride(tables) < tables.size(1)) return "the rows of block_tables must not overlap";
     r = index_reason("context_lens", lens, at::kInt, {q.size(0)});
-    return r.empty() ? scale_reason(scale) : r;
+    if (r.empty()) r = scale_reason(scale);
+    if (!r.empty()) return r;
+    const nanovllm_kv_cache cache = cache_struct(c, q.scalar_type());
+    return sizes_reason("attention_paged",
+                        nanovllm_attention_paged_workspace_bytes(&cache, q.size(0), q.size(1), tables.size(1)));
 }
 
 at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -632,7 +657,7 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache, const
     const at::Tensor ws = bytes_like(q, need > 0 ? need : 1);
     check_rc(nanovllm_attention_paged(q.data_ptr(), &cache, static_cast<const int32_t*>(tables.data_ptr()),
                                       static_cast<const int32_t*>(lens.data_ptr()), out.data_ptr(), batch, q.size(1),
-                                      blocks, batch > 1 && blocks > 0 ? tables.stride(0) : blocks, stride_of(q, 0),
+                                      blocks, table_stride(tables), stride_of(q, 0),
                                       stride_of(q, 1), static_cast<float>(scale), dtype_code(q.scalar_type()),
                                       ws.data_ptr(), need, stream_of(q)),
              "nanovllm_attention_paged");

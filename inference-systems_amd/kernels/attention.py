@@ -61,6 +61,7 @@ from .gemm import _CODE, default_backend, register_op, run_hip, validate_gemm_ba
 _HALF = (torch.float16, torch.bfloat16)
 HEAD_DIMS = (64, 128, 256)
 GROUP = 64       # channels that share a 4-bit scale and minimum
+ROW_STRIDES = 1 << 24      # row strides of operands, in elements, are below this
 
 
 class KVCache(NamedTuple):
@@ -176,6 +177,8 @@ def _rows_reason(name: str, t: torch.Tensor, dtype, heads: Optional[int], dim: i
         return f"{name} must have unit stride in its last dimension"
     if any(x % 8 for x in _strides(t)):
         return f"the strides of {name} must be multiples of 8"
+    if _strides(t)[0] >= ROW_STRIDES:
+        return f"the row stride of {name} must be below 2^24"
     if t.numel() and t.data_ptr() % 16:
         return f"{name} must be 16-byte aligned"
     return None
@@ -211,6 +214,11 @@ def _heads_reason(q, kv_heads: int) -> Optional[str]:
     return None
 
 
+def _sizes_reason(op: str, rc: int) -> Optional[str]:
+    """The library's words for sizes it refuses (``rc`` of its check or workspace function)."""
+    return None if rc >= 0 else _lib.last_error().removeprefix(f"{op}: ")
+
+
 def rope_append_contract_reason(q, k, v, positions, cos_sin, slots, k_cache, v_cache, k_scales=None,
                                 v_scales=None) -> Optional[str]:
     """Why rope_append cannot take these inputs, or None if it can."""
@@ -233,7 +241,8 @@ def rope_append_contract_reason(q, k, v, positions, cos_sin, slots, k_cache, v_c
     rotary = cos_sin.shape[1]
     if rotary < 16 or rotary % 16 or rotary > dim:
         return f"rotary_dim ({rotary}) must be a multiple of 16 from 16 to head_dim ({dim})"
-    return None
+    cache = _cache_struct(k_cache, v_cache, k_scales, v_scales, q.dtype)
+    return _sizes_reason("rope_append", _lib.rope_append_check(cache, q.shape[0], q.shape[1]))
 
 
 def kv_gather_contract_reason(k_cache, v_cache, slots, k_scales=None, v_scales=None,
@@ -249,7 +258,11 @@ def kv_gather_contract_reason(k_cache, v_cache, slots, k_scales=None, v_scales=N
         return "out_dtype of a 4-bit cache must be float16 or bfloat16"
     if slots.dim() != 1:
         return "slots must be one-dimensional"
-    return _index_reason("slots", slots, torch.int32, slots.shape)
+    reason = _index_reason("slots", slots, torch.int32, slots.shape)
+    if reason is not None:
+        return reason
+    cache = _cache_struct(k_cache, v_cache, k_scales, v_scales, k_cache.dtype if out_dtype is None else out_dtype)
+    return _sizes_reason("kv_gather", _lib.kv_gather_check(cache, slots.shape[0]))
 
 
 def attention_prompt_contract_reason(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal=True) -> Optional[str]:
@@ -271,8 +284,15 @@ def attention_prompt_contract_reason(q, k, v, cu_seqlens_q, cu_seqlens_k, scale,
     if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1:
         return "cu_seqlens_q must be one-dimensional with at least one offset"
     reason = (_index_reason("cu_seqlens_q", cu_seqlens_q, torch.int32, cu_seqlens_q.shape)
-              or _index_reason("cu_seqlens_k", cu_seqlens_k, torch.int32, cu_seqlens_q.shape))
-    return reason or _scale_reason(scale)
+              or _index_reason("cu_seqlens_k", cu_seqlens_k, torch.int32, cu_seqlens_q.shape)
+              or _scale_reason(scale))
+    return reason or _sizes_reason("attention_prompt", _lib.attention_prompt_workspace_bytes(
+        *_prompt_sizes(q, k, cu_seqlens_q), _CODE[q.dtype]))
+
+
+def _prompt_sizes(q, k, cu_seqlens_q):
+    """(batch, q_rows, k_rows, heads, kv_heads, head_dim)."""
+    return cu_seqlens_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
 
 
 def _scale_reason(scale: float) -> Optional[str]:
@@ -300,7 +320,20 @@ def attention_paged_contract_reason(q, k_cache, v_cache, block_tables, context_l
         return "block_tables must be an int32 (batch, blocks) tensor"
     if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
         return "block_tables must have unit stride in its last dimension"
-    return _index_reason("context_lens", context_lens, torch.int32, (q.shape[0],)) or _scale_reason(scale)
+    if _table_stride(block_tables) < block_tables.shape[1]:
+        return "the rows of block_tables must not overlap"
+    reason = _index_reason("context_lens", context_lens, torch.int32, (q.shape[0],)) or _scale_reason(scale)
+    if reason is not None:
+        return reason
+    cache = _cache_struct(k_cache, v_cache, k_scales, v_scales, q.dtype)
+    return _sizes_reason("attention_paged", _lib.attention_paged_workspace_bytes(cache, *q.shape[:2],
+                                                                                 block_tables.shape[1]))
+
+
+def _table_stride(block_tables) -> int:
+    """Entries between rows of a block table."""
+    batch, blocks = block_tables.shape
+    return block_tables.stride(0) if batch > 1 and blocks else blocks
 
 
 # ---------------------------------------------------------------------------
@@ -370,7 +403,7 @@ def _attention_prompt_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     _refuse("attention_prompt", attention_prompt_contract_reason(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if q.shape[0]:
-        sizes = (cu_seqlens_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        sizes = _prompt_sizes(q, k, cu_seqlens_q)
         need = _lib.attention_prompt_workspace_bytes(*sizes, _CODE[q.dtype])
         _lib.check(need if need < 0 else _lib.OK, "nanovllm_attention_prompt_workspace_bytes")
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
@@ -397,13 +430,12 @@ def _attention_paged_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if batch:
         cache = _cache_struct(k_cache, v_cache, k_scales, v_scales, q.dtype)
         blocks = block_tables.shape[1]
-        stride = block_tables.stride(0) if batch > 1 and blocks else blocks
         need = _lib.attention_paged_workspace_bytes(cache, batch, heads, blocks)
         _lib.check(need if need < 0 else _lib.OK, "nanovllm_attention_paged_workspace_bytes")
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         with torch.cuda.device(q.device):
             _lib.attention_paged_raw(q.data_ptr(), cache, block_tables.data_ptr(), context_lens.data_ptr(),
-                                     out.data_ptr(), batch, heads, blocks, stride, *_strides(q), float(scale),
+                                     out.data_ptr(), batch, heads, blocks, _table_stride(block_tables), *_strides(q), float(scale),
                                      _CODE[q.dtype], workspace.data_ptr(), need,
                                      torch.cuda.current_stream(q.device).cuda_stream)
     return out
@@ -590,8 +622,15 @@ def _torch_attention_paged(q, k_cache, v_cache, block_tables, context_lens, scal
 
 def _switch(op, plain, reason, backend: Optional[str], *args):
     backend = validate_gemm_backend(backend) if backend is not None else default_backend()
-    if backend == "hip" or (backend == "auto" and reason(*args) is None):
+    if backend == "hip":
         return run_hip(op, reason, *args)
+    if backend == "auto" and all(t.is_cuda for t in args if isinstance(t, torch.Tensor)):
+        # The op checks its contract itself, before it launches or writes anything.
+        try:
+            return op(*args)
+        except RuntimeError:
+            if reason(*args) is None:
+                raise
     return plain(*args)
 
 
