@@ -113,8 +113,10 @@ int nanovllm_kv_gather_check(const nanovllm_kv_cache* cache, int64_t rows);
  * keys cu_k[b] .. cu_k[b + 1] (batch + 1 offsets each, not decreasing, the
  * first of cu_q 0); its row i attends to key j where causal is 0 or
  * j <= i + (keys - queries), so the last query sees every key.
- * out = softmax(scale q k^T) v, fp32 sums, rounded once; a row with no key to
- * attend to is 0, and so are rows behind the last sequence.  q, k, v as in
+ * out = softmax(scale q k^T) v; a row with no key to attend to is 0, and so are
+ * rows behind the last sequence.  Scores, maxima, totals and sums are fp32; the
+ * weights are rounded to dtype before they multiply v (the total is that of the
+ * rounded ones), and out is rounded once.  q, k, v as in
  * nanovllm_rope_append; out is [q_rows, heads, head_dim], contiguous.
  * Workspace: nanovllm_attention_prompt_workspace_bytes() bytes, 16-byte
  * aligned scratch.
@@ -139,7 +141,9 @@ int64_t nanovllm_attention_prompt_workspace_bytes(int64_t batch, int64_t q_rows,
  * tables[b, 0 .. table_blocks) (row stride table_stride, in entries).  Page
  * sizes are multiples of 16, and a table holds at most 2^31 - 1024 tokens.  No
  * token: 0.  A page number outside the cache, or a length behind the table,
- * makes the sequence's output NaN.  q is [batch, heads, head_dim] with strides
+ * makes the sequence's output NaN.  Roundings as above on 16-bit pages; on 4-bit
+ * ones weights, weights times scales, and minimum + 7.5 scale are rounded to
+ * float16, whatever the dtype of q.  q is [batch, heads, head_dim] with strides
  * as above, out contiguous.  Workspace:
  * nanovllm_attention_paged_workspace_bytes() bytes, 16-byte aligned scratch.
  */

@@ -22,7 +22,8 @@
 //   product adds up P (m_g + 7.5 s_g) and P.  Around its middle a group's values
 //   are small, so the roundings of P s_g and P weigh as much as they would on
 //   the values themselves (131072 tokens, fp16: 6.2e-4 off with c and m_g
-//   taken apart and 1024 + c, 2.8e-4 so).
+//   taken apart and 1024 + c, 2.8e-4 so).  P is held 2^10 fold in fp16 (here and in
+//   16-bit fp16 pages), so that P, or P s_g, is lost below 2^-35 of the largest P.
 //
 // The work is split over a fixed grid: all (sequence, key-value head) pairs in
 // units of 128 tokens, laid end to end, each workgroup an equal run of units.
@@ -93,12 +94,13 @@ __device__ __forceinline__ Units all_units(const Split& s) {
 }
 
 // Units of a workgroup's run.  16-bit pages are bound by HBM, and where there is
-// work for it half of the workgroups that fit stream it better and leave half of
-// the parts: at 32 sequences of 4100 tokens 64.7 -> 57.9 us (2 heads of 256), 62.4
-// -> 57.7 (4 of 128), 68.5 -> 63.4 (8 of 64); 40 of 3000 63.5 -> 55.1, 56.4 -> 57.7,
-// 55.5 -> 56.7.  Where there is little, their number is what keeps loads in
-// flight: 32 ragged sequences (64 pairs of 8 units or so) 27.8 us, 33.9 on half.
-// Pages of 4 bits wait on the arithmetic and take all that fit.
+// work for it half of the grid (at head_dim 256 as many workgroups as fit at once)
+// stream it better and leave half of the parts: 32 sequences of 4100 tokens 64.7 ->
+// 57.9 us (2 heads of 256), 62.4 -> 57.7 (4 of 128), 68.5 -> 63.4 (8 of 64); at 128
+// and 64 not for every batch: 40 of 3000 63.5 -> 55.1, 56.4 -> 57.7, 55.5 -> 56.7.
+// Where there is little, their number is what keeps loads in flight: 32 ragged
+// sequences (64 pairs of 8 units or so) 27.8 us, 33.9 on half.  Pages of 4 bits wait
+// on the arithmetic and take the whole grid.
 __device__ __forceinline__ int units_per_group(const Split& s, int total) {
     const int groups = total >= s.many ? s.grid / 2 : s.grid;
     return (total + groups - 1) / groups;
@@ -837,7 +839,10 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const Split s
     }
 }
 
-// Workgroups that the chip runs at once, by the registers of a kernel.
+// Workgroups of a grid that has work for all of them, 2 to 4 a CU.  By the registers
+// of its kernel a CU runs 4 at once at head_dim 64, 3 at 128, and at 256 2 in 4 bits
+// and 1 in 16.  16 bits take 2 a CU at 128 and at 256, where half of them run at
+// first; large calls take half of the grid (units_per_group).
 int resident(int head_dim, int bits) {
     const int per_cu = head_dim == 64 ? 4 : head_dim == 128 ? (bits == 4 ? 3 : 2) : 2;
     return 256 * per_cu;

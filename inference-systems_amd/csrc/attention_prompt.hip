@@ -12,17 +12,18 @@
 // V^T is read from LDS transposed (ds_read_b64_tr_b16), 4 keys of a channel at
 // a time, which is the run of keys a lane's accumulators hold.
 //
-// Short blocks, and many, have a workgroup each.  The others (see in_runs) are
-// split over a fixed grid: all (sequence, head, 128 queries) blocks in units of
-// one tile of keys, laid end to end, each workgroup an equal run of units; a
-// block starts with six units that hold no key and stand for what it costs to
+// Many blocks, and the short ones of one sequence, have a workgroup each.  The
+// others (see in_runs: of several sequences the host knows only the sum of keys, so
+// short ones are among them) are split over a fixed grid: all (sequence, head, 128
+// queries) blocks in units of one tile of keys, laid end to end, each workgroup an
+// equal run of units; a block starts with six units that hold no key and stand for what it costs to
 // begin one.  So a causal prompt's long rows and short ones, a few queries
 // against many keys, and sequences of any lengths load the chip evenly.  A block
 // whose keys lie in one run is finished there; the parts of others go to a
 // workspace (at most two per workgroup) and a second kernel joins them.
 //
 // Bound by the matrix cores, which run at the chip's power limit: on MI355X 16384
-// tokens of 8 heads of 256 take 1121-1145 us, 960-980 TFLOP/s (a large library
+// tokens of 8 heads of 256 take 1121-1147 us, 960-980 TFLOP/s (a large library
 // product 1265; the products alone 807 us); a chunk of 512 behind 8188 cached
 // tokens, 32 heads of 128, 85-88 us, 12 of them in the join; 2048 tokens of 8
 // heads of 256 48 us, 18 of them for the traffic of 35 MB of parts.

@@ -5,12 +5,12 @@
 // (token, head) is taken by head_dim / 8 lanes of 8 channels each, so a lane
 // reads and writes 16-byte chunks and the 64 channels of a 4-bit group are 8
 // neighbouring lanes.  Measured on MI355X (a large copy: 5.1 TB/s): 8000 tokens
-// of 16 + 2 x 4 heads of 128 into a 4-bit cache 23 us for 101 MB, 4.4 TB/s (a row
+// of 16 + 2 x 4 heads of 128 into a 4-bit cache 23-24 us for 101 MB, 4.3 TB/s (a row
 // a team, with its own cosines and divisions: 49 us); 20000 tokens of 8 + 2 x 2
-// heads of 256, 16 bits, 45 us; one token 2.6 us.  Rows of 4 + 4 heads of 128
-// gathered: 20000 from 16-bit pages 13 us, partly from the last-level cache, 8000
-// and 20000 from 4-bit ones 6.6 and 13.2 us (values by a team a row, three of four
-// of them idle: 9.2 and 19.1 us).
+// heads of 256, 16 bits, 45 us for 272 MB, partly through the last-level cache; one
+// token 2.6 us.  Rows of 4 + 4 heads of 128 gathered: 20000 from 16-bit pages 13 us,
+// partly from the last-level cache, 8000 and 20000 from 4-bit ones 6.6 and 13.2 us
+// (values by a team a row, three of four of them idle: 9.2 and 19.1 us).
 #include <type_traits>
 
 #include "attention_common.hpp"

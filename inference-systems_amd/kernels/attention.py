@@ -31,11 +31,17 @@ nanovllm/layers/attention.py, nanovllm/layers/rotary_embedding.py).
         tokens.  A page number outside the cache, or a length behind the
         table, makes a sequence's output NaN.
 
+Scores, softmax statistics and sums are held in 32 bits.  Weights are rounded
+to q's type before they multiply the values (their total is of the rounded
+ones); next to 4-bit values weights, weights times scales and the middle of a
+group are rounded to float16.  Errors are up to 1.5 times those of a softmax
+that stays in 32 bits.
+
 Types: float16 or bfloat16, D of 64, 128 or 256, H a multiple of KV.  q, k and
 v may be strided views (a column range of one projection) with unit stride in
 the last dimension, and strides that are multiples of 8, that of rows below
 2^24.  ``positions`` is int64, the other index tensors int32,
-``cos_sin`` float32.
+``cos_sin`` float32.  A block table holds at most 2^31 - 1024 tokens.
 
 A paged cache (``new_kv_cache``) holds 16-bit elements, [blocks, block_size,
 KV, D] for keys and for values, or 4-bit codes with a float16 scale and minimum
