@@ -498,7 +498,15 @@ __global__ __launch_bounds__(256, D == 256 && BITS == 16 ? 1 : 2) void attention
                 }
                 extra *= down;
             }
-            const float shift = (m == -__builtin_inff() ? 0.0f : m * s.a.c) - boost;
+            const float base = m == -__builtin_inff() ? 0.0f : m;
+            float shift = base * s.a.c - boost;
+            if (__ballot(fabsf(base) * s.a.c > kFarScore)) {
+                shift = -boost;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[h][i] -= base;
+            }
             float p[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h)

@@ -258,7 +258,7 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
 // channels 8 i + 4 half + 0..3.
 template <int DT, int D>
 __device__ __forceinline__ void add_keys(const PromptArgs& p, const uint16_t* qrow, const uint16_t* kbase,
-                                         const uint16_t* vbase, int key0, int key1, int last, int half, float shift,
+                                         const uint16_t* vbase, int key0, int key1, int last, int half, float base,
                                          float* sums) {
     for (int j = key0; j < key1; ++j) {
         const uint16_t* vrow = vbase + int64_t(j) * p.v_row;
@@ -275,7 +275,7 @@ __device__ __forceinline__ void add_keys(const PromptArgs& p, const uint16_t* qr
 #pragma unroll
             for (int w = 0; w < 4; ++w) s = dot2<DT>(a[w], b[w], s);
         }
-        const float pj = exp2_hw(__builtin_fmaf(s, p.c, -shift));
+        const float pj = exp2_hw(__builtin_fmaf(s - base, p.c, kBoost<DT>));
         for (int ch = 4 * half; ch < D; ch += 8)
             for (int i = ch; i < ch + 4; ++i)
                 if (!finite1<DT>(vrow[i])) sums[i] = __builtin_fmaf(pj, half_to_f32<DT>(vrow[i]), sums[i]);
@@ -485,7 +485,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
 #pragma unroll
                 for (int i = 0; i < DTILES; ++i) o[i] *= down;
             }
-            const float shift = (m == -__builtin_inff() ? 0.0f : m * p.c) - kBoost<DT>;
+            const float base = m == -__builtin_inff() ? 0.0f : m;
+            float shift = base * p.c - kBoost<DT>;
+            if (__ballot(fabsf(base) * p.c > kFarScore)) {
+                shift = -kBoost<DT>;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) sc[n][v] -= base;
+            }
             const uint32_t v_at = v_read + (t & 1) * TILE;
             u32x4_t vf[2][DTILES];      // values of 16 keys, and of the next 16
             auto read = [&](int g, int i) {
@@ -573,10 +581,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                 for (int v = 0; v < 16; v += 4)
                     *reinterpret_cast<f32x4_t*>(sums + 32 * i + 2 * v + 4 * half) =
                         f32x4_t{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]};
-            const float shift = (m == -__builtin_inff() ? 0.0f : m * p.c) - kBoost<DT>;
+            const float base = m == -__builtin_inff() ? 0.0f : m;
             for (int t = full; t < t1; ++t)
                 if (late >> (t - full) & 1)
-                    add_keys<DT, D>(p, qrow, kbase, vbase, t * kKeys, min(lk, t * kKeys + kKeys), last, half, shift, sums);
+                    add_keys<DT, D>(p, qrow, kbase, vbase, t * kKeys, min(lk, t * kKeys + kKeys), last, half, base, sums);
             for (int ch = 4 * half; ch < D; ch += 8) store(ch, *reinterpret_cast<const f32x4_t*>(sums + ch));
         }
         if (unit >= end) break;
