@@ -10,6 +10,8 @@
 //   O^T[channel, head] += V^T P  contraction over tokens: the order of the
 //                                accumulators of S^T is taken as the order of the
 //                                contraction, so P is packed where it is
+// P is rounded to the operands' type for its product, and its total is that of the
+// rounded P: 0.0021 off in bf16 against 64 bits, 0.0017 with P in fp32.
 // V^T needs 8 tokens of one channel per lane.  16-bit pages give that by a
 // 2 x 2 transposition in registers, 4-bit pages by their layout (4 tokens of a
 // channel in one word).
