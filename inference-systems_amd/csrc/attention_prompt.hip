@@ -20,10 +20,10 @@
 // others (see in_runs: of several sequences the host knows only the sum of keys, so
 // short ones are among them) are split over a fixed grid: all (sequence, head, 128
 // queries) blocks in units of one tile of keys, laid end to end, each workgroup an
-// equal run of units; a block starts with six units that hold no key and stand for what it costs to
-// begin one.  So a causal prompt's long rows and short ones, a few queries
-// against many keys, and sequences of any lengths load the chip evenly.  A block
-// whose keys lie in one run is finished there; the parts of others go to a
+// equal run of units; a block starts with six units that hold no key and stand for
+// what it costs to begin one.  So a causal prompt's long rows and short ones, a few
+// queries against many keys, and sequences of any lengths load the chip evenly.  A
+// block whose keys lie in one run is finished there; the parts of others go to a
 // workspace (at most two per workgroup) and a second kernel joins them.
 //
 // Bound by the matrix cores, which run at the chip's power limit: on MI355X 16384

@@ -441,8 +441,8 @@ def _attention_paged_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         with torch.cuda.device(q.device):
             _lib.attention_paged_raw(q.data_ptr(), cache, block_tables.data_ptr(), context_lens.data_ptr(),
-                                     out.data_ptr(), batch, heads, blocks, _table_stride(block_tables), *_strides(q), float(scale),
-                                     _CODE[q.dtype], workspace.data_ptr(), need,
+                                     out.data_ptr(), batch, heads, blocks, _table_stride(block_tables), *_strides(q),
+                                     float(scale), _CODE[q.dtype], workspace.data_ptr(), need,
                                      torch.cuda.current_stream(q.device).cuda_stream)
     return out
 
