@@ -1,5 +1,5 @@
-"""ctypes binding of libnanovllm_gemm.so (declared in include/nanovllm_gemm.h
-and include/nanovllm_attention.h).
+"""ctypes binding of libnanovllm_gemm.so (declared in include/nanovllm_gemm.h,
+nanovllm_attention.h, nanovllm_int8.h and nanovllm_sampling.h).
 
 The loader mirrors the reference's ``load_cuda_ops``
 (nanovllm/kernels/_extension.py:36-68) in spirit: one cached load of a
@@ -85,6 +85,11 @@ SIGNATURES = {
     "nanovllm_attention_prompt_workspace_bytes": (_I64, [_I64] * 6 + [_INT]),
     "nanovllm_attention_paged": (_INT, [_VP, _CACHE, _VP, _VP, _VP] + [_I64] * 6 + [_F32, _INT, _VP, _I64, _VP]),
     "nanovllm_attention_paged_workspace_bytes": (_I64, [_CACHE, _I64, _I64, _I64]),
+    "nanovllm_quantize_rows": (_INT, [_VP, _VP, _VP, _I64, _I64, _I64, _INT, _VP]),
+    "nanovllm_add_rmsnorm_quantize": (_INT, [_VP, _VP, _VP, _F32, _VP, _VP, _VP] + [_I64] * 4 + [_INT, _VP]),
+    "nanovllm_gemm_int8": (_INT, [_VP] * 5 + [_I64] * 6 + [_INT, _INT, _VP]),
+    "nanovllm_sample_logits": (_INT, [_VP] * 8 + [_I64] * 3 + [_INT, _VP, _I64, _VP]),
+    "nanovllm_sample_logits_workspace_bytes": (_I64, [_I64, _I64, _INT]),
     "nanovllm_gemm_kernel_name": (ctypes.c_char_p, [_INT]),
     "nanovllm_gemm_last_error": (ctypes.c_char_p, []),
     "nanovllm_gemm_last_kernel": (ctypes.c_char_p, []),
@@ -321,3 +326,36 @@ def attention_paged_raw(q_ptr, cache, tables_ptr, lens_ptr, out_ptr, batch, head
     check(load().nanovllm_attention_paged(q_ptr, cache, tables_ptr, lens_ptr, out_ptr, batch, heads, table_blocks,
                                           table_stride, q_row, q_head, scale, dtype, ws_ptr, ws_bytes, stream),
           "nanovllm_attention_paged")
+
+
+def quantize_rows_raw(x_ptr, codes_ptr, scales_ptr, m, k, ldx, dtype, stream) -> None:
+    """Enqueue the rows' quantisation to 8 bits on `stream`; raise on error."""
+    check(load().nanovllm_quantize_rows(x_ptr, codes_ptr, scales_ptr, m, k, ldx, dtype, stream),
+          "nanovllm_quantize_rows")
+
+
+def add_rmsnorm_quantize_raw(h_ptr, r_ptr, w_ptr, eps, codes_ptr, scales_ptr, res_ptr, m, k, ldh, ldr, dtype,
+                             stream) -> None:
+    """Enqueue the residual add and RMSNorm with the rows in 8 bits on `stream`; raise on error."""
+    check(load().nanovllm_add_rmsnorm_quantize(h_ptr, r_ptr, w_ptr, eps, codes_ptr, scales_ptr, res_ptr, m, k, ldh,
+                                               ldr, dtype, stream), "nanovllm_add_rmsnorm_quantize")
+
+
+def gemm_int8_raw(a_ptr, a_scales_ptr, w_ptr, w_scales_ptr, c_ptr, m, n, k, lda, ldw, ldc, silu_mul, dtype_out,
+                  stream) -> None:
+    """Enqueue the 8-bit GEMM on `stream`; raise on error."""
+    check(load().nanovllm_gemm_int8(a_ptr, a_scales_ptr, w_ptr, w_scales_ptr, c_ptr, m, n, k, lda, ldw, ldc,
+                                    int(silu_mul), dtype_out, stream), "nanovllm_gemm_int8")
+
+
+def sample_logits_workspace_bytes(m, vocab, dtype) -> int:
+    """Workspace bytes of the sampler on logits (negative code if invalid)."""
+    return load().nanovllm_sample_logits_workspace_bytes(m, vocab, dtype)
+
+
+def sample_logits_raw(logits_ptr, temperatures_ptr, uniforms_ptr, top_k_ptr, top_p_ptr, min_p_ptr, tokens_ptr,
+                      logprobs_ptr, m, vocab, ld, dtype, ws_ptr, ws_bytes, stream) -> None:
+    """Enqueue the sampler on logits on `stream`; raise on error."""
+    check(load().nanovllm_sample_logits(logits_ptr, temperatures_ptr, uniforms_ptr, top_k_ptr, top_p_ptr, min_p_ptr,
+                                        tokens_ptr, logprobs_ptr, m, vocab, ld, dtype, ws_ptr, ws_bytes, stream),
+          "nanovllm_sample_logits")

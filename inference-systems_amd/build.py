@@ -14,8 +14,8 @@ kernel-resource-usage remarks (with a rocprofv3 kernel-stats CSV: per family,
 and for each kernel that run launched).
 
 ``build(sanitize=True, out=path)`` (``build.py --sanitize PATH``) builds a
-copy whose host code in capi.cpp and capi_attention.cpp (argument validation, the
-selection table, workspace sizes, error reporting) carries AddressSanitizer and
+copy whose host code in capi.cpp, capi_attention.cpp and capi_int8.cpp (argument
+validation, the selection table, workspace sizes, error reporting) carries AddressSanitizer and
 UndefinedBehaviorSanitizer; device code is built as usual.  It is loaded
 through ``NANOVLLM_GEMM_LIB`` with the sanitizer runtime preloaded
 (``sanitizer_runtime()``), for the CPU tests of the C ABI.
@@ -68,6 +68,10 @@ SOURCES = [
     "kv_cache.hip",
     "attention_prompt.hip",
     "attention_paged.hip",
+    "capi_int8.cpp",
+    "quantize.hip",
+    "gemm_int8.hip",
+    "sample_logits.hip",
 ]
 
 # attention_prompt.hip: a kernel of head_dim 256 has more than 256 registers, and
@@ -101,7 +105,7 @@ SANITIZE_FLAGS = [
     "-Xarch_host", "-fno-omit-frame-pointer",
     "-Xarch_host", "-g",
 ]
-SANITIZED_SOURCES = ("capi.cpp", "capi_attention.cpp")
+SANITIZED_SOURCES = ("capi.cpp", "capi_attention.cpp", "capi_int8.cpp")
 
 
 def sanitizer_runtime() -> Path:

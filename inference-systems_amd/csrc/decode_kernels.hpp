@@ -71,7 +71,8 @@ template <int DT, int DT_OUT, int AROWS, int RG, int WAVES, int LPB, int PARTS, 
 __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
     const uint16_t* __restrict__ a, const uint16_t* __restrict__ w, void* __restrict__ c,
     int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int64_t ldc, uint64_t* __restrict__ keys,
-    ProArgs pro, SampleArgs sa) {
+    ProArgs pro, SampleArgs sa, const float* __restrict__ row_scale, const float* __restrict__ col_scale,
+    int dtype_out) {
     static_assert(AROWS == 8 || AROWS == 16 || AROWS == 32 || AROWS == 64, "rows of A per line");
     constexpr int MG = AROWS == 8 ? 1 : AROWS / 16;   // 16-row groups of A in the MFMA
     constexpr int IW = 2 * RG;                 // W copies per line (8 rows each)
@@ -83,6 +84,9 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
     constexpr int IL = IW + IA + IP;
     static_assert(PRO == PRO_NONE || EPI == EPI_NONE || (PRO == PRO_ADD_NORM && EPI == EPI_SILU_MUL),
                   "prologues come with the plain store (and the norm also with SiLU-and-mul)");
+    // The 8-bit form is built once for all output types (DT_OUT is kI8 too).
+    static_assert((DT == kI8) == (DT_OUT == kI8), "int8: the output type is an argument");
+    static_assert(DT != kI8 || (PRO == PRO_NONE && EPI != EPI_ARGMAX && !KN), "int8: stored sums of W[N,K]");
     static_assert(!KN || (RG == 4 && EPI == EPI_NONE && PRO == PRO_NONE), "B[K,N]: 64 columns, plain store");
     static_assert(LPB * IL < 64, "vmcnt range");
     static_assert(PARTS % WAVES == 0, "whole partitions per wave");
@@ -115,9 +119,11 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
         nblk += kNumXcd * blockIdx.z;
         const int64_t row0 = int64_t(blockIdx.y) * AROWS;
         a += row0 * lda;
-        c = static_cast<char*>(c) + row0 * ldc * (DT_OUT == NANOVLLM_GEMM_F32 ? 4 : 2);
+        const int out = DT == kI8 ? dtype_out : DT_OUT;
+        c = static_cast<char*>(c) + row0 * ldc * (out == NANOVLLM_GEMM_F32 ? 4 : 2);
         m = min_i64(m - row0, AROWS);
         if constexpr (PRO != PRO_NONE) pro.a2 += row0 * pro.lda2;
+        if constexpr (DT == kI8) row_scale += row0;
         if constexpr (PRO == PRO_ADD_NORM) pro.res_out += row0 * pro.ldres;
     }
 
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
 
     const int64_t lines = (k + kLine - 1) / kLine;
     const uint32_t base = lds_address(&buf[wave][0]);
-    f32x4_t acc[PW][RG][MG];
+    acc4_t<DT> acc[PW][RG][MG];
     // PRO_ADD_NORM: this lane's sum of s^2 for its fragment rows.
     float ss[MG];
 #pragma unroll
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
 #pragma unroll
         for (int r = 0; r < RG; ++r)
 #pragma unroll
-            for (int g = 0; g < MG; ++g) acc[q][r][g] = f32x4_t{};
+            for (int g = 0; g < MG; ++g) acc[q][r][g] = acc4_t<DT>{};
 
     // EPI_ARGMAX: thread x ranks row x / ETPR of A.  On a sampled head the
     // noise of its columns (log2 E, which does not depend on the logits) is
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
                     for (int r = 0; r < RG; ++r)
 #pragma unroll
                         for (int g = 0; g < MG; ++g)
-                            acc[q][r][g] = mfma_16x16x32<DT>(wf[r], af[g], acc[q][r][g]);
+                            acc[q][r][g] = mma_16<DT>(wf[r], af[g], acc[q][r][g]);
                 }
             }
             // The next lines' copies overwrite the slots just read.
@@ -421,8 +427,9 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
     // 16 n and 4 consecutive m) each touch 64 distinct banks.  (With
     // 16 n + (m ^ n) the writes touched 16 banks, four lanes each: the
     // bank-conflict stalls the counters showed.)
-    auto part = [&](int wv, int q, int r, int g, int nn, int mm) -> float& {
-        return reinterpret_cast<float*>(&buf[wv][0])[((q * RG + r) * MG + g) * 256 + 64 * (nn & 3) + 16 * (nn >> 2) +
+    using sum_t = std::conditional_t<DT == kI8, int32_t, float>;
+    auto part = [&](int wv, int q, int r, int g, int nn, int mm) -> sum_t& {
+        return reinterpret_cast<sum_t*>(&buf[wv][0])[((q * RG + r) * MG + g) * 256 + 64 * (nn & 3) + 16 * (nn >> 2) +
                                                      (mm ^ (4 * (nn & 3)))];
     };
 #pragma unroll
@@ -447,7 +454,7 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
     __syncthreads();
     // Sum of the partitions in partition order.
     auto total = [&](int r, int g, int nn, int mm) {
-        float sum = part(0, 0, r, g, nn, mm);
+        sum_t sum = part(0, 0, r, g, nn, mm);
 #pragma unroll
         for (int pp = 1; pp < PARTS; ++pp) sum += part(pp % WAVES, pp / WAVES, r, g, nn, mm);
         return sum;
@@ -521,7 +528,15 @@ __global__ __launch_bounds__(WAVES * 64) void splitk_decode_kernel(
             for (int wv = 1; wv < WAVES; ++wv) sum_sq += sspart[wv][row];
             rs = norm_scale(sum_sq, k, pro.eps);
         }
-        if constexpr (EPI == EPI_SILU_MUL) {
+        if constexpr (DT == kI8) {
+            const float ri = row_scale[row];
+            float x = static_cast<float>(total(EPI == EPI_SILU_MUL ? 2 * o : o, g, nn, mm)) * col_scale[col] * ri;
+            if constexpr (EPI == EPI_SILU_MUL)
+                x = silu_f32(x) * (static_cast<float>(total(2 * o + 1, g, nn, mm)) * col_scale[n + col] * ri);
+            if (dtype_out == NANOVLLM_GEMM_F32) store_elem<NANOVLLM_GEMM_F32>(c, row * ldc + col, x);
+            else if (dtype_out == NANOVLLM_GEMM_F16) store_elem<NANOVLLM_GEMM_F16>(c, row * ldc + col, x);
+            else store_elem<NANOVLLM_GEMM_BF16>(c, row * ldc + col, x);
+        } else if constexpr (EPI == EPI_SILU_MUL) {
             float gate = total(2 * o, g, nn, mm), up = total(2 * o + 1, g, nn, mm);
             if constexpr (PRO == PRO_ADD_NORM) {
                 gate *= rs;
@@ -554,7 +569,7 @@ int launch_cfg(const Problem& p, hipStream_t s) {
     hipLaunchKernelGGL((splitk_decode_kernel<DT, DT_OUT, AROWS, RG, WAVES, LPB, PARTS, EPI, PRO, KN, AREG, RB>),
                        grid, block, 0, s,
                        static_cast<const uint16_t*>(p.a), static_cast<const uint16_t*>(p.b), p.c, p.m, p.n, p.k,
-                       p.lda, p.ldb, p.ldc, p.keys, pro, p.sample);
+                       p.lda, p.ldb, p.ldc, p.keys, pro, p.sample, p.row_scale, p.col_scale, p.dtype_out);
     return check_launch("splitk_decode", AROWS, 16 * OG);
 }
 

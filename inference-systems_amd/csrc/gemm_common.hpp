@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/nanovllm_gemm.h"
 
 namespace nvg {
@@ -16,6 +18,21 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+typedef int32_t i32x16_t __attribute__((ext_vector_type(16)));
+
+// dtype_in of the 8-bit integer GEMMs (nanovllm_int8.h), inside the library
+// only.  Their operands travel as pairs of bytes: k, lda and ldb of a Problem
+// count 16-bit units, so a K-tile of 64 units is 128 codes and every copy, LDS
+// place and fragment is that of a bf16 GEMM; the matrix instruction takes twice
+// the K in the same time, and sums in int32, which is exact.
+constexpr int kI8 = 3;
+
+// Row scales of an output tile (RS of the kernels below): none, one per row of
+// A, or one per row of A and one per row of W.
+constexpr int RS_NONE = 0;
+constexpr int RS_ROW = 1;
+constexpr int RS_BOTH = 2;
 
 // Output epilogues.  EPI_NONE stores the product.  EPI_SILU_MUL is the fused
 // SiluAndMul of a gate/up projection: W = [W_gate; W_up] has 2n rows, output
@@ -69,6 +86,7 @@ struct Problem {
     SampleArgs sample;                // EPI_ARGMAX: per-row temperatures and noise (sampled LM head)
     const float* row_scale = nullptr; // mfma_staged, EPI_NONE / EPI_SILU_MUL: output row i (both
                                       // sums of a SiLU pair) times row_scale[i] before rounding
+    const float* col_scale = nullptr; // kI8: the sum of row j of b times col_scale[j] (and row_scale[i])
     int pro = PRO_NONE;
     // PRO_GATE: gate element (i, k) at a2[i * lda2 + (k / group) * group_stride + k % group].
     // PRO_ADD_NORM: residual r[i, k] at a2[i * lda2 + k]; norm weight norm_w[k];
@@ -162,11 +180,74 @@ __device__ __forceinline__ f32x4_t mfma_16x16x32(u32x4_t a, u32x4_t b, f32x4_t c
     }
 }
 
+// The same with 16 packed int8 values per lane and int32 sums: lane l holds
+// k = 16 (l / 32 or l / 16) + [0, 16); the places of the sums are those above.
+template <int DT>
+using acc4_t = std::conditional_t<DT == kI8, i32x4_t, f32x4_t>;
+template <int DT>
+using acc16_t = std::conditional_t<DT == kI8, i32x16_t, f32x16_t>;
+
+template <int DT>
+__device__ __forceinline__ acc16_t<DT> mma_32(u32x4_t a, u32x4_t b, acc16_t<DT> c) {
+    if constexpr (DT == kI8) {
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0,
+                                                     0, 0);
+    } else {
+        return mfma_32x32x16<DT>(a, b, c);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ acc4_t<DT> mma_16(u32x4_t a, u32x4_t b, acc4_t<DT> c) {
+    if constexpr (DT == kI8) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0,
+                                                     0, 0);
+    } else {
+        return mfma_16x16x32<DT>(a, b, c);
+    }
+}
+
+// Four sums of one output row as fp32, scaled: by the row (rs), or by the row
+// and each column (cs).  An int32 sum is rounded to fp32 once (it is exact up
+// to 2^24), each scale rounds once more.
+template <int RS, typename V>
+__device__ __forceinline__ f32x4_t scaled4(V v, float rs, f32x4_t cs) {
+    if constexpr (RS == RS_BOTH) {
+        f32x4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(v[i]) * cs[i] * rs;
+        return x;
+    } else {
+        if constexpr (RS == RS_ROW) v *= rs;
+        return v;
+    }
+}
+
+// Column scales of output columns col .. col + 3 (of n; those past it repeat
+// the last).
+__device__ __forceinline__ f32x4_t col_scales4(const float* col_scale, int64_t col, int64_t n) {
+    f32x4_t s;
+    if (col + 4 <= n) {
+        __builtin_memcpy(&s, col_scale + col, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = col_scale[col + i < n ? col + i : n - 1];
+    }
+    return s;
+}
+
 // s_waitcnt vmcnt(N) alone (expcnt and lgkmcnt left at their no-wait maximum).
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
     static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// A pointer that is the same in every lane, in scalar registers.
+__device__ __forceinline__ const uint16_t* scalar_pointer(const uint16_t* p) {
+    const uint64_t v = reinterpret_cast<uintptr_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+    return reinterpret_cast<const uint16_t*>((uint64_t(hi) << 32) | lo);
 }
 
 // LDS byte address of a pointer into a __shared__ array.

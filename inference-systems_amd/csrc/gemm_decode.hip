@@ -291,6 +291,8 @@ int launch_kn(const Problem& p, hipStream_t s) {
 }  // namespace
 
 int launch_splitk_decode(const Problem& p, hipStream_t s) {
+    if (p.dtype_in == kI8)
+        return p.epi == EPI_SILU_MUL ? launch_epi<kI8, kI8, EPI_SILU_MUL>(p, s) : launch_epi<kI8, kI8, EPI_NONE>(p, s);
     if (p.b_layout == NANOVLLM_GEMM_B_KN) {
         if (p.epi != EPI_NONE || p.pro != PRO_NONE)
             return set_error(NANOVLLM_GEMM_EUNSUPPORTED, "splitk_decode: B[K,N] takes the plain GEMM only");

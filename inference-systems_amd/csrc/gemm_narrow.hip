@@ -33,7 +33,8 @@ __device__ __forceinline__ int panel_swizzle(int r) { return 2 * (((r >> 1) & 1)
 template <int DT, int DT_OUT, int BM, int BN, int KS, int WGM, int WGN, int STAGES, int EPI, int RS, int KN>
 __global__ __launch_bounds__(WGM * WGN * 64) void mfma_narrow_kernel(
     const uint16_t* __restrict__ a, const uint16_t* __restrict__ w, int64_t m, int64_t n, int64_t k, int64_t lda,
-    int64_t ldb, void* __restrict__ c, int64_t ldc, int c_vec, const float* __restrict__ row_scale) {
+    int64_t ldb, void* __restrict__ c, int64_t ldc, int c_vec, const float* __restrict__ row_scale,
+    const float* __restrict__ col_scale) {
     constexpr int NW = WGM * WGN, NT = NW * 64;
     constexpr int BK = 64 * KS;
     constexpr int BNO = EPI == EPI_SILU_MUL ? BN / 2 : BN;
@@ -120,15 +121,16 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_narrow_kernel(
         }
     };
 
-    f32x4_t acc[NI][MI];
+    acc4_t<DT> acc[NI][MI];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) acc[i][j] = f32x4_t{};
+        for (int j = 0; j < MI; ++j) acc[i][j] = acc4_t<DT>{};
 
 #pragma unroll
     for (int t = 0; t < AHEAD; ++t) issue(t, t);
     asm volatile("" :: "s"(c), "s"(ldc), "s"(c_vec), "s"(m), "s"(n), "s"(row_scale));
+    if constexpr (RS == RS_BOTH) asm volatile("" :: "s"(col_scale));
 
     const int swz = (r16 >> 1) & 7;
     auto read_step = [&](const u32x4_t* tile, int s, u32x4_t (&af)[MI], u32x4_t (&wf)[NI]) {
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_narrow_kernel(
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < MI; ++j) acc[i][j] = mfma_16x16x32<DT>(wf[s][i], af[s][j], acc[i][j]);
+                for (int j = 0; j < MI; ++j) acc[i][j] = mma_16<DT>(wf[s][i], af[s][j], acc[i][j]);
         cur = cur + 1 == STAGES ? 0 : cur + 1;
     }
     wait_vmcnt<0>();   // copies of zeros past the last K-tile
@@ -192,11 +194,19 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_narrow_kernel(
         if constexpr (RS) rs = row_scale[min_i64(m0 + row, m - 1)];
 #pragma unroll
         for (int i = 0; i < NJ; ++i) {
-            f32x4_t x = acc[EPI == EPI_SILU_MUL ? 2 * i : i][j];
-            if constexpr (RS) x *= rs;
+            f32x4_t x, u;
+            if constexpr (RS == RS_BOTH) {
+                const int64_t col = n0 + wn * 16 * NJ + 16 * i + 4 * quad;
+                x = scaled4<RS>(acc[EPI == EPI_SILU_MUL ? 2 * i : i][j], rs, col_scales4(col_scale, col, n));
+                if constexpr (EPI == EPI_SILU_MUL)
+                    u = scaled4<RS>(acc[2 * i + 1][j], rs, col_scales4(col_scale + n, col, n));
+            } else {
+                x = acc[EPI == EPI_SILU_MUL ? 2 * i : i][j];
+                if constexpr (RS) x *= rs;
+            }
             if constexpr (EPI == EPI_SILU_MUL) {
-                f32x4_t u = acc[2 * i + 1][j];
-                if constexpr (RS) u *= rs;
+                if constexpr (RS != RS_BOTH) u = acc[2 * i + 1][j];
+                if constexpr (RS == RS_ROW) u *= rs;
 #pragma unroll
                 for (int v = 0; v < 4; ++v) x[v] = silu_f32(x[v]) * u[v];
             }
@@ -242,7 +252,7 @@ int launch_tile(const Problem& p, hipStream_t s) {
     hipLaunchKernelGGL((mfma_narrow_kernel<DT, DT_OUT, BM, BN, KS, WGM, WGN, STAGES, EPI, RS, KN>),
                        dim3(static_cast<uint32_t>(tiles)), dim3(WGM * WGN * 64), 0, s,
                        static_cast<const uint16_t*>(p.a), static_cast<const uint16_t*>(p.b), p.m, p.n, p.k, p.lda, p.ldb,
-                       p.c, p.ldc, c_vec, p.row_scale);
+                       p.c, p.ldc, c_vec, p.row_scale, p.col_scale);
     return check_launch("mfma_narrow", BM, BNO);
 }
 
@@ -339,6 +349,12 @@ int launch_typed(const Problem& p, hipStream_t s) {
     return launch_plain<DT, DT_OUT, EPI_NONE, 0, 0>(p, s);
 }
 
+template <int DT_OUT>
+int launch_int8(const Problem& p, hipStream_t s) {
+    if (p.epi == EPI_SILU_MUL) return launch_silu<kI8, DT_OUT, RS_BOTH>(p, s);
+    return launch_plain<kI8, DT_OUT, EPI_NONE, RS_BOTH, 0>(p, s);
+}
+
 }  // namespace
 
 // K-tiles are counted in 32 bits.
@@ -350,6 +366,11 @@ bool mfma_narrow_pays(const Problem& p) {
 }
 
 int launch_mfma_narrow(const Problem& p, hipStream_t s) {
+    if (p.dtype_in == kI8) {
+        if (p.dtype_out == NANOVLLM_GEMM_F32) return launch_int8<NANOVLLM_GEMM_F32>(p, s);
+        return p.dtype_out == NANOVLLM_GEMM_F16 ? launch_int8<NANOVLLM_GEMM_F16>(p, s)
+                                                : launch_int8<NANOVLLM_GEMM_BF16>(p, s);
+    }
     if (p.dtype_in == NANOVLLM_GEMM_BF16) {
         if (p.dtype_out == NANOVLLM_GEMM_BF16) return launch_typed<NANOVLLM_GEMM_BF16, NANOVLLM_GEMM_BF16>(p, s);
         return launch_typed<NANOVLLM_GEMM_BF16, NANOVLLM_GEMM_F32>(p, s);

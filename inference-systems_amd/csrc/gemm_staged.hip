@@ -74,7 +74,7 @@ template <int DT, int DT_OUT, int BM, int BN, int WGM, int WGN, int STAGES, int 
 __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
     const uint16_t* __restrict__ a, const uint16_t* __restrict__ w, int64_t m, int64_t n, int64_t k, int64_t lda,
     int64_t ldb, void* __restrict__ c, int64_t ldc, int c_vec, uint64_t* __restrict__ keys,
-    const float* __restrict__ row_scale, SampleArgs sa) {
+    const float* __restrict__ row_scale, SampleArgs sa, const float* __restrict__ col_scale) {
     // The arguments the copies need first (a, w, m, n, k, lda, ldb: 56
     // bytes) lead the list, so with kernel-argument preloading (14 SGPRs)
     // the first K-tiles are requested before any argument load returns;
@@ -123,6 +123,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
     // every fragment wait into lgkmcnt(0).
     auto hold_epilogue_args = [&] {
         asm volatile("" :: "s"(c), "s"(ldc), "s"(c_vec), "s"(m), "s"(n), "s"(keys), "s"(row_scale));
+        if constexpr (RS == RS_BOTH) asm volatile("" :: "s"(col_scale));
     };
 
     const int tiles_m = static_cast<int>((m + BM - 1) / BM);
@@ -211,11 +212,11 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
         dma16(chunk_src(j, k0), dst);
     };
 
-    f32x16_t acc[NI][MJ];
+    acc16_t<DT> acc[NI][MJ];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) acc[i][j] = f32x16_t{};
+        for (int j = 0; j < MJ; ++j) acc[i][j] = acc16_t<DT>{};
 
     // Fragment rows: lane l reads row (base + l % 32) with base a multiple of
     // 32, so the swizzle key is ((l % 32) >> 1) & 7 = (l >> 1) & 7.
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_32x32x16<DT>(wf[i], af[j], acc[i][j]);
+            for (int j = 0; j < MJ; ++j) acc[i][j] = mma_32<DT>(wf[i], af[j], acc[i][j]);
     };
     // Wait until tile u has landed in every wave's part of its stage (each
     // wave waits on its own vmcnt, the barrier covers the others), then
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
             constexpr int J0 = decltype(j0_c)::value, CNT = decltype(cnt_c)::value;
 #pragma unroll
             for (int x = 0; x < STEP; ++x) {
-                acc[x / MJ][x % MJ] = mfma_32x32x16<DT>(wf[x / MJ], af[x % MJ], acc[x / MJ][x % MJ]);
+                acc[x / MJ][x % MJ] = mma_32<DT>(wf[x / MJ], af[x % MJ], acc[x / MJ][x % MJ]);
                 const int from = x * CNT / STEP, to = (x + 1) * CNT / STEP;
                 if (to > from) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -436,7 +437,21 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mfma_staged_kernel(
             for (int q = 0; q < 4; ++q) {
                 const int col = wn * (NIO * 32) + 32 * i + 8 * q + 4 * half;
                 float x0, x1, x2, x3;
-                if constexpr (EPI == EPI_SILU_MUL) {
+                if constexpr (DT == kI8) {
+                    constexpr int G = EPI == EPI_SILU_MUL ? 2 : 1;
+                    auto part = [&](int b, int64_t at) {
+                        const acc16_t<DT>& v = acc[b][j];
+                        return scaled4<RS>(acc4_t<DT>{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}, rs,
+                                           col_scales4(col_scale + at, n0 + col, n));
+                    };
+                    f32x4_t x = part(G * i, 0);
+                    if constexpr (EPI == EPI_SILU_MUL) {
+                        const f32x4_t u = part(2 * i + 1, n);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = silu_f32(x[e]) * u[e];
+                    }
+                    x0 = x[0]; x1 = x[1]; x2 = x[2]; x3 = x[3];
+                } else if constexpr (EPI == EPI_SILU_MUL) {
                     const f32x16_t& g = acc[2 * i][j];
                     const f32x16_t& u = acc[2 * i + 1][j];
                     if constexpr (RS) {
@@ -563,7 +578,7 @@ int launch_tile(const Problem& p, hipStream_t s) {
     if (EPI == EPI_ARGMAX) *p.key_blocks = tiles_n;
     hipLaunchKernelGGL((mfma_staged_kernel<DT, DT_OUT, BM, BN, WGM, WGN, STAGES, EPI, RS, SP, KN>), grid, block, 0, s,
                        static_cast<const uint16_t*>(p.a), static_cast<const uint16_t*>(p.b), p.m, p.n, p.k, p.lda,
-                       p.ldb, p.c, p.ldc, c_vec, p.keys, p.row_scale, p.sample);
+                       p.ldb, p.c, p.ldc, c_vec, p.keys, p.row_scale, p.sample, p.col_scale);
     return check_launch("mfma_staged", BM, BNO);
 }
 
@@ -650,12 +665,24 @@ int launch_typed(const Problem& p, hipStream_t s) {
     return launch_epi<DT, DT_OUT, EPI_NONE>(p, s);
 }
 
+// 8-bit integers: the bf16 choices of the same bytes.
+template <int DT_OUT>
+int launch_int8(const Problem& p, hipStream_t s) {
+    if (p.epi == EPI_SILU_MUL) return launch_epi<kI8, DT_OUT, EPI_SILU_MUL, RS_BOTH>(p, s);
+    return launch_epi<kI8, DT_OUT, EPI_NONE, RS_BOTH>(p, s);
+}
+
 }  // namespace
 
 int launch_mfma_staged(const Problem& p, hipStream_t s) {
     if (mfma_wide_pays(p)) return launch_mfma_wide(p, s);
     if (mfma_narrow_pays(p)) return launch_mfma_narrow(p, s);
     if (mfma_mid_pays(p)) return launch_mfma_mid(p, s);
+    if (p.dtype_in == kI8) {
+        if (p.dtype_out == NANOVLLM_GEMM_F32) return launch_int8<NANOVLLM_GEMM_F32>(p, s);
+        return p.dtype_out == NANOVLLM_GEMM_F16 ? launch_int8<NANOVLLM_GEMM_F16>(p, s)
+                                                : launch_int8<NANOVLLM_GEMM_BF16>(p, s);
+    }
     if (p.epi == EPI_ARGMAX) {
         constexpr int F = NANOVLLM_GEMM_F32;
         if (p.dtype_in == NANOVLLM_GEMM_BF16) return launch_epi<NANOVLLM_GEMM_BF16, F, EPI_ARGMAX>(p, s);

@@ -53,7 +53,8 @@ __device__ __forceinline__ void dma16_at(const void* base, uint32_t off, uint32_
 template <int DT, int DT_OUT, int EPI, int RS>
 __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
     const uint16_t* __restrict__ a, const uint16_t* __restrict__ w, int64_t m, int64_t n, int64_t k, int64_t lda,
-    int64_t ldb, void* __restrict__ c, int64_t ldc, int c_vec, const float* __restrict__ row_scale) {
+    int64_t ldb, void* __restrict__ c, int64_t ldc, int c_vec, const float* __restrict__ row_scale,
+    const float* __restrict__ col_scale) {
     constexpr int BNO = EPI == EPI_SILU_MUL ? kBN / 2 : kBN;   // output columns per tile
     constexpr int OB = DT_OUT == NANOVLLM_GEMM_F32 ? 4 : 2;
     constexpr int PITCH = BNO * OB + 16;
@@ -90,6 +91,12 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
     };
     const uint16_t* abase = a + m0 * lda;
     const uint16_t* wbase = w + n0 * ldb;
+    if constexpr (DT == kI8) {
+        // The column scales' addresses have n0 in vector registers; the copies
+        // need their bases in scalar ones.
+        abase = scalar_pointer(abase);
+        wbase = scalar_pointer(wbase);
+    }
     uint32_t off[kCopies];
 #pragma unroll
     for (int j = 0; j < kCopies; ++j) {
@@ -126,11 +133,11 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
         }
     };
 
-    f32x4_t acc[kNI][kMI];
+    acc4_t<DT> acc[kNI][kMI];
 #pragma unroll
     for (int i = 0; i < kNI; ++i)
 #pragma unroll
-        for (int j = 0; j < kMI; ++j) acc[i][j] = f32x4_t{};
+        for (int j = 0; j < kMI; ++j) acc[i][j] = acc4_t<DT>{};
 
     // Fragment of a 16-row block: lane l reads row l % 16, chunk 4 s + l / 16
     // of K-step s.
@@ -160,6 +167,7 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
         wait_vmcnt<0>();
     }
     asm volatile("" :: "s"(c), "s"(ldc), "s"(c_vec), "s"(m), "s"(n), "s"(row_scale));
+    if constexpr (RS == RS_BOTH) asm volatile("" :: "s"(col_scale));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     barrier();
 #pragma unroll
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < kNI; ++j) acc[j][i] = mfma_16x16x32<DT>(wf0[j], af[i], acc[j][i]);
+            for (int j = 0; j < kNI; ++j) acc[j][i] = mma_16<DT>(wf0[j], af[i], acc[j][i]);
             if (i < kNI) wf1[i] = read_w(st, 1, i);
             af[i] = read_a(st, 1, i);
             if constexpr (NEXT) {
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
         for (int i = 0; i < kMI; ++i) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < kNI; ++j) acc[j][i] = mfma_16x16x32<DT>(wf1[j], af[i], acc[j][i]);
+            for (int j = 0; j < kNI; ++j) acc[j][i] = mma_16<DT>(wf1[j], af[i], acc[j][i]);
             if constexpr (NEXT) {
                 if (i == 4) {
                     // Region Q of K-tile t + 1 has landed, and every wave has
@@ -252,6 +260,15 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
     // kept through the K loop, which has no register left for them.
     const float* scale = RS ? row_scale + m0 : nullptr;
     const int last_row = static_cast<int>(min_i64(kBM, m - m0)) - 1;
+    f32x4_t cg[NJ], cu[NJ];   // column scales
+    if constexpr (RS == RS_BOTH) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int64_t col = n0 + wn * 16 * NJ + 16 * j + 4 * quad;
+            cg[j] = col_scales4(col_scale, col, n);
+            if constexpr (EPI == EPI_SILU_MUL) cu[j] = col_scales4(col_scale + n, col, n);
+        }
+    }
 #pragma unroll 1
     for (int ep = 0; ep < EPASS; ++ep) {
         __syncthreads();
@@ -264,11 +281,9 @@ __global__ __launch_bounds__(kThreads) void mfma_wide_kernel(
                 char* rowp = ctile + (row - ep * EP_ROWS) * PITCH;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    f32x4_t x = acc[j][i];
-                    if constexpr (RS) x *= rs;
+                    f32x4_t x = scaled4<RS>(acc[j][i], rs, cg[j]);
                     if constexpr (EPI == EPI_SILU_MUL) {
-                        f32x4_t u = acc[j + NJ][i];
-                        if constexpr (RS) u *= rs;
+                        const f32x4_t u = scaled4<RS>(acc[j + NJ][i], rs, cu[j]);
 #pragma unroll
                         for (int v = 0; v < 4; ++v) x[v] = silu_f32(x[v]) * u[v];
                     }
@@ -326,7 +341,7 @@ int launch_tile(const Problem& p, hipStream_t s) {
     const int c_vec = (reinterpret_cast<uintptr_t>(p.c) % 16 == 0) && ((p.ldc * out_bytes) % 16 == 0);
     hipLaunchKernelGGL((mfma_wide_kernel<DT, DT_OUT, EPI, RS>), dim3(static_cast<uint32_t>(tiles)), dim3(kThreads), 0, s,
                        static_cast<const uint16_t*>(p.a), static_cast<const uint16_t*>(p.b), p.m, p.n, p.k, p.lda,
-                       p.ldb, p.c, p.ldc, c_vec, p.row_scale);
+                       p.ldb, p.c, p.ldc, c_vec, p.row_scale, p.col_scale);
     return check_launch("mfma_wide", kBM, BNO);
 }
 
@@ -338,6 +353,12 @@ int launch_typed(const Problem& p, hipStream_t s) {
     }
     if (p.epi == EPI_SILU_MUL) return launch_tile<DT, DT_OUT, EPI_SILU_MUL, 0>(p, s);
     return launch_tile<DT, DT_OUT, EPI_NONE, 0>(p, s);
+}
+
+template <int DT_OUT>
+int launch_int8(const Problem& p, hipStream_t s) {
+    if (p.epi == EPI_SILU_MUL) return launch_tile<kI8, DT_OUT, EPI_SILU_MUL, RS_BOTH>(p, s);
+    return launch_tile<kI8, DT_OUT, EPI_NONE, RS_BOTH>(p, s);
 }
 
 }  // namespace
@@ -387,6 +408,11 @@ bool mfma_wide_pays(const Problem& p) {
 }
 
 int launch_mfma_wide(const Problem& p, hipStream_t s) {
+    if (p.dtype_in == kI8) {
+        if (p.dtype_out == NANOVLLM_GEMM_F32) return launch_int8<NANOVLLM_GEMM_F32>(p, s);
+        return p.dtype_out == NANOVLLM_GEMM_F16 ? launch_int8<NANOVLLM_GEMM_F16>(p, s)
+                                                : launch_int8<NANOVLLM_GEMM_BF16>(p, s);
+    }
     if (p.dtype_in == NANOVLLM_GEMM_BF16) {
         if (p.dtype_out == NANOVLLM_GEMM_BF16) return launch_typed<NANOVLLM_GEMM_BF16, NANOVLLM_GEMM_BF16>(p, s);
         return launch_typed<NANOVLLM_GEMM_BF16, NANOVLLM_GEMM_F32>(p, s);

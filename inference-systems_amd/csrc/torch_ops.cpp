@@ -1,6 +1,8 @@
 // torch_ops.cpp — nanovllm::gemm, gemm_kn, the fused ops (gemm_silu_mul,
-// gemm_argmax, gemm_sample, gemm_gated, gemm_add_rmsnorm) and the attention ops
-// (rope_append, kv_gather, attention_prompt, attention_paged) registered from C++.
+// gemm_argmax, gemm_sample, gemm_gated, gemm_add_rmsnorm), the attention ops
+// (rope_append, kv_gather, attention_prompt, attention_paged), the 8-bit ops
+// (quantize_rows, add_rmsnorm_quantize, gemm_int8, gemm_int8_silu_mul) and
+// sample_logits registered from C++.
 //
 // The registration pattern of nanovllm/csrc/ops.cpp:48-80 (TORCH_LIBRARY
 // block, one CUDA-key implementation per op) over the C ABI of
@@ -10,7 +12,7 @@
 // reference's add op (nanovllm/csrc/add_kernel.cu:49-67).
 //
 // The argument contract and its messages are those of the Python
-// registration (kernels/gemm.py, kernels/prologue.py, kernels/attention.py), so callers see the same
+// registration (kernels/gemm.py, prologue.py, attention.py, int8.py, sampling.py), so callers see the same
 // RuntimeError text from either registration; the schemas are identical.
 // The fake (meta) implementations stay in Python (torch.library.register_fake).
 //
@@ -35,6 +37,8 @@
 
 #include "nanovllm_attention.h"
 #include "nanovllm_gemm.h"
+#include "nanovllm_int8.h"
+#include "nanovllm_sampling.h"
 
 namespace {
 
@@ -664,6 +668,207 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache, const
     return out;
 }
 
+// ---------------------------------------------------------------------------
+// The 8-bit ops and the sampler: kernels/int8.py's and kernels/sampling.py's
+// contracts, in their order and wording, and their launches.
+// ---------------------------------------------------------------------------
+bool float_type(const at::Tensor& t) { return dtype_code(t.scalar_type()) >= 0; }
+
+constexpr int64_t kMaxRows = int64_t(1) << 23, kMaxK = 131071;
+constexpr int64_t kMaxVocab = int64_t(1) << 23, kMaxSampleRows = int64_t(1) << 20;
+
+// Elements between rows of a contiguous tensor or a 2-D view.
+int64_t row_stride(const at::Tensor& x) {
+    return x.dim() == 2 && x.size(0) > 1 && !x.is_contiguous() ? x.stride(0) : x.size(-1);
+}
+
+std::string view_reason(const char* name, const at::Tensor& x) {
+    const std::string n = name;
+    if (x.dim() < 1) return n + " must have at least one dimension";
+    if (x.size(-1) == 0) return "K must be positive";
+    if (!x.is_contiguous()) {
+        if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1))
+            return n + " must be contiguous, or 2-D with unit stride in its last dimension";
+        if (x.size(0) > 1 && x.stride(0) < x.size(1)) return "the rows of " + n + " must not overlap";
+    }
+    if (x.numel() / x.size(-1) > kMaxRows) return n + " must have at most 2^23 rows";
+    return {};
+}
+
+std::string quantize_rows_reason(const at::Tensor& x) {
+    if (!x.is_cuda()) return "x must be a CUDA (HIP) tensor";
+    if (!float_type(x)) return "x must be float32, float16 or bfloat16";
+    return view_reason("x", x);
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
+    const std::string reason = quantize_rows_reason(x);
+    TORCH_CHECK(reason.empty(), "nanovllm::quantize_rows: ", reason);
+    at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    at::Tensor scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    if (x.numel() == 0) return {codes, scales};
+    const c10::DeviceGuard guard(x.device());
+    const int64_t k = x.size(-1);
+    check_rc(nanovllm_quantize_rows(x.data_ptr(), static_cast<int8_t*>(codes.data_ptr()),
+                                    static_cast<float*>(scales.data_ptr()), x.numel() / k, k, row_stride(x),
+                                    dtype_code(x.scalar_type()), stream_of(x)),
+             "nanovllm_quantize_rows");
+    return {codes, scales};
+}
+
+std::string add_rmsnorm_quantize_reason(const at::Tensor& h, const at::Tensor& residual, const at::Tensor& norm_weight,
+                                        double eps) {
+    if (!(h.is_cuda() && residual.is_cuda() && norm_weight.is_cuda()))
+        return "h, residual and norm_weight must be CUDA (HIP) tensors";
+    if (!(h.device() == residual.device() && h.device() == norm_weight.device()))
+        return "h, residual and norm_weight must be on the same device";
+    if (!half_type(h)) return "h must be float16 or bfloat16";
+    if (residual.scalar_type() != h.scalar_type() || norm_weight.scalar_type() != h.scalar_type())
+        return "h, residual and norm_weight must have the same dtype";
+    if (h.dim() != 2 || residual.sizes() != h.sizes()) return "h and residual must be (M, K) tensors of the same shape";
+    std::string r = view_reason("h", h);
+    if (r.empty()) r = view_reason("residual", residual);
+    if (!r.empty()) return r;
+    if (norm_weight.dim() != 1 || norm_weight.size(0) != h.size(1) || !norm_weight.is_contiguous())
+        return "norm_weight must be a contiguous (K,) tensor (K = " + std::to_string(h.size(1)) + ")";
+    if (!(eps >= 0.0 && eps < 3.0e38)) return "eps must be finite and not negative";
+    return {};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_quantize(const at::Tensor& h, const at::Tensor& residual,
+                                                                    const at::Tensor& norm_weight, double eps) {
+    const std::string reason = add_rmsnorm_quantize_reason(h, residual, norm_weight, eps);
+    TORCH_CHECK(reason.empty(), "nanovllm::add_rmsnorm_quantize: ", reason);
+    const int64_t m = h.size(0), k = h.size(1);
+    at::Tensor codes = at::empty({m, k}, h.options().dtype(at::kChar));
+    at::Tensor scales = at::empty({m}, h.options().dtype(at::kFloat));
+    at::Tensor res = at::empty({m, k}, h.options());
+    if (m == 0) return {codes, scales, res};
+    const c10::DeviceGuard guard(h.device());
+    check_rc(nanovllm_add_rmsnorm_quantize(h.data_ptr(), residual.data_ptr(), norm_weight.data_ptr(),
+                                           static_cast<float>(eps), static_cast<int8_t*>(codes.data_ptr()),
+                                           static_cast<float*>(scales.data_ptr()), res.data_ptr(), m, k, row_stride(h),
+                                           row_stride(residual), dtype_code(h.scalar_type()), stream_of(h)),
+             "nanovllm_add_rmsnorm_quantize");
+    return {codes, scales, res};
+}
+
+std::string gemm_int8_reason(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w,
+                             const at::Tensor& w_scales, std::optional<at::ScalarType> out_dtype, bool silu_mul) {
+    if (!(a.is_cuda() && a_scales.is_cuda() && w.is_cuda() && w_scales.is_cuda()))
+        return "a, w and their scales must be CUDA (HIP) tensors";
+    if (!(a.device() == a_scales.device() && a.device() == w.device() && a.device() == w_scales.device()))
+        return "a, w and their scales must be on the same device";
+    if (a.scalar_type() != at::kChar || w.scalar_type() != at::kChar) return "a and w must be int8";
+    if (a_scales.scalar_type() != at::kFloat || w_scales.scalar_type() != at::kFloat)
+        return "a_scales and w_scales must be float32";
+    if (out_dtype.has_value() && dtype_code(*out_dtype) < 0)
+        return "out_dtype " + dtype_name(*out_dtype) + " is not supported: float32, float16 or bfloat16";
+    if (w.dim() != 2) return "w must be 2-D";
+    if (a.dim() < 1 || a.size(-1) != w.size(1))
+        return "a must have rows of w.size(1) (" + std::to_string(w.size(1)) + ") codes, got shape " + tuple_text(a.sizes());
+    const int64_t k = w.size(1);
+    if (k < 1 || k > kMaxK) return "K (" + std::to_string(k) + ") must be from 1 to " + std::to_string(kMaxK);
+    if (silu_mul && w.size(0) % 2)
+        return "w must hold gate and up halves of equal height (got " + std::to_string(w.size(0)) + " rows)";
+    if (!a.is_contiguous() || !w.is_contiguous()) return "a and w must be contiguous";
+    const at::IntArrayRef rows = a.sizes().slice(0, a.dim() - 1), cols = w.sizes().slice(0, 1);
+    if (a_scales.sizes() != rows || !a_scales.is_contiguous())
+        return "a_scales must be a contiguous " + tuple_text(rows) + " tensor, got shape " + tuple_text(a_scales.sizes());
+    if (w_scales.sizes() != cols || !w_scales.is_contiguous())
+        return "w_scales must be a contiguous " + tuple_text(cols) + " tensor, got shape " + tuple_text(w_scales.sizes());
+    return {};
+}
+
+at::Tensor launch_gemm_int8(const char* op, const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w,
+                            const at::Tensor& w_scales, std::optional<at::ScalarType> out_dtype, bool silu_mul) {
+    const std::string reason = gemm_int8_reason(a, a_scales, w, w_scales, out_dtype, silu_mul);
+    TORCH_CHECK(reason.empty(), "nanovllm::", op, ": ", reason);
+    const at::ScalarType od = out_dtype.value_or(at::kBFloat16);
+    const int64_t k = w.size(1), n = silu_mul ? w.size(0) / 2 : w.size(0), m = a.numel() / k;
+    std::vector<int64_t> sizes = a.sizes().vec();
+    sizes.back() = n;
+    at::Tensor out = at::empty(sizes, a.options().dtype(od));
+    if (m == 0 || n == 0) return out;
+    const c10::DeviceGuard guard(a.device());
+    check_rc(nanovllm_gemm_int8(static_cast<const int8_t*>(a.data_ptr()), static_cast<const float*>(a_scales.data_ptr()),
+                                static_cast<const int8_t*>(w.data_ptr()), static_cast<const float*>(w_scales.data_ptr()),
+                                out.data_ptr(), m, n, k, k, k, n, silu_mul, dtype_code(od), stream_of(a)),
+             "nanovllm_gemm_int8");
+    return out;
+}
+
+at::Tensor gemm_int8(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w, const at::Tensor& w_scales,
+                     std::optional<at::ScalarType> out_dtype) {
+    return launch_gemm_int8("gemm_int8", a, a_scales, w, w_scales, out_dtype, false);
+}
+
+at::Tensor gemm_int8_silu_mul(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w,
+                              const at::Tensor& w_scales, std::optional<at::ScalarType> out_dtype) {
+    return launch_gemm_int8("gemm_int8_silu_mul", a, a_scales, w, w_scales, out_dtype, true);
+}
+
+struct RowParameter {
+    const char* name;
+    const at::Tensor* t;
+    at::ScalarType dtype;
+};
+
+std::string sample_logits_reason(const at::Tensor& logits, const std::vector<RowParameter>& given) {
+    for (const RowParameter& g : given)
+        if (!logits.is_cuda() || !g.t->is_cuda()) return "logits and the rows' parameters must be CUDA (HIP) tensors";
+    for (const RowParameter& g : given)
+        if (g.t->device() != logits.device()) return "logits and the rows' parameters must be on the same device";
+    if (!float_type(logits)) return "logits must be float32, float16 or bfloat16";
+    if (logits.dim() < 1 || logits.size(-1) < 1 || logits.size(-1) > kMaxVocab)
+        return "logits must have rows of 1 to " + std::to_string(kMaxVocab) + " entries, got shape " +
+               tuple_text(logits.sizes());
+    const std::string r = view_reason("logits", logits);
+    if (!r.empty()) return r;
+    if (logits.numel() / logits.size(-1) > kMaxSampleRows) return "logits must have at most 2^20 rows";
+    const at::IntArrayRef rows = logits.sizes().slice(0, logits.dim() - 1);
+    for (const RowParameter& g : given) {
+        const std::string n = g.name;
+        if (g.t->scalar_type() != g.dtype) return n + " must be " + dtype_name(g.dtype);
+        if (g.t->sizes() != rows || !g.t->is_contiguous())
+            return n + " must be a contiguous " + tuple_text(rows) + " tensor, got shape " + tuple_text(g.t->sizes());
+    }
+    return {};
+}
+
+std::tuple<at::Tensor, at::Tensor> sample_logits(const at::Tensor& logits, const at::Tensor& temperatures,
+                                                 const at::Tensor& uniforms, const std::optional<at::Tensor>& top_k,
+                                                 const std::optional<at::Tensor>& top_p,
+                                                 const std::optional<at::Tensor>& min_p) {
+    std::vector<RowParameter> given = {{"temperatures", &temperatures, at::kFloat}, {"uniforms", &uniforms, at::kFloat}};
+    if (top_k.has_value()) given.push_back({"top_k", &*top_k, at::kInt});
+    if (top_p.has_value()) given.push_back({"top_p", &*top_p, at::kFloat});
+    if (min_p.has_value()) given.push_back({"min_p", &*min_p, at::kFloat});
+    const std::string reason = sample_logits_reason(logits, given);
+    TORCH_CHECK(reason.empty(), "nanovllm::sample_logits: ", reason);
+    const int64_t vocab = logits.size(-1), m = logits.numel() / vocab;
+    const at::IntArrayRef rows = logits.sizes().slice(0, logits.dim() - 1);
+    at::Tensor tokens = at::empty(rows, logits.options().dtype(at::kLong));
+    at::Tensor logprobs = at::empty(rows, logits.options().dtype(at::kFloat));
+    if (m == 0) return {tokens, logprobs};
+    const int code = dtype_code(logits.scalar_type());
+    const int64_t need = nanovllm_sample_logits_workspace_bytes(m, vocab, code);
+    check_rc(need, "nanovllm_sample_logits_workspace_bytes");
+    const at::Tensor ws = bytes_like(logits, need > 0 ? need : 1);
+    const c10::DeviceGuard guard(logits.device());
+    auto floats = [](const std::optional<at::Tensor>& t) {
+        return t.has_value() ? static_cast<const float*>(t->data_ptr()) : nullptr;
+    };
+    check_rc(nanovllm_sample_logits(logits.data_ptr(), static_cast<const float*>(temperatures.data_ptr()),
+                                    static_cast<const float*>(uniforms.data_ptr()),
+                                    top_k.has_value() ? static_cast<const int32_t*>(top_k->data_ptr()) : nullptr,
+                                    floats(top_p), floats(min_p), static_cast<int64_t*>(tokens.data_ptr()),
+                                    static_cast<float*>(logprobs.data_ptr()), m, vocab, row_stride(logits), code,
+                                    ws.data_ptr(), need, stream_of(logits)),
+             "nanovllm_sample_logits");
+    return {tokens, logprobs};
+}
+
 at::Tensor gemm(const at::Tensor& a, const at::Tensor& w, std::optional<at::ScalarType> out_dtype) {
     return launch(a, w, out_dtype, NANOVLLM_GEMM_B_NK);
 }
@@ -695,6 +900,13 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
           "bool causal=True) -> Tensor");
     m.def("attention_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, "
           "float scale, Tensor? k_scales=None, Tensor? v_scales=None) -> Tensor");
+    m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
+    m.def("add_rmsnorm_quantize(Tensor h, Tensor residual, Tensor norm_weight, float eps) -> (Tensor, Tensor, Tensor)");
+    m.def("gemm_int8(Tensor a, Tensor a_scales, Tensor w, Tensor w_scales, ScalarType? out_dtype=None) -> Tensor");
+    m.def("gemm_int8_silu_mul(Tensor a, Tensor a_scales, Tensor w, Tensor w_scales, ScalarType? out_dtype=None) -> "
+          "Tensor");
+    m.def("sample_logits(Tensor logits, Tensor temperatures, Tensor uniforms, Tensor? top_k=None, Tensor? top_p=None, "
+          "Tensor? min_p=None) -> (Tensor, Tensor)");
 }
 
 namespace {
@@ -711,6 +923,11 @@ void implement(torch::Library& m) {
     m.impl("kv_gather", &kv_gather);
     m.impl("attention_prompt", &attention_prompt);
     m.impl("attention_paged", &attention_paged);
+    m.impl("quantize_rows", &quantize_rows);
+    m.impl("add_rmsnorm_quantize", &add_rmsnorm_quantize);
+    m.impl("gemm_int8", &gemm_int8);
+    m.impl("gemm_int8_silu_mul", &gemm_int8_silu_mul);
+    m.impl("sample_logits", &sample_logits);
 }
 
 }  // namespace
@@ -721,10 +938,11 @@ TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) { implement(m); }
 
 TORCH_LIBRARY_IMPL(nanovllm, CPU, m) { implement(m); }
 
-// The fused ops and the attention ops have no backward: asking for one raises, as it does for a
-// custom_op without an autograd formula.
+// The fused ops, the attention ops, the 8-bit ops and the sampler have no backward: asking for one
+// raises, as it does for a custom_op without an autograd formula.
 TORCH_LIBRARY_IMPL(nanovllm, Autograd, m) {
     for (const char* op : {"gemm_silu_mul", "gemm_argmax", "gemm_sample", "gemm_gated", "gemm_add_rmsnorm", "rope_append",
-                           "kv_gather", "attention_prompt", "attention_paged"})
+                           "kv_gather", "attention_prompt", "attention_paged", "quantize_rows",
+                           "add_rmsnorm_quantize", "gemm_int8", "gemm_int8_silu_mul", "sample_logits"})
         m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

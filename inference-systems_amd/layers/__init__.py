@@ -5,12 +5,14 @@ from .gdn_projection import GdnInputProjection
 from .linear import (
     ColumnParallelLinear,
     GemmLinear,
+    Int8Weight,
     LinearBase,
     MergedColumnParallelLinear,
     ParallelLMHead,
     QKVParallelLinear,
     ReplicatedLinear,
     RowParallelLinear,
+    quantize_int8,
 )
 from .mlp import Qwen35MLP
 from .norm import Qwen35RMSNorm
@@ -19,6 +21,7 @@ __all__ = [
     "ColumnParallelLinear",
     "GdnInputProjection",
     "GemmLinear",
+    "Int8Weight",
     "LinearBase",
     "MergedColumnParallelLinear",
     "ParallelLMHead",
@@ -28,4 +31,5 @@ __all__ = [
     "Qwen35RMSNorm",
     "ReplicatedLinear",
     "RowParallelLinear",
+    "quantize_int8",
 ]

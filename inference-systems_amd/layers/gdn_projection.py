@@ -24,7 +24,8 @@ contiguous outputs there by running the four GEMMs on the weight's row
 ranges (what the reference does), not one GEMM and four copies: measured on
 MI355X at M = 32 (N = 8224, K = 1024, bf16, W from HBM), one GEMM with
 views 8.6 us, the four GEMMs 17.7 us, one GEMM plus four .contiguous()
-copies 20.0 us.
+copies 20.0 us.  With the weight in 8 bits (``quantize_int8``) it is one GEMM
+either way.
 """
 from __future__ import annotations
 
@@ -33,14 +34,14 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ..kernels import add_rmsnorm_linear
+from ..kernels import add_rmsnorm_linear, int8_add_rmsnorm_linear, int8_linear
 from ..kernels import linear as gemm_linear
-from .linear import _tp_rank_size, divide
+from .linear import Int8Weight, _tp_rank_size, divide
 
 SHARDS = ("qkv", "z", "b", "a")
 
 
-class GdnInputProjection(nn.Module):
+class GdnInputProjection(Int8Weight):
 
     def __init__(self, hidden_size: int, num_key_heads: int, num_value_heads: int, key_head_dim: int,
                  value_head_dim: int):
@@ -88,6 +89,10 @@ class GdnInputProjection(nn.Module):
 
     def forward(self, x: torch.Tensor,
                 contiguous: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        if self.is_int8:
+            y = int8_linear(x, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
+            parts = y.split(self.output_sizes, dim=-1)
+            return tuple(part.contiguous() for part in parts) if contiguous else parts
         if contiguous and x.numel() // x.shape[-1] > 1:
             return tuple(gemm_linear(x, self.weight.narrow(0, self.shard_offsets[sid], self.shard_sizes[sid]), None,
                                      backend=self.gemm_backend) for sid in SHARDS)
@@ -99,6 +104,10 @@ class GdnInputProjection(nn.Module):
         a linear-attention decoder layer and the merged projection
         (nanovllm/models/qwen3_5.py:157-163).  On the HIP path the residual
         add and the norm run inside the GEMM."""
-        y, new_residual = add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, self.weight,
-                                             backend=self.gemm_backend)
+        if self.is_int8:
+            y, new_residual = int8_add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, self.weight_codes,
+                                                      self.weight_scales, backend=self.gemm_backend)
+        else:
+            y, new_residual = add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, self.weight,
+                                                 backend=self.gemm_backend)
         return y.split(self.output_sizes, dim=-1), new_residual

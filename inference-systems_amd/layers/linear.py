@@ -11,6 +11,10 @@ Routing is opt-in per process with ``NANOVLLM_GEMM_BACKEND`` = ``torch``
 of nanovllm/layers/layernorm.py:17-20 -- or per module with the
 ``gemm_backend`` attribute.  The tensor-parallel collectives are unchanged
 (one GPU here: tp_size is 1 unless a process group says otherwise).
+
+``quantize_int8()`` on a loaded layer keeps its weight in 8 bits, a scale for
+each output channel; from then on its rows go through ``quantize_rows`` and
+``gemm_int8``.  Move or convert a module first: the scales stay float32.
 """
 from __future__ import annotations
 
@@ -20,7 +24,8 @@ import torch
 import torch.distributed as dist
 from torch import nn
 
-from ..kernels import gated_linear, gemm_sample, greedy_linear, sample_contract_reason, sample_linear, torch_sampler
+from ..kernels import gated_linear, gemm_sample, greedy_linear, int8_linear, quantize_rows, sample_contract_reason
+from ..kernels import gated_contract_reason, sample_linear, sample_rows, sigmoid_gate, torch_quantize_rows, torch_sampler
 from ..kernels import linear as gemm_linear
 from ..kernels import validate_gemm_backend
 from ..kernels.gemm import default_backend
@@ -41,7 +46,41 @@ def _tp_rank_size() -> tuple[int, int]:
     return 0, 1
 
 
-class LinearBase(nn.Module):
+class Int8Weight(nn.Module):
+    """A module whose ``weight`` [N, K] can be kept in 8 bits: ``weight_codes`` (int8) and ``weight_scales`` (float32,
+    a scale for each row) in its place, both in the state dict."""
+
+    weight_codes: Optional[torch.Tensor]
+    weight_scales: Optional[torch.Tensor]
+
+    def __init__(self):
+        super().__init__()
+        self.register_buffer("weight_codes", None)
+        self.register_buffer("weight_scales", None)
+
+    @property
+    def is_int8(self) -> bool:
+        return self.weight_codes is not None
+
+    @torch.no_grad()
+    def quantize_int8(self) -> None:
+        """Replaces the weight by its codes and scales; again: nothing."""
+        if self.is_int8:
+            return
+        weight = self.weight.detach()
+        self.weight_codes, self.weight_scales = quantize_rows(weight) if weight.is_cuda else torch_quantize_rows(weight)
+        self.weight = None
+
+
+def quantize_int8(module: nn.Module) -> nn.Module:
+    """Every layer of ``module`` that can keep its weight in 8 bits does so from here on."""
+    for layer in module.modules():
+        if isinstance(layer, Int8Weight):
+            layer.quantize_int8()
+    return module
+
+
+class LinearBase(Int8Weight):
 
     def __init__(self, input_size: int, output_size: int, bias: bool = False, tp_dim: Optional[int] = None):
         super().__init__()
@@ -57,6 +96,9 @@ class LinearBase(nn.Module):
         self.gemm_backend: Optional[str] = None   # None: NANOVLLM_GEMM_BACKEND
 
     def matmul(self, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+        if self.is_int8:
+            y = int8_linear(x, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
+            return y if bias is None else y + bias.to(y.dtype)
         return gemm_linear(x, self.weight, bias, backend=self.gemm_backend)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -160,7 +202,16 @@ class RowParallelLinear(LinearBase):
         this rank's heads [M, heads, head_dim] (or [M, K]) and ``gate`` the
         matching view of q_proj's output; on the HIP path the gate is applied
         in front of the GEMM."""
-        y = gated_linear(x, gate, self.weight, backend=self.gemm_backend)
+        if self.is_int8:
+            backend = validate_gemm_backend(self.gemm_backend) if self.gemm_backend is not None else default_backend()
+            one = x.new_empty((1, x[0].numel())) if backend == "auto" else None
+            if backend == "hip" or (backend == "auto" and gated_contract_reason(x, gate, one) is None):
+                gated = sigmoid_gate(x, gate)
+            else:
+                gated = (x.reshape(gate.shape) * torch.sigmoid(gate)).reshape(x.shape[0], -1)
+            y = int8_linear(gated, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
+        else:
+            y = gated_linear(x, gate, self.weight, backend=self.gemm_backend)
         if self.bias is not None and self.tp_rank == 0:
             y = y + self.bias.to(y.dtype)
         if self.tp_size > 1:
@@ -168,7 +219,7 @@ class RowParallelLinear(LinearBase):
         return y
 
 
-class ParallelLMHead(nn.Module):
+class ParallelLMHead(Int8Weight):
     """Tied / vocab-parallel LM head (embed_head.py:45-66).
 
     The reference selects the last token of each sequence from the forward
@@ -179,7 +230,9 @@ class ParallelLMHead(nn.Module):
     (embed_head.py:61), and the greedy and sampled heads rank those rounded
     values (Sampler takes ``logits.float()``, sampler.py:15), so the tokens
     are the reference's.  ``logits_dtype = torch.float32`` opts into fp32
-    logits written by the GEMM directly and fp32 ranking."""
+    logits written by the GEMM directly and fp32 ranking.  A head in 8 bits
+    (``quantize_int8``) gives logits and draws from them (``draw``); the fused
+    greedy and sampled heads take its 16-bit weight."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, bias: bool = False):
         super().__init__()
@@ -203,12 +256,33 @@ class ParallelLMHead(nn.Module):
     def forward(self, x: torch.Tensor, last_indices: Optional[torch.Tensor] = None):
         if last_indices is not None:
             x = x[last_indices].contiguous()
-        logits = gemm_linear(x, self.weight, None, out_dtype=self.logits_dtype, backend=self.gemm_backend)
+        if self.is_int8:
+            logits = int8_linear(x, self.weight_codes, self.weight_scales, out_dtype=self.logits_dtype,
+                                 backend=self.gemm_backend)
+        else:
+            logits = gemm_linear(x, self.weight, None, out_dtype=self.logits_dtype, backend=self.gemm_backend)
         if self.tp_size > 1:
             all_logits = [torch.empty_like(logits) for _ in range(self.tp_size)] if self.tp_rank == 0 else None
             dist.gather(logits, all_logits, 0)
             logits = torch.cat(all_logits, -1) if self.tp_rank == 0 else None
         return logits
+
+    def draw(self, x: torch.Tensor, temperatures: torch.Tensor, uniforms: torch.Tensor,
+             top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+             min_p: Optional[torch.Tensor] = None, last_indices: Optional[torch.Tensor] = None):
+        """Tokens of this head's logits by temperature, top-k, top-p and min-p
+        from given random numbers (``sample_logits``), and the logarithms of
+        their shares among the kept tokens.  The logits are written; rows that
+        only have a temperature need none (``sample``).  With tensor parallelism
+        rank 0 draws from the gathered logits; other ranks return (None, None)."""
+        logits = self.forward(x, last_indices)
+        if logits is None:
+            return None, None
+        return sample_rows(logits, temperatures, uniforms, top_k, top_p, min_p, backend=self.gemm_backend)
+
+    def _refuse_int8(self, name: str) -> None:
+        if self.is_int8:
+            raise RuntimeError(f"ParallelLMHead.{name} takes a 16-bit weight; a head in 8 bits draws with draw()")
 
     def greedy(self, x: torch.Tensor, last_indices: Optional[torch.Tensor] = None):
         """Greedy tokens without the logits: the temperature-0 branch of
@@ -220,6 +294,7 @@ class ParallelLMHead(nn.Module):
         tensor parallelism every rank finds the best token of its vocabulary
         shard and rank 0 keeps the best pair, the lower rank on equal logits
         (the first index of the gathered logits); other ranks return None."""
+        self._refuse_int8("greedy")
         if last_indices is not None:
             x = x[last_indices].contiguous()
         tokens, values = greedy_linear(x, self.weight, backend=self.gemm_backend, logits_dtype=self.logits_dtype)
@@ -252,6 +327,7 @@ class ParallelLMHead(nn.Module):
         mixed with the rank, so shards draw independent noise), and rank 0
         keeps the best score, the lower rank on ties; other ranks return
         (None, None)."""
+        self._refuse_int8("sample")
         if last_indices is not None:
             x = x[last_indices].contiguous()
         if self.tp_size == 1:

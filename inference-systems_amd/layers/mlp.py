@@ -8,7 +8,8 @@ MergedColumnParallelLinear over [intermediate, intermediate] rows,
 [T, 2 * intermediate] projection; on the HIP path ``gate_up_proj`` and
 SiluAndMul (nanovllm/layers/activation.py:8-11) are one launch of
 ``nanovllm::gemm_silu_mul``.  Each rank's gate_up weight is [gate rows of
-the rank; up rows of the rank], exactly the layout the fused op takes.
+the rank; up rows of the rank], exactly the layout the fused op takes.  With
+weights in 8 bits (``quantize_int8``) both projections run on the 8-bit ops.
 """
 from __future__ import annotations
 
@@ -17,7 +18,7 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ..kernels import add_rmsnorm_linear, silu_mul_linear
+from ..kernels import add_rmsnorm_linear, int8_add_rmsnorm_linear, int8_silu_mul_linear, silu_mul_linear
 from .linear import MergedColumnParallelLinear, RowParallelLinear
 from .norm import Qwen35RMSNorm
 
@@ -45,7 +46,11 @@ class Qwen35MLP(nn.Module):
         self.down_proj.gemm_backend = value
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        h = silu_mul_linear(x, self.gate_up_proj.weight, backend=self._gemm_backend)
+        proj = self.gate_up_proj
+        if proj.is_int8:
+            h = int8_silu_mul_linear(x, proj.weight_codes, proj.weight_scales, backend=self._gemm_backend)
+        else:
+            h = silu_mul_linear(x, proj.weight, backend=self._gemm_backend)
         return self.down_proj(h)
 
     def forward_add_norm(self, hidden: torch.Tensor, residual: torch.Tensor,
@@ -53,7 +58,13 @@ class Qwen35MLP(nn.Module):
         """``self(norm(hidden, residual))`` with the new residual: the
         post-attention norm and MLP of a decoder layer
         (nanovllm/models/qwen3_5.py:200-204).  On the HIP path the residual
-        add, the norm, gate_up_proj and SiluAndMul are one launch."""
-        h, new_residual = add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, self.gate_up_proj.weight,
-                                             silu_mul=True, backend=self._gemm_backend)
+        add, the norm, gate_up_proj and SiluAndMul are one launch (two with
+        weights in 8 bits)."""
+        proj = self.gate_up_proj
+        if proj.is_int8:
+            h, new_residual = int8_add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, proj.weight_codes,
+                                                      proj.weight_scales, silu_mul=True, backend=self._gemm_backend)
+        else:
+            h, new_residual = add_rmsnorm_linear(hidden, residual, norm.weight, norm.eps, proj.weight, silu_mul=True,
+                                                 backend=self._gemm_backend)
         return self.down_proj(h), new_residual
