@@ -39,29 +39,32 @@ def test_step_in_8_bits(pkg, rows):
     k = torch.full((rows,), 30, dtype=torch.int32, device=DEV)
     p = torch.full((rows,), 0.95, device=DEV)
 
-    def step():
+    def step(given=None):
+        """The stages' outputs; each takes the one before it, or that of ``given``."""
+        before = [None] * 4 if given is None else given
         a = parts["o_proj"].forward_gated(heads, gate)
-        out, res = parts["mlp"].forward_add_norm(a + h, r, parts["norm"])
-        plain = parts["mlp"](out)
-        return a, out, res, plain, parts["head"](out), *parts["head"].draw(out, t, u, k, p)
+        out, res = parts["mlp"].forward_add_norm((a if given is None else before[0]) + h, r, parts["norm"])
+        plain = parts["mlp"](out if given is None else before[1])
+        logits = parts["head"](out if given is None else before[1])
+        return a, out, res, plain, logits
 
     backend(parts, "hip")
     hip = step()
     again = step()
     assert all(torch.equal(x, y) for x, y in zip(hip, again))
+    tokens, shares = parts["head"].draw(hip[1], t, u, k, p)
     backend(parts, "torch")
-    ref = step()
     # Codes and sums are the same but where a rounding to 16 bits, or the norm's
     # last bits, fall to the other side: then an element is a step (2^-8 of it)
     # or a code (1 / 127 of a row's largest value, a third of which is the rms)
     # off.  Were each off by as much at random, outputs were off by 1%.
-    for x, y in zip(hip[:5], ref[:5]):
+    for x, y in zip(hip, step(hip)):
         assert x.dtype == y.dtype and x.shape == y.shape
         assert (x.float() - y.float()).norm() <= 0.01 * y.float().norm()
     logits = hip[4].double().cpu().numpy()
     for i in range(rows):
         token, share = orc.sample(logits[i], float(t[i]), float(u[i]), 30, float(p[i]))
-        assert hip[5][i] == token and abs(hip[6][i].item() - share) <= abs(share) * 2.0 ** -24 + 1e-11
+        assert tokens[i] == token and abs(shares[i].item() - share) <= abs(share) * 2.0 ** -24 + 1e-11
 
 
 @torch.no_grad()
