@@ -5,16 +5,31 @@
 // logit first, lowest index first among equals), so what is kept is given by one
 // border: the pair (logit, index) of the last token that all of them keep.  No
 // row is sorted.  With c = 16 log2(e) / T a token's weight is 2^((l c) / 16), and
-// floor(l c) puts it into one of 1024 bins of 1/16 octave below the largest
-// logit's; within a bin weights differ by less than 2^(1/16), and the exponent's
-// fraction is a short polynomial.  A histogram of counts and weights by bin
-// finds the bin of a border, and only that bin's members are put in order.
+// the whole number next to l c puts it into one of 1024 bins of 1/16 octave below
+// the largest logit's; within a bin weights differ by less than 2^(1/16), and
+// what is left of l c is the argument of a short polynomial.  A histogram of
+// counts and weights by bin finds the bin of a border, and only that bin's
+// members are put in order.
 //
-// Numerics: l c is held as a product and its remainder in 64 bits, so its
-// fraction is exact at any size of l c; a weight within its bin is rounded to a
-// multiple of 2^-40 and summed as an integer.  Sums do not depend on the order
-// of atomics, and a border falls where 64-bit arithmetic puts it.  The last bin
-// holds everything from 2^-63.9 of the largest weight down, which counts as 0.
+// A row is read once.  Workgroups keep slices of it in LDS, bin them below their
+// own largest logit (the whole number is the same whatever it is counted from,
+// so slices are joined by a shift) and leave their histogram and their first few
+// members, 1/64 of a slice.  One workgroup a row joins the histograms; where all
+// that is kept is among the listed members (usual: a top-k, or a distribution
+// with peaks), it puts those in order and draws.  Otherwise it looks the members
+// of the border's bin up in the row, and draws in the slice in which the running
+// sum passes u times the total, which it reads again.
+//
+// What bounds it: with many rows the instructions of a weight (about 30 a logit);
+// with few the join, a chain of short steps whose code is fetched from L2 as it
+// runs (75 ns a 64-byte line): loops are left rolled and what a step shares with
+// another is a call.
+//
+// Numerics: l c is held as a product and its remainder; a weight within its bin
+// is a whole number of 2^-36, off by two of them at most, and summed as one, in
+// one 64-bit word with the count.  Sums over bins are in 64 bits and do not depend
+// on the order of atomics.  The last bin holds everything from 2^-63.9 of the
+// largest weight down, which counts as 0.
 #include "int8_common.hpp"
 
 namespace nvg {
@@ -25,7 +40,7 @@ constexpr int kBins = 1024;
 constexpr int kRest = kBins - 1;      // bin of the tokens without weight
 constexpr int kPer = 8;               // logits a thread takes at once
 constexpr int kTile = kThreads * kPer;
-constexpr int kList = 4096;           // members of a bin that are put in order at once
+constexpr int kList = 512;           // members of a bin that are put in order at once
 constexpr uint32_t kNanKey = 0xFFC00000u;
 
 // Logits as integers of the same order (argmax_order), and back.
@@ -38,69 +53,147 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int index) {
     return (uint64_t(key) << 32) | uint64_t(0xFFFFFFFFu - uint32_t(index));
 }
 
+// A token's weight: 2^(-bin / 16) * (1 + off * 2^-36).
 struct Weight {
     int bin;
-    double part;   // weight within its bin, 0.97 .. 1.03, a multiple of 2^-40
+    int32_t off;   // within 1.6e9 of 0
 };
+constexpr double kUnit = 0x1p-36;
+
+__device__ __forceinline__ double part_of(int32_t off) { return 1.0 + double(off) * kUnit; }
+// A part in units.
+__device__ __forceinline__ uint64_t units_of(int32_t off) { return (uint64_t(1) << 36) + int64_t(off); }
 
 // How a row weighs its logits.
 struct Scale {
-    double c;      // 16 log2(e) / T
-    double top;    // floor(c * largest logit)
+    double c;        // 16 log2(e) / T
+    float ch, cl;    // the same as a sum
+    double top;      // the largest logit's rounded product with it
+    float topf;
     float largest;
-    bool flat;     // the largest logit is an infinity: its holders share the row
+    bool flat;       // the largest logit is an infinity: its holders share the row
 };
+
+// A logit's product with c, rounded to a whole number: in 32 bits where it is at
+// most kNear, beyond that in 64 (never nearer to 0 than kNear, so that it does
+// not fall with the logit).
+constexpr float kNear = 16384.0f;
+
+__device__ __forceinline__ double far_product(float l, const Scale& s, double& rest) {
+#pragma clang fp contract(off)   // hi - f below is of the rounded product
+    const double hi = double(l) * s.c, lo = __builtin_fma(double(l), s.c, -hi);
+    double f = __builtin_rint(hi);
+    f = f > 0.0 ? __builtin_fmax(f, double(kNear)) : __builtin_fmin(f, -double(kNear));
+    // Beyond 2^53 a product has no fraction, and its remainder, the same for all
+    // tokens that can share its bin, is cut.
+    rest = __builtin_fmin(__builtin_fmax((hi - f) + lo, -0.5), 0.5);
+    return f;
+}
+
+// A logit's product as a whole number.
+__device__ __forceinline__ double top_of(float l, const Scale& s) {
+    const float hi = l * s.ch;
+    double rest;
+    return __builtin_fabsf(hi) <= kNear ? double(__builtin_rintf(hi)) : far_product(l, s, rest);
+}
 
 __device__ __forceinline__ Scale scale_of(float largest, float t) {
     Scale s;
     s.c = 16.0 * 1.4426950408889634074 / double(t);
-    s.top = __builtin_floor(double(largest) * s.c);
+    s.ch = float(s.c);
+    s.cl = float(s.c - double(s.ch));
+    s.top = top_of(largest, s);
+    s.topf = float(s.top);
     s.largest = largest;
     s.flat = !(__builtin_fabsf(largest) < __builtin_inff());
     return s;
 }
 
-// 1 unit is 2^-40: 2^12 * 1.5 plus a part is rounded to a multiple of it.
-constexpr double kRound = 6144.0;
+// Of a row whose largest logit is finite.  Near 0 the product is a sum of two
+// floats whose error is below 2^-24 of its last place, 2^-36 of a weight at a
+// product of 2^13 and less below; y, the product less the whole number, is exact.
+// 2^(y / 16) - 1 in units of 2^-36: the linear term as a float and its remainder,
+// the others, to the 5th power, with the remainder (off by less than 2^-43).
+// A vector instruction in 64 bits takes as long as four in 32 here, and the
+// sum of both terms as integers takes the place of a wider type.
+__device__ __forceinline__ Weight weigh_finite(float l, const Scale& s) {
+#pragma clang fp contract(off)
+    constexpr double a = 0.69314718055994530942 / 16.0, unit = 0x1p36;
+    constexpr float ah = float(a * unit), al = float(a * unit - double(float(a * unit)));
+    const float hi = l * s.ch;
+    float y, low, down;
+    if (__builtin_fabsf(hi) > kNear && !(hi < s.topf - 2048.0f)) {
+        double rest;
+        down = float(s.top - far_product(l, s, rest));
+        y = float(rest);
+        low = float(rest - double(y));
+    } else {
+        const float f = __builtin_rintf(hi);
+        y = hi - f;
+        low = __builtin_fmaf(l, s.cl, __builtin_fmaf(l, s.ch, -hi));
+        down = s.topf - f;
+    }
+    const float z = y + low;   // of the terms from the 2nd power on
+    float q = __builtin_fmaf(float(a * a * a * a * a / 120.0 * unit), z, float(a * a * a * a / 24.0 * unit));
+    q = __builtin_fmaf(q, z, float(a * a * a / 6.0 * unit));
+    q = __builtin_fmaf(q, z, float(a * a / 2.0 * unit));
+    const float p = ah * y;
+    float r = __builtin_fmaf(al, y, __builtin_fmaf(ah, y, -p));
+    r = __builtin_fmaf(ah, low, r);
+    r = __builtin_fmaf(q, z * z, r);
+    // -inf is as far down as there is, and so is 0 * inf at T = inf (a NaN).
+    return Weight{int(__builtin_fminf(down, float(kRest))), int32_t(p) + int32_t(r)};
+}
 
 __device__ __forceinline__ Weight weigh(float l, const Scale& s) {
-#pragma clang fp contract(off)   // hi - f below is of the rounded product
-    if (s.flat) return Weight{l == s.largest ? 0 : kRest, 1.0};
-    const double hi = double(l) * s.c, lo = __builtin_fma(double(l), s.c, -hi), f = __builtin_floor(hi);
-    const double down = s.top - f;
-    // -inf, and 0 * inf at T = inf, are not below kRest either.
-    const int bin = down < double(kRest) ? int(down) : kRest;
-    // 2^(x / 16) around the middle of the bin: e^(x ln2 / 16) to the 6th power
-    // is off by less than 2^-51.  Beyond 2^53 a product has no fraction, and its
-    // remainder, the same for all tokens that can share its bin, is cut.
-    double x = (hi - f) + lo - 0.5;
-    x = __builtin_fmin(__builtin_fmax(x, -1.0), 1.0);
-    constexpr double a = 0.69314718055994530942 / 16.0;
-    double p = a * a * a * a * a * a / 720.0;
-    p = __builtin_fma(p, x, a * a * a * a * a / 120.0);
-    p = __builtin_fma(p, x, a * a * a * a / 24.0);
-    p = __builtin_fma(p, x, a * a * a / 6.0);
-    p = __builtin_fma(p, x, a * a / 2.0);
-    p = __builtin_fma(p, x, a);
-    p = __builtin_fma(p, x, 1.0);
-    return Weight{bin, (p + kRound) - kRound};
+    if (s.flat) return Weight{l == s.largest ? 0 : kRest, 0};
+    return weigh_finite(l, s);
 }
 
-// A part in units of 2^-40.
-__device__ __forceinline__ uint64_t units_of(double part) {
-    return __builtin_bit_cast(uint64_t, part + kRound) - __builtin_bit_cast(uint64_t, kRound);
+// A bin's count and weight in one word: the count from bit 48 up, and below it
+// off + kOff of its members, each below 2^32, so 2^15 members fit.
+constexpr int32_t kOff = 1600000000;
+constexpr int kCountBit = 48;
+constexpr int kMostSlice = 1 << 15;
+
+__device__ __forceinline__ uint64_t packed(int32_t off) {
+    return (uint64_t(1) << kCountBit) | uint32_t(off + kOff);
+}
+__device__ __forceinline__ uint32_t count_of(uint64_t word) { return uint32_t(word >> kCountBit); }
+__device__ __forceinline__ uint64_t sum_of(uint64_t word) {
+    return (word & ((uint64_t(1) << kCountBit) - 1)) + count_of(word) * ((uint64_t(1) << 36) - uint64_t(kOff));
 }
 
-// 2^(-bin / 16).
+// A key no larger than that of any logit of bin `last` or above: what its bound
+// in 64 bits says, with room for the roundings.  0 where that says nothing.
+__device__ __forceinline__ uint32_t key_floor(int last, const Scale& s) {
+    const double l = (s.top - double(last) - 0.5) / s.c;
+    if (s.flat || last >= kRest || !(__builtin_fabs(l) < 3.0e38)) return 0;
+    const uint32_t key = argmax_order(float(l));
+    return key > 4 ? key - 4 : 0;
+}
+
+// The same from above: no smaller than any key of bin `first` or below.
+__device__ __forceinline__ uint32_t key_ceiling(int first, const Scale& s) {
+    const uint32_t most = argmax_order(s.largest);
+    const double l = (s.top - double(first) + 0.5) / s.c;
+    if (s.flat || !(__builtin_fabs(l) < 3.0e38)) return most;
+    const uint32_t key = argmax_order(float(l)) + 4;
+    return key < most ? key : most;
+}
+
+// 2^(-bin / 16), by the bits of bin.
 __device__ __forceinline__ double bin_scale(int bin) {
-    constexpr double root[16] = {1.0,
-                                 0.95760328069857364694, 0.91700404320467123174, 0.87812608018664974156,
-                                 0.84089641525371454303, 0.80524516597462715411, 0.77110541270397041180,
-                                 0.73841307296974965571, 0.70710678118654752440, 0.67712777346844636414,
-                                 0.64841977732550483296, 0.62092890603674202431, 0.59460355750136053336,
-                                 0.56939431737834582684, 0.54525386633262882960, 0.52213689121370692017};
-    return __builtin_ldexp(root[bin & 15], -(bin >> 4));
+    double x = bin & 1 ? 0.95760328069857364694 : 1.0;
+    x *= bin & 2 ? 0.91700404320467123174 : 1.0;
+    x *= bin & 4 ? 0.84089641525371454303 : 1.0;
+    x *= bin & 8 ? 0.70710678118654752440 : 1.0;
+    return __builtin_ldexp(x, -(bin >> 4));
 }
+
+// weigh_finite and log as calls, for where they run once.
+__device__ __attribute__((noinline)) Weight weigh_once(float l, Scale s) { return weigh_finite(l, s); }
+__device__ __attribute__((noinline)) double log_once(double x) { return log(x); }
 
 template <int DT>
 __device__ __forceinline__ float logit_at(const char* row, int i) {
@@ -108,167 +201,274 @@ __device__ __forceinline__ float logit_at(const char* row, int i) {
     else return half_to_f32<DT>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// Logits i .. i + 7 of a row of n (-inf past its end; they are told apart by their index).
-template <int DT>
-__device__ __forceinline__ void load_logits(const char* row, int i, int n, float (&l)[kPer]) {
-    if (i + kPer <= n) {
+// Logits i .. i + C - 1 (4 or 8) of a row of n; NaN past its end.
+template <int DT, int C>
+__device__ __forceinline__ void load_logits(const char* row, int i, int n, float* l) {
+    if (i + C <= n) {
         if constexpr (DT == NANOVLLM_GEMM_F32) {
-            f32x4_t v[2];
-            __builtin_memcpy(v, row + int64_t(i) * 4, 32);
+            f32x4_t v[C / 4];
+            __builtin_memcpy(v, row + int64_t(i) * 4, C * 4);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) l[e] = v[e >> 2][e & 3];
+            for (int e = 0; e < C; ++e) l[e] = v[e >> 2][e & 3];
         } else {
-            u32x4_t v;
-            __builtin_memcpy(&v, row + int64_t(i) * 2, 16);
+            u32x2_t v[C / 4];
+            __builtin_memcpy(v, row + int64_t(i) * 2, C * 2);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) l[e] = half_to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
+            for (int e = 0; e < C; ++e) l[e] = half_to_f32<DT>(uint16_t(v[e >> 2][(e >> 1) & 1] >> (16 * (e & 1))));
         }
         return;
     }
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) l[e] = i + e < n ? logit_at<DT>(row, i + e) : -__builtin_inff();
+    for (int e = 0; e < C; ++e) l[e] = i + e < n ? logit_at<DT>(row, i + e) : __builtin_nanf("");
 }
 
 // ---------------------------------------------------------------------------
 // Sums over the workgroup.
 // ---------------------------------------------------------------------------
+constexpr int kMostSlices = 256;
+constexpr int kFew = 2 * kThreads;    // listed members that decide: two a thread
+
+// Where a bin is cut.
+struct Border {
+    uint64_t place;   // the last member in front of the cut
+    double mass;      // weight up to and with it, in parts
+    bool listed;      // sh.list holds the bin's members
+};
+
 struct Shared {
-    uint32_t count[kBins];     // tokens of a bin, then of the bins up to it
-    uint64_t units[kBins];     // weight of a bin in units
-    double mass[kBins];        // weight of the bins up to it
+    uint32_t count[kBins];     // tokens of the bins up to one
+    uint64_t words[kBins];     // the histogram (packed) while a slice is binned
+    double mass[kBins];        // weight of the bins up to one
     union {
-        uint64_t list[kList];
+        struct { uint64_t list[kList], units[kList], front[kList]; uint32_t rank[kList]; };
+        uint64_t few[kFew];    // listed members of a row of one slice, by index
         struct { uint32_t count[kBins]; uint64_t units[kBins]; } sub;
         double tile[kBins];    // kept weight of the row's tiles
     };
     uint64_t part64[kThreads / 64];
     double partd[kThreads / 64];
     uint32_t part32[kThreads / 64];
-    int pick;
+    int listed[kMostSlices];         // members a slice lists
+    int shift[kMostSlices];          // bins from the row's largest logit down to a slice's
+    uint64_t slice[kMostSlices];     // kept members of the border's bin by slice, in units
+    uint32_t some[kThreads / 64];
     int fill;
-    uint64_t border;
+    Scale scale;
+    Border border;
 };
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int off) {
-    return (uint64_t(uint32_t(__shfl_xor(int(v >> 32), off))) << 32) | uint32_t(__shfl_xor(int(uint32_t(v)), off));
-}
+// Moves between lanes as DPP: rows are 16 lanes; kShr + n takes the value n lanes
+// down the row, kBcast15 and kBcast31 give a row's last lane to the next row, and
+// lane 31 to the upper half.  Lanes that get none keep `old`.
+constexpr int kShr = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;
 
-__device__ __forceinline__ uint64_t max_all(uint64_t v, Shared& sh) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const uint64_t o = shfl_xor64(v, off);
-        v = o > v ? o : v;
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T moved(T old, T v) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t o = __builtin_bit_cast(uint64_t, old), b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(int(uint32_t(o)), int(uint32_t(b)), CTRL, ROWS, 15, false));
+        const uint32_t hi =
+            uint32_t(__builtin_amdgcn_update_dpp(int(uint32_t(o >> 32)), int(uint32_t(b >> 32)), CTRL, ROWS, 15, false));
+        return __builtin_bit_cast(T, (uint64_t(hi) << 32) | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v),
+                                                                 CTRL, ROWS, 15, false));
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.part64[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) v = sh.part64[w] > v ? sh.part64[w] : v;
-    return v;
 }
 
-__device__ __forceinline__ double sum_all(double v, Shared& sh) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
+// What lane `lane` (the same in all) holds.
+template <typename T>
+__device__ __forceinline__ T from_lane(T v, int lane) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), lane));
+        const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b >> 32)), lane));
+        return __builtin_bit_cast(T, (uint64_t(hi) << 32) | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+
+constexpr int kWaves = kThreads / 64;
+static_assert(kWaves == 16, "a wave's partial sums fill a row");
+
+struct Add {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T x, T y) const { return x + y; }
+};
+struct Max {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T x, T y) const { return x > y ? x : y; }
+};
+
+// Inclusive over the lanes of a row, and over those of a wave (0 is neutral).
+template <typename F, typename T>
+__device__ __forceinline__ T row_scan(T v, F f) {
+    v = f(v, moved<kShr + 1, 15>(T(0), v));
+    v = f(v, moved<kShr + 2, 15>(T(0), v));
+    v = f(v, moved<kShr + 4, 15>(T(0), v));
+    return f(v, moved<kShr + 8, 15>(T(0), v));
+}
+template <typename F, typename T>
+__device__ __forceinline__ T wave_scan(T v, F f) {
+    v = row_scan(v, f);
+    v = f(v, moved<kBcast15, 10>(T(0), v));
+    return f(v, moved<kBcast31, 12>(T(0), v));
+}
+
+template <typename T>
+__device__ __attribute__((noinline)) T max_over(T v, T* part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v, Max{});
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.partd[threadIdx.x >> 6] = v;
+    if (lane == 63) part[wave] = v;
     __syncthreads();
-    v = 0.0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) v += sh.partd[w];
-    return v;
+    return from_lane(row_scan(part[lane & (kWaves - 1)], Max{}), kWaves - 1);
 }
 
 // Inclusive sums over the threads in order.
-__device__ __forceinline__ double scan(double v, Shared& sh) {
+template <typename T>
+__device__ __attribute__((noinline)) T scan_over(T v, T* part) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_scan(v, Add{});
+    __syncthreads();
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    const T upto = row_scan(part[lane & (kWaves - 1)], Add{});
+    return wave > 0 ? from_lane(upto, wave - 1) + v : v;
+}
+
+// The number of the first (or last) thread that says yes; `none` if none does.
+__device__ __attribute__((noinline)) int pick(bool yes, int number, int none, bool last, uint32_t* part, uint32_t* some) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(v, off);
-        if (lane >= off) v += o;
+    uint64_t all = __ballot(yes);
+    int at = last ? 63 - __builtin_clzll(all | 1) : __builtin_ctzll(all | (uint64_t(1) << 63));
+    const int mine = from_lane(number, __builtin_amdgcn_readfirstlane(at));
+    __syncthreads();
+    if (lane == 0) {
+        part[wave] = uint32_t(mine);
+        some[wave] = all != 0;
     }
     __syncthreads();
-    if (lane == 63) sh.partd[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < wave; ++w) before += sh.partd[w];
-    return before + v;
+    const uint32_t theirs = part[lane & (kWaves - 1)];
+    all = __ballot(lane < kWaves && some[lane & (kWaves - 1)] != 0);
+    at = last ? 63 - __builtin_clzll(all | 1) : __builtin_ctzll(all | (uint64_t(1) << 63));
+    const int found = int(from_lane(theirs, __builtin_amdgcn_readfirstlane(at) & (kWaves - 1)));
+    return all != 0 ? found : none;
 }
 
-__device__ __forceinline__ uint32_t scan(uint32_t v, Shared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), off));
-        if (lane >= off) v += o;
-    }
-    __syncthreads();
-    if (lane == 63) sh.part32[wave] = v;
-    __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < wave; ++w) before += sh.part32[w];
-    return before + v;
+template <typename S>
+__device__ __forceinline__ uint64_t max_all(uint64_t v, S& sh) { return max_over<uint64_t>(v, sh.part64); }
+template <typename S>
+__device__ __forceinline__ uint32_t max_all(uint32_t v, S& sh) { return max_over<uint32_t>(v, sh.part32); }
+__device__ __forceinline__ double scan(double v, Shared& sh) { return scan_over<double>(v, sh.partd); }
+template <typename S>
+__device__ __forceinline__ uint32_t scan(uint32_t v, S& sh) { return scan_over<uint32_t>(v, sh.part32); }
+template <typename S>
+__device__ __forceinline__ uint64_t scan(uint64_t v, S& sh) { return scan_over<uint64_t>(v, sh.part64); }
+template <typename S>
+__device__ __forceinline__ int first_of(bool yes, int number, int none, S& sh) {
+    return pick(yes, number, none, false, sh.part32, sh.some);
 }
-
-// The first number for which a thread says yes (`none` if none does).
-__device__ __forceinline__ int first_of(bool yes, int number, int none, Shared& sh) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.pick = none;
-    __syncthreads();
-    if (yes) atomicMin(&sh.pick, number);
-    __syncthreads();
-    return sh.pick;
-}
-
 __device__ __forceinline__ int last_of(bool yes, int number, int none, Shared& sh) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.pick = none;
-    __syncthreads();
-    if (yes) atomicMax(&sh.pick, number);
-    __syncthreads();
-    return sh.pick;
+    return pick(yes, number, none, true, sh.part32, sh.some);
 }
 
-// ---------------------------------------------------------------------------
-// The border within a bin: the place of its need-th member (by_mass false), or
-// of the member at which the running weight, in parts, reaches `want` (true),
-// and the weight up to and with it, in parts.
-// ---------------------------------------------------------------------------
-struct Border {
-    uint64_t place;
-    double mass;
-};
+// What thread `from` holds, in every thread.
+template <typename T>
+__device__ __forceinline__ T given_by(int from, T v, T* part) {
+    __syncthreads();
+    if (int(threadIdx.x) == from) part[0] = v;
+    __syncthreads();
+    return part[0];
+}
 
 // Calls f(index, logit) for every logit of the row.
 template <int DT, typename F>
 __device__ __forceinline__ void each_logit(const char* row, int vocab, F f) {
-    for (int i = threadIdx.x * kPer; i < vocab; i += kTile) {
-        float l[kPer];
-        load_logits<DT>(row, i, vocab, l);
+    constexpr int kAhead = 2;   // loads in flight
+    for (int base = threadIdx.x * kPer; base < vocab; base += kAhead * kTile) {
+        float l[kAhead][kPer];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            if (i + e < vocab) f(i + e, l[e]);
+        for (int a = 0; a < kAhead; ++a)
+            if (base + a * kTile < vocab) load_logits<DT, kPer>(row, base + a * kTile, vocab, l[a]);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = base + a * kTile;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (i + e < vocab) f(i + e, l[a][e]);
+        }
     }
 }
 
+// ---------------------------------------------------------------------------
+// The border within a bin, in sh.border: its need-th member (kByCount), the
+// member at which the running weight, in parts, reaches `want` (kByMass), or the
+// key `need` itself (kByKey, for the list of the bin's members).
+// ---------------------------------------------------------------------------
+enum { kByCount, kByMass, kByKey };
+
+// The border among the `members` places in sh.list, which are of one bin.  The
+// threads of a member, 1024 / members of them, count the places in front of it
+// and sum their weights (whole numbers, in any order).
+__device__ __attribute__((noinline)) void border_of_list(int members, int mode, uint32_t need, double want, double above,
+                                                         bool whole, Shared& sh) {
+    int size = 64;
+    while (size < members) size *= 2;
+    const int i = threadIdx.x & (size - 1), part = threadIdx.x / size, parts = kThreads / size;
+    __syncthreads();
+    const uint64_t place = i < members ? sh.list[i] : 0;
+    const uint64_t units = i < members ? units_of(weigh(logit_of(uint32_t(place >> 32)), sh.scale).off) : 0;
+    if (part == 0) {
+        sh.units[i] = units;
+        sh.front[i] = 0;
+        sh.rank[i] = 0;
+    }
+    if (threadIdx.x == 0) sh.border = Border{uint64_t(need) << 32, above, whole};   // where all lie behind the cut
+    __syncthreads();
+    uint32_t rank = 0;
+    uint64_t front = 0;
+#pragma unroll 4
+    for (int j = part; j < members; j += parts) {
+        const bool ahead = sh.list[j] > place;
+        rank += ahead;
+        front += ahead ? sh.units[j] : 0;
+    }
+    if (i < members) {
+        atomicAdd(&sh.rank[i], rank);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.front[i]), static_cast<unsigned long long>(front));
+    }
+    __syncthreads();
+    // The one that the cut lies behind; the last where rounding leaves the whole
+    // a little short.
+    if (part == 0 && i < members) {
+        rank = sh.rank[i];
+        const double before = double(sh.front[i]) * kUnit, upto = double(sh.front[i] + units) * kUnit;
+        bool cut;
+        if (mode == kByMass) cut = (upto >= want || rank + 1 == uint32_t(members)) && (before < want || rank == 0);
+        else if (mode == kByCount) cut = rank + 1 == need;
+        else cut = false;
+        if (cut) sh.border = Border{place, above + upto, whole};
+    }
+    __syncthreads();
+}
+
 template <int DT>
-__device__ Border border_in(const char* row, int vocab, const Scale& sc, int bin, uint32_t members, bool by_mass,
-                            uint32_t need, double want, Shared& sh) {
+__device__ __forceinline__ void border_in(const char* row, int vocab, const Scale& sc, int bin, uint32_t members,
+                                          int mode, uint32_t need, double want, Shared& sh) {
+    const bool by_mass = mode == kByMass;
     // Keys of the members still in question, lo .. hi; need and want go down by
     // what lies above them.
-    uint32_t lo = 0, hi = 0xFFFFFFFFu;
+    uint32_t lo = key_floor(bin, sc), hi = key_ceiling(bin, sc);
     double above = 0.0;
+    const bool whole = members <= uint32_t(kList);
     auto inside = [&](float l, uint32_t key) { return key >= lo && key <= hi && weigh(l, sc).bin == bin; };
-    if (members > uint32_t(kList)) {
-        uint32_t low = 0xFFFFFFFFu, high = 0;
-        each_logit<DT>(row, vocab, [&](int, float l) {
-            if (weigh(l, sc).bin != bin) return;
-            const uint32_t key = argmax_order(l);
-            low = key < low ? key : low;
-            high = key > high ? key : high;
-        });
-        hi = uint32_t(max_all(high, sh));
-        lo = 0xFFFFFFFFu - uint32_t(max_all(0xFFFFFFFFu - low, sh));
+    if (members > uint32_t(kList) && mode == kByKey) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.border = Border{uint64_t(need) << 32, 0.0, false};
+        __syncthreads();
+        return;
     }
     while (members > uint32_t(kList) && lo < hi) {
         const uint32_t width = (hi - lo) / kBins + 1;
@@ -282,11 +482,11 @@ __device__ Border border_in(const char* row, int vocab, const Scale& sc, int bin
             const uint32_t b = (hi - key) / width;
             atomicAdd(&sh.sub.count[b], 1u);
             atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sub.units[b]),
-                      static_cast<unsigned long long>(units_of(weigh(l, sc).part)));
+                      static_cast<unsigned long long>(units_of(weigh(l, sc).off)));
         });
         __syncthreads();
         const uint32_t n = sh.sub.count[threadIdx.x];
-        const double m = double(sh.sub.units[threadIdx.x]) * 0x1p-40;
+        const double m = double(sh.sub.units[threadIdx.x]) * kUnit;
         const uint32_t counts = scan(n, sh);
         const double masses = scan(m, sh);
         const int at = first_of(n > 0 && (by_mass ? masses >= want : counts >= need), threadIdx.x, kBins, sh);
@@ -308,7 +508,7 @@ __device__ Border border_in(const char* row, int vocab, const Scale& sc, int bin
     }
     if (members > uint32_t(kList)) {
         // Equals: the c-th of them by index.
-        const double part = weigh(logit_of(hi), sc).part;
+        const double part = part_of(weigh(logit_of(hi), sc).off);
         uint32_t c = need;
         if (by_mass) {
             c = want > 0.0 ? uint32_t(__builtin_ceil(want / part)) : 1u;
@@ -319,7 +519,7 @@ __device__ Border border_in(const char* row, int vocab, const Scale& sc, int bin
             const int i = base + int(threadIdx.x) * kPer;
             uint32_t here = 0;
             float l[kPer];
-            load_logits<DT>(row, i, vocab, l);
+            load_logits<DT, kPer>(row, i, vocab, l);
 #pragma unroll
             for (int e = 0; e < kPer; ++e) here += i + e < vocab && argmax_order(l[e]) == hi;
             const uint32_t upto = scan(here, sh);
@@ -332,70 +532,25 @@ __device__ Border border_in(const char* row, int vocab, const Scale& sc, int bin
                 if (k < c && seen + upto >= c) {
 #pragma unroll
                     for (int e = 0; e < kPer; ++e)
-                        if (i + e < vocab && argmax_order(l[e]) == hi && ++k == c) sh.border = place_of(hi, i + e);
+                        if (i + e < vocab && argmax_order(l[e]) == hi && ++k == c)
+                            sh.border = Border{place_of(hi, i + e), above + double(c) * part, false};
                 }
                 __syncthreads();
-                return Border{sh.border, above + double(c) * part};
+                return;
             }
             seen += all;
         }
-        return Border{place_of(hi, vocab - 1), above + double(members) * part};   // not reached
+        return;   // not reached: there are c of them
     }
-    // A list in order.
+    // The members, in any order; each finds what lies in front of it.
     __syncthreads();
     if (threadIdx.x == 0) sh.fill = 0;
-    int size = 64;
-    while (size < int(members)) size *= 2;
-    for (int i = threadIdx.x; i < size; i += kThreads) sh.list[i] = 0;
     __syncthreads();
     each_logit<DT>(row, vocab, [&](int i, float l) {
         const uint32_t key = argmax_order(l);
         if (inside(l, key)) sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place_of(key, i);
     });
-    for (int span = 2; span <= size; span *= 2) {
-        for (int step = span / 2; step >= 1; step /= 2) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int i = 2 * t - (t & (step - 1)), j = i + step;
-                const uint64_t x = sh.list[i], y = sh.list[j];
-                if ((x < y) == ((i & span) == 0)) {   // descending runs first
-                    sh.list[i] = y;
-                    sh.list[j] = x;
-                }
-            }
-        }
-    }
-    __syncthreads();
-    constexpr int kEach = kList / kThreads;
-    uint64_t place[kEach];
-    double part[kEach], mine = 0.0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int i = int(threadIdx.x) * kEach + e;
-        place[e] = i < int(members) ? sh.list[i] : 0;
-        part[e] = i < int(members) ? weigh(logit_of(uint32_t(place[e] >> 32)), sc).part : 0.0;
-        mine += part[e];
-    }
-    double run = scan(mine, sh) - mine;   // exact: at most 2^12 parts of 2^-40
-    int at = kList;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int i = int(threadIdx.x) * kEach + e;
-        run += part[e];
-        part[e] = run;
-        if (at == kList && i < int(members) && (by_mass ? run >= want : i + 1 >= int(need))) at = i;
-    }
-    at = first_of(at < kList, at, int(members) - 1, sh);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-        if (int(threadIdx.x) * kEach + e == at) {
-            sh.border = place[e];
-            sh.partd[0] = part[e];
-        }
-    __syncthreads();
-    const Border b{sh.border, above + sh.partd[0]};
-    __syncthreads();
-    return b;
+    border_of_list(int(members), mode, need, want, above, whole, sh);
 }
 
 struct RowArgs {
@@ -407,168 +562,659 @@ struct RowArgs {
     float* logprobs;
     int64_t ld;
     int32_t vocab;
+    // What slices leave: `slices` of `step` logits a row.
+    char* work;
+    int32_t slices, step;
 };
 
-// One workgroup a row.
-template <int DT>
+// A slice's record in the workspace.
+struct Record {
+    uint64_t best;       // its first place
+    int32_t listed;      // members listed
+    int32_t last;        // its last bin (counted from its own largest) all of whose members are listed; -1: none
+    uint64_t words[kBins];
+    // then the listed places, by index, list_room of them at most
+};
+
+// Members a slice lists: a few of its tokens, and of a row kFew at most.  Even, so
+// that a thread of the join takes two next to each other.
+__host__ __device__ inline int list_room(int step, int slices) {
+    const int share = kFew / (slices > 0 ? slices : 1) & ~1;
+    return step / 128 < share ? step / 128 : share;
+}
+__host__ __device__ inline int64_t record_bytes(int step, int slices) {
+    return int64_t(sizeof(Record)) + list_room(step, slices) * 8;
+}
+
+template <int STEP>
+struct SliceShared {
+    uint64_t words[kBins];
+    uint64_t part64[kWaves];
+    uint32_t part32[kWaves], some[kWaves];
+};
+
+// A slice of up to STEP logits from `begin` on, kept in LDS as they are given;
+// NaN past the end.  Thread t has logits 8 t .. 8 t + 7 of every 8192.
+template <int DT, int STEP>
+struct Slice {
+    static constexpr int B = DT == NANOVLLM_GEMM_F32 ? 4 : 2, E = 16 / B, G = STEP / kTile;
+    static_assert(G * kTile == STEP && G <= 4, "a count of 16 bits a group");
+    char* kept;      // STEP * B bytes
+    int begin, n;
+    uint64_t best;   // its first place
+    Scale sc;
+
+    __device__ __forceinline__ int first(int g) const { return g * kTile + int(threadIdx.x) * kPer; }
+
+    static constexpr int R = G * kPer / E;   // 16-byte loads a thread
+    // Whole runs of 8 logits of the slice from `from` on (of size logits).
+    static __device__ __forceinline__ void request(const char* row, int from, int size, u32x4_t (&v)[R]) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int i = g * kTile + int(threadIdx.x) * kPer;
+            if (i + kPer <= size) {
+#pragma unroll
+                for (int h = 0; h < kPer / E; ++h)
+                    __builtin_memcpy(&v[g * (kPer / E) + h], row + int64_t(from + i + h * E) * B, 16);
+            }
+        }
+    }
+
+    // Puts it into LDS and finds its first place: the largest key, then the first
+    // index that holds it.
+    template <typename S>
+    __device__ __forceinline__ void take(const char* row, const u32x4_t (&v)[R], S& sh) {
+        float top = -__builtin_inff();
+        bool nan = false;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int i = first(g);
+            if (i + kPer <= n) {
+#pragma unroll
+                for (int h = 0; h < kPer / E; ++h) {
+                    chunk(i + h * E) = v[g * (kPer / E) + h];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float l = element(v[g * (kPer / E) + h], e);
+                        top = __builtin_fmaxf(top, l);
+                        nan |= l != l;
+                    }
+                }
+            } else if (i < n) {
+#pragma unroll 1
+                for (int e = 0; e < kPer; ++e) {
+                    uint32_t bits = DT == NANOVLLM_GEMM_F32 ? 0x7FC00000u : DT == NANOVLLM_GEMM_F16 ? 0x7E00u : 0x7FC0u;
+                    if (i + e < n) {
+                        const float l = logit_at<DT>(row, begin + i + e);
+                        top = __builtin_fmaxf(top, l);
+                        nan |= l != l;
+                        if constexpr (B == 4) bits = reinterpret_cast<const uint32_t*>(row)[begin + i + e];
+                        else bits = reinterpret_cast<const uint16_t*>(row)[begin + i + e];
+                    }
+                    if constexpr (B == 4) reinterpret_cast<uint32_t*>(kept)[i + e] = bits;
+                    else reinterpret_cast<uint16_t*>(kept)[i + e] = uint16_t(bits);
+                }
+            }
+        }
+        const uint32_t mine = nan ? kNanKey : argmax_order(top), key = max_all(mine, sh);
+        uint32_t at = 0;   // all bits less the index
+        if (mine == key) {
+#pragma unroll 1
+            for (int g = 0; g < G && at == 0; ++g)
+#pragma unroll 1
+                for (int e = 0; e < kPer && at == 0; ++e)
+                    if (first(g) + e < n && argmax_order(at_index(first(g) + e)) == key)
+                        at = 0xFFFFFFFFu - uint32_t(begin + first(g) + e);
+        }
+        best = (uint64_t(key) << 32) | max_all(at, sh);
+    }
+
+    // Element e of 16 bytes of logits, and the 16 bytes from logit i on.
+    static __device__ __forceinline__ float element(u32x4_t v, int e) {
+        if constexpr (B == 4) {
+            const uint32_t bits = v[e];   // of a vector's element the cast takes the first
+            return __builtin_bit_cast(float, bits);
+        }
+        else return half_to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
+    }
+    __device__ __forceinline__ u32x4_t& chunk(int i) const { return *reinterpret_cast<u32x4_t*>(kept + i * B); }
+
+    __device__ __forceinline__ float at_index(int i) const {
+        if constexpr (B == 4) return __builtin_bit_cast(float, reinterpret_cast<const uint32_t*>(kept)[i]);
+        else return logit_at<DT>(kept, i);
+    }
+
+    // Its histogram in sh.words, four logits side by side.  A slice of infinities
+    // leaves none.
+    template <typename S>
+    __device__ __forceinline__ void bins(S& sh) {
+        sh.words[threadIdx.x] = 0;
+        __syncthreads();
+        if (!sc.flat) {
+#pragma unroll 1
+            for (int i = int(threadIdx.x) * kPer; i < n; i += (i & 4) ? kTile - 4 : 4) {
+                float l[4];
+                if constexpr (B == 4) {
+                    const u32x4_t v = chunk(i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) l[e] = element(v, e);
+                } else {
+                    const u32x2_t v = *reinterpret_cast<const u32x2_t*>(kept + i * B);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) l[e] = half_to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
+                }
+                Weight w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = weigh_finite(l[e], sc);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (w[e].bin < kRest)
+                        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.words[w[e].bin]),
+                                  static_cast<unsigned long long>(packed(w[e].off)));
+            }
+        }
+        __syncthreads();
+    }
+
+    // Calls put(at, index, key) for the logits from `least` on, at = 0, 1, ... by
+    // index; returns how many there are.  16 bits of a word count the logits of
+    // one of its groups.
+    template <typename S, typename F>
+    __device__ __forceinline__ uint32_t list(float least, S& sh, F put) {
+        uint32_t hits = 0;   // bit 8 g + e: logit e of group g is listed
+        uint64_t mine = 0;
+#pragma unroll 1
+        for (int g = 0; g < G; ++g) {
+            if (first(g) >= n) break;
+            uint32_t here = 0;
+#pragma unroll
+            for (int h = 0; h < kPer / E; ++h) {
+                const u32x4_t v = chunk(first(g) + h * E);
+#pragma unroll
+                for (int e = 0; e < E; ++e) here |= element(v, e) >= least ? 1u << (h * E + e) : 0u;
+            }
+            hits |= here << (kPer * g);
+            mine |= uint64_t(__builtin_popcount(here)) << (16 * g);
+        }
+        const uint64_t upto = scan(mine, sh);
+        const uint64_t all = given_by(kThreads - 1, upto, sh.part64);
+        uint64_t at = upto - mine;   // by group, its groups' starts to come
+        uint32_t start = 0;
+#pragma unroll 1
+        for (int g = 0; g < G; ++g) {
+            uint32_t where = start + uint32_t(at >> (16 * g) & 0xFFFFu);
+            for (uint32_t here = hits >> (kPer * g) & 0xFFu; here; here &= here - 1) {
+                const int i = first(g) + __builtin_ctz(here);
+                put(where++, begin + i, argmax_order(at_index(i)));
+            }
+            start += uint32_t(all >> (16 * g) & 0xFFFFu);
+        }
+        return start;
+    }
+};
+
+__device__ __forceinline__ bool draws(float t, uint64_t best) {
+    return t > 1e-10f && uint32_t(best >> 32) != kNanKey;
+}
+
+// The least logit that may be in bin `last` or above.
+__device__ __forceinline__ float least_of(int last, const Scale& s) {
+    const uint32_t floor = key_floor(last, s);
+    return floor > 0 ? logit_of(floor) : -__builtin_inff();
+}
+
+// Workgroups take slice after slice, the logits of the next one on their way
+// while this one is binned.
+template <int DT, int STEP>
+__global__ __launch_bounds__(kThreads, STEP <= 2 * kTile ? 8 : 4) void sample_slices_kernel(
+    RowArgs p, int64_t rows) {
+    using S = Slice<DT, STEP>;
+    __shared__ SliceShared<STEP> sh;
+    __shared__ u32x4_t kept[STEP * S::B / 16];
+    const int64_t total = rows * p.slices;
+    const uint32_t cap = list_room(p.step, p.slices);
+    S slice;
+    slice.kept = reinterpret_cast<char*>(kept);
+    u32x4_t next[S::R];
+    auto row_of = [&](int64_t r) { return p.logits + r * p.ld * S::B; };
+    auto size_of = [&](int s) { return (s + 1) * p.step < p.vocab ? p.step : p.vocab - s * p.step; };
+    int64_t r = blockIdx.x / p.slices;
+    int s = int(blockIdx.x - r * p.slices);
+    S::request(row_of(r), s * p.step, size_of(s), next);
+    for (int64_t at = blockIdx.x; at < total;) {
+        const float t = p.temperatures[r];
+        Record* out = reinterpret_cast<Record*>(p.work + at * record_bytes(p.step, p.slices));
+        slice.begin = s * p.step;
+        slice.n = size_of(s);
+        slice.take(row_of(r), next, sh);
+        at += gridDim.x;
+        r = at / p.slices;
+        s = int(at - r * p.slices);
+        if (at < total) S::request(row_of(r), s * p.step, size_of(s), next);
+        if (threadIdx.x == 0) out->best = slice.best;
+        if (draws(t, slice.best)) {
+            slice.sc = scale_of(logit_of(uint32_t(slice.best >> 32)), t);
+            slice.bins(sh);
+            const uint64_t word = sh.words[threadIdx.x];
+            out->words[threadIdx.x] = word;
+            const uint32_t upto = scan(count_of(word), sh);
+            const int last = first_of(upto > cap, threadIdx.x, kRest, sh) - 1;
+            // Listed is what a logit's size may put into the bins up to `last`; the
+            // join looks again.  Where that is more than there is room for (equals
+            // next to the bin's end), none counts as listed.
+            uint64_t* list = reinterpret_cast<uint64_t*>(out + 1);
+            uint32_t listed = cap + 1;
+            if (last >= 0)
+                listed = slice.list(least_of(last, slice.sc), sh, [&](uint32_t i, int index, uint32_t key) {
+                    if (i < cap) list[i] = place_of(key, index);
+                });
+            if (threadIdx.x == 0) {
+                out->listed = listed <= cap ? int(listed) : 0;
+                out->last = listed <= cap ? last : -1;
+            }
+        }
+        __syncthreads();   // the slice in LDS has been read
+    }
+}
+
+// One workgroup a row.  STEP 0: behind sample_slices_kernel; otherwise the row is
+// one slice of its own.
+template <int DT, int STEP>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     __shared__ Shared sh;
+    __shared__ u32x4_t kept_logits[STEP > 0 ? STEP * Slice<DT, kTile>::B / 16 : 1];
     const int64_t r = blockIdx.x;
-    const int vocab = p.vocab;
+    const int vocab = p.vocab, tid = threadIdx.x;
     const char* row = p.logits + r * p.ld * (DT == NANOVLLM_GEMM_F32 ? 4 : 2);
-    const float t = p.temperatures[r];
+    const float t = p.temperatures[r], u = p.uniforms[r];
+    const int32_t k = p.top_k != nullptr ? p.top_k[r] : 0;
+    const float top_p = p.top_p != nullptr ? p.top_p[r] : 1.0f;
+    const float min_p = p.min_p != nullptr ? p.min_p[r] : 0.0f;
+    const int64_t record = record_bytes(p.step, p.slices);
+    const char* records = p.work + r * p.slices * record;
+    auto record_of = [&](int s) { return reinterpret_cast<const Record*>(records + s * record); };
 
-    uint64_t best = 0;
-    each_logit<DT>(row, vocab, [&](int i, float l) {
-        const uint64_t place = place_of(argmax_order(l), i);
-        best = place > best ? place : best;
-    });
-    best = max_all(best, sh);
+    Slice<DT, STEP == 0 ? kTile : STEP> slice;
+    uint64_t best = 0, its_best = 0;   // of the row, and of slice `tid`
+    int its_last = 0, its_listed = 0;
+    uint64_t place[2] = {0, 0};        // two of the row's listed members, by index
+    if constexpr (STEP > 0) {
+        u32x4_t v[Slice<DT, STEP>::R];
+        Slice<DT, STEP>::request(row, 0, vocab, v);
+        slice.kept = reinterpret_cast<char*>(kept_logits);
+        slice.begin = 0;
+        slice.n = vocab;
+        slice.take(row, v, sh);
+        best = slice.best;
+    } else {
+        if (tid < p.slices) {
+            const Record* rec = record_of(tid);
+            its_best = rec->best;
+            its_last = rec->last;
+            its_listed = rec->listed;
+        }
+        const int cap = list_room(p.step, p.slices), s = 2 * tid / cap, i = 2 * tid - s * cap;
+        if (s < p.slices) __builtin_memcpy(place, reinterpret_cast<const uint64_t*>(record_of(s) + 1) + i, 16);
+        best = max_all(its_best, sh);
+    }
     const uint32_t best_key = uint32_t(best >> 32);
-    const int best_index = int(0xFFFFFFFFu - uint32_t(best));
-    if (!(t > 1e-10f) || best_key == kNanKey) {
-        if (threadIdx.x == 0) {
-            p.tokens[r] = best_index;
+    if (!draws(t, best)) {
+        if (tid == 0) {
+            p.tokens[r] = int(0xFFFFFFFFu - uint32_t(best));
             p.logprobs[r] = best_key == kNanKey ? __builtin_nanf("") : 0.0f;
         }
         return;
     }
     const Scale sc = scale_of(logit_of(best_key), t);
+    if (tid == 0) sh.scale = sc;   // read behind the barriers of what follows
 
-    sh.count[threadIdx.x] = 0;
-    sh.units[threadIdx.x] = 0;
-    __syncthreads();
-    each_logit<DT>(row, vocab, [&](int, float l) {
-        const Weight w = weigh(l, sc);
-        atomicAdd(&sh.count[w.bin], 1u);
-        if (w.bin < kRest)
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.units[w.bin]),
-                      static_cast<unsigned long long>(units_of(w.part)));
-    });
-    __syncthreads();
-    {
-        const uint32_t counts = scan(sh.count[threadIdx.x], sh);
-        const double masses = scan(double(sh.units[threadIdx.x]) * 0x1p-40 * bin_scale(threadIdx.x), sh);
-        sh.count[threadIdx.x] = counts;
-        sh.mass[threadIdx.x] = masses;
+    // The row's histogram, and the last bin whose members are all listed.
+    int covered = kRest;
+    uint32_t count = 0;
+    uint64_t units = 0;
+    if (sc.flat) {
+        // The holders of an infinity share the row.
+        each_logit<DT>(row, vocab, [&](int, float l) { count += l == sc.largest; });
+        count = given_by(kThreads - 1, scan(count, sh), sh.part32);
+        count = tid == 0 ? count : 0;
+        units = uint64_t(count) << 36;
+        covered = -1;
+    } else if constexpr (STEP > 0) {
+        slice.sc = sc;
+        slice.bins(sh);
+        count = count_of(sh.words[tid]);
+        units = sum_of(sh.words[tid]);
+    } else {
+        int mine = kRest;
+        if (tid < p.slices) {
+            const float largest = logit_of(uint32_t(its_best >> 32));
+            const double down = sc.top - top_of(largest, sc);
+            const bool some = __builtin_fabsf(largest) < __builtin_inff() && down < double(kRest);
+            sh.shift[tid] = some ? int(down) : kRest;
+            sh.listed[tid] = some ? its_listed : 0;
+            if (some && int(down) + its_last < mine) mine = int(down) + its_last;
+        }
+        // The least of them, as the largest of what they are below kRest.
+        covered = kRest - int(max_all(uint32_t(kRest - mine), sh));
+        constexpr int kBatch = 16;   // loads in flight
+        for (int first = 0; first < p.slices; first += kBatch) {
+            uint64_t word[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int s = first + e, b = s < p.slices ? tid - sh.shift[s] : -1;
+                word[e] = b >= 0 && tid < kRest ? record_of(s)->words[b] : 0;
+            }
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                count += count_of(word[e]);
+                units += sum_of(word[e]);
+            }
+        }
     }
+    sh.count[tid] = scan(count, sh);
+    sh.mass[tid] = scan(double(units) * kUnit * bin_scale(tid), sh);
     __syncthreads();
     auto members = [&](int b) { return b ? sh.count[b] - sh.count[b - 1] : sh.count[0]; };
     auto mass_before = [&](int b) { return b ? sh.mass[b - 1] : 0.0; };
 
-    uint64_t border = 0;   // places from here on are kept
-    double total = sh.mass[kRest];
-    const int32_t k = p.top_k != nullptr ? p.top_k[r] : 0;
-    if (k > 0 && k < vocab) {
-        const int b = first_of(sh.count[threadIdx.x] >= uint32_t(k), threadIdx.x, kRest, sh);
-        if (b < kRest) {
-            const Border at = border_in<DT>(row, vocab, sc, b, members(b), false,
-                                            uint32_t(k) - (b ? sh.count[b - 1] : 0u), 0.0, sh);
-            border = at.place;
-            total = mass_before(b) + at.mass * bin_scale(b);
+    // The least logit whose weight is min_p or more, as a key.
+    uint32_t least = 0;
+    int least_bin = kRest;   // no member of a lower one has that weight
+    if (min_p > 0.0f) {
+        const double l = min_p >= 1.0f ? double(sc.largest) : double(sc.largest) + double(t) * log_once(double(min_p));
+        const float near = float(l);
+        least = argmax_order(near) + (double(near) < l ? 1u : 0u);
+        if (min_p > 1.0f || least > best_key) least = best_key;
+        least_bin = sc.flat ? 0 : weigh_once(logit_of(least), sc).bin;
+    }
+    const int k_bin = k > 0 && k < vocab ? first_of(sh.count[tid] >= uint32_t(k), tid, kRest, sh) : kRest;
+    const double whole = sh.mass[kRest];
+    const double share = u > 0.0f ? double(u) : 0.0;
+
+    // Where everything up to the border is listed, and not too many, the listed
+    // members decide.  With a top-k in front of the top-p its whole bin is needed.
+    int last = k_bin;
+    if (top_p < 1.0f && k_bin == kRest) last = first_of(sh.mass[tid] >= double(top_p) * whole, tid, kRest - 1, sh);
+    const int p_bin = last;   // of the top-p where there is no top-k
+    if (!(top_p < 1.0f && k_bin < kRest)) last = least_bin < last ? least_bin : last;
+    if (last >= kRest) last = kRest - 1;
+    bool few = covered >= last && sh.count[last] <= uint32_t(kFew);
+    if constexpr (STEP > 0) {
+        if (few) {
+            const uint32_t n = slice.list(least_of(last, sc), sh, [&](uint32_t at, int i, uint32_t key) {
+                if (at < uint32_t(kFew)) sh.few[at] = place_of(key, i);
+            });
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) place[e] = 2 * uint32_t(tid) + e < n ? sh.few[2 * tid + e] : 0;
+            few = n <= uint32_t(kFew);
+        }
+    } else {
+        const int cap = list_room(p.step, p.slices), s = 2 * tid / cap, i = 2 * tid - s * cap;
+        const int there = s < p.slices ? sh.listed[s] - i : 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) place[e] = e < there ? place[e] : 0;
+    }
+    if (few) {
+        Weight mine[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mine[e] = Weight{kRest, 0};
+            if (place[e] != 0) mine[e] = weigh_once(logit_of(uint32_t(place[e] >> 32)), sc);
+        }
+        uint64_t border = uint64_t(least) << 32;
+        double total = whole;
+#pragma unroll 1
+        for (int mode = kByCount; mode <= kByMass; ++mode) {
+            int b = k_bin;
+            double want = 0.0;
+            if (mode == kByCount) {
+                if (k_bin > last) continue;
+            } else {
+                if (!(top_p < 1.0f)) continue;
+                want = double(top_p) * total;
+                b = first_of(sh.mass[tid] >= want, tid, kRest - 1, sh);
+                if (b > last) continue;
+            }
+            const int n = int(members(b));
+            if (n > kList) {   // uniform: more than are put in order at once
+                few = false;
+                break;
+            }
+            __syncthreads();
+            if (tid == 0) sh.fill = 0;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (mine[e].bin == b) sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place[e];
+            border_of_list(n, mode, mode == kByMass ? 0u : uint32_t(k) - (b ? sh.count[b - 1] : 0u),
+                           (want - mass_before(b)) / bin_scale(b), 0.0, true, sh);
+            const Border at = sh.border;
+            if (mode == kByCount) total = mass_before(b) + at.mass * bin_scale(b);
+            border = at.place > border ? at.place : border;
+        }
+        border = border > best || min_p > 1.0f ? best : border;
+        double w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            w[e] = place[e] >= border && mine[e].bin <= last ? part_of(mine[e].off) * bin_scale(mine[e].bin) : 0.0;
+        if (few) {
+            const double sum = scan(w[0] + w[1], sh);
+            total = given_by(kThreads - 1, sum, sh.partd);
+            const double target = share * total;
+            const int one = w[0] > 0.0 && sum - w[1] > target ? 0 : w[1] > 0.0 && sum > target ? 1 : -1;
+            int at = first_of(one >= 0, 2 * tid + one, -1, sh);
+            if (at < 0) at = last_of(w[0] + w[1] > 0.0, 2 * tid + (w[1] > 0.0), 0, sh);
+            if (tid == at >> 1) {
+                p.tokens[r] = int64_t(0xFFFFFFFFu - uint32_t(place[at & 1]));
+                p.logprobs[r] = static_cast<float>(log_once(w[at & 1] / total));
+            }
+            return;
         }
     }
-    const float top_p = p.top_p != nullptr ? p.top_p[r] : 1.0f;
-    if (top_p < 1.0f) {
-        const double want = double(top_p) * total;
-        const int b = first_of(sh.mass[threadIdx.x] >= want, threadIdx.x, kRest - 1, sh);
-        const Border at = border_in<DT>(row, vocab, sc, b, members(b), true, 0u,
-                                        (want - mass_before(b)) / bin_scale(b), sh);
-        border = at.place > border ? at.place : border;
+
+    // The borders one after the other, from the bins' members in the row: the
+    // top-k's, the top-p's of what that keeps, the min-p's.
+    uint64_t border = 0;   // places from here on are kept
+    double total = whole;
+    bool listed = true;    // sh.list holds the members of the border's bin
+    int border_bin = kRest;
+#pragma unroll 1
+    for (int mode = kByCount; mode <= kByKey; ++mode) {
+        int b = k_bin;
+        double want = 0.0;
+        uint32_t need = 0;
+        if (mode == kByCount) {
+            // Without a top-p behind it a lower border than the min-p's is none.
+            if (k_bin == kRest || (!(top_p < 1.0f) && least_bin < k_bin)) continue;
+            need = uint32_t(k) - (b ? sh.count[b - 1] : 0u);
+        } else if (mode == kByMass) {
+            if (!(top_p < 1.0f) || (k_bin == kRest && least_bin < p_bin)) continue;
+            want = double(top_p) * total;
+            b = first_of(sh.mass[tid] >= want, tid, kRest - 1, sh);
+            if (b > border_bin) continue;   // rounding alone: the top-k's border stands
+        } else {
+            if (!(min_p > 0.0f) || least_bin > border_bin || least_bin == kRest) continue;
+            b = least_bin;
+            need = least;
+        }
+        border_in<DT>(row, vocab, sc, b, members(b), mode, need, (want - mass_before(b)) / bin_scale(b), sh);
+        const Border at = sh.border;
+        // The list is of bin b now, where the border lies already or comes to lie.
+        listed = at.listed;
+        if (at.place > border) {
+            border = at.place;
+            border_bin = b;
+            if (mode == kByCount) total = mass_before(b) + at.mass * bin_scale(b);
+        }
     }
-    const float min_p = p.min_p != nullptr ? p.min_p[r] : 0.0f;
-    if (min_p > 0.0f) {
-        // The least logit whose weight is min_p or more.
-        const double least = min_p >= 1.0f ? double(sc.largest) : double(sc.largest) + double(t) * log(double(min_p));
-        const float near = float(least);
-        const uint64_t at = uint64_t(argmax_order(near) + (double(near) < least ? 1u : 0u)) << 32;
-        border = at > border ? at : border;
-        if (min_p > 1.0f) border = best;
+    if (border > best || min_p > 1.0f) {
+        border = best;
+        border_bin = 0;
+        listed = false;
     }
-    border = border < best ? border : best;
 
     auto kept = [&](int i, float l) {
         const uint32_t key = argmax_order(l);
         if (place_of(key, i) < border) return 0.0;
         const Weight w = weigh(l, sc);
-        return w.bin < kRest ? w.part * bin_scale(w.bin) : 0.0;
+        return w.bin < kRest ? part_of(w.off) * bin_scale(w.bin) : 0.0;
     };
-    // Kept weight tile by tile, then the tile in which the running sum passes
-    // u times the total, then the token.
-    __syncthreads();
-    sh.tile[threadIdx.x] = 0.0;
-    for (int base = 0; base < vocab; base += kTile) {
-        const int i = base + int(threadIdx.x) * kPer;
-        double mine = 0.0;
-        if (i < vocab) {
-            float l[kPer];
-            load_logits<DT>(row, i, vocab, l);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (i + e < vocab) mine += kept(i + e, l[e]);
+    // Kept weight slice by slice, from the histograms and the members of the
+    // border's bin; then the slice, and in it the tile, in which the running sum
+    // passes u times the total.
+    int from = 0, to = vocab;
+    double ahead = 0.0;
+    const bool by_slice = STEP == 0 && !sc.flat;
+    if (by_slice) {
+        __syncthreads();
+        if (tid < p.slices) sh.slice[tid] = 0;
+        __syncthreads();
+        auto add = [&](int i, Weight w) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.slice[i / p.step]),
+                      static_cast<unsigned long long>(units_of(w.off)));
+        };
+        if (border_bin < kRest && listed) {
+            for (int i = tid; i < int(members(border_bin)); i += kThreads) {
+                const uint64_t at = sh.list[i];
+                if (at >= border) add(int(0xFFFFFFFFu - uint32_t(at)), weigh_once(logit_of(uint32_t(at >> 32)), sc));
+            }
+        } else if (border_bin < kRest) {
+            const uint32_t most = key_ceiling(border_bin, sc);
+            each_logit<DT>(row, vocab, [&](int i, float l) {
+                const uint32_t key = argmax_order(l);
+                if (key > most || place_of(key, i) < border) return;
+                const Weight w = weigh_once(l, sc);
+                if (w.bin == border_bin) add(i, w);
+            });
         }
-        const double all = sum_all(mine, sh);
-        if (threadIdx.x == 0) sh.tile[base / kTile] = all;
+        __syncthreads();
+        const int wave = tid >> 6, lane = tid & 63;
+        for (int s = wave; s < p.slices; s += kThreads / 64) {
+            const uint64_t* words = record_of(s)->words;
+            double sum = 0.0;
+#pragma unroll 4
+            for (int b = lane; b < kRest; b += 64)   // the whole bins that are kept
+                if (b + sh.shift[s] < border_bin)
+                    sum += double(sum_of(words[b])) * kUnit * bin_scale(b + sh.shift[s]);
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+            if (border_bin < kRest) sum += double(sh.slice[s]) * kUnit * bin_scale(border_bin);
+            if (lane == 0) sh.mass[s] = sum;
+        }
+        __syncthreads();
+        const double here = tid < p.slices ? sh.mass[tid] : 0.0;
+        const double upto = scan(here, sh);
+        total = given_by(kThreads - 1, upto, sh.partd);
+        int s = first_of(here > 0.0 && upto > share * total, tid, kBins, sh);
+        if (s == kBins) s = last_of(here > 0.0, tid, 0, sh);
+        ahead = given_by(s, upto - here, sh.partd);
+        from = s * p.step;
+        to = from + p.step < vocab ? from + p.step : vocab;
     }
     __syncthreads();
-    const double here = sh.tile[threadIdx.x];
+    sh.tile[tid] = 0.0;
+    for (int base = from; base < to; base += kTile) {
+        const int i = base + tid * kPer;
+        double mine = 0.0;
+        if (i < to) {
+            float l[kPer];
+            load_logits<DT, kPer>(row, i, to, l);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (i + e < to) mine += kept(i + e, l[e]);
+        }
+        const double all = scan(mine, sh);
+        if (tid == kThreads - 1) sh.tile[(base - from) / kTile] = all;
+    }
+    __syncthreads();
+    const double here = sh.tile[tid];
     const double upto = scan(here, sh);
-    __syncthreads();
-    if (threadIdx.x == kThreads - 1) sh.partd[0] = upto;
-    __syncthreads();
-    total = sh.partd[0];
-    const float u = p.uniforms[r];
-    const double target = u > 0.0f ? double(u) * total : 0.0;
-    int tile = first_of(here > 0.0 && upto > target, threadIdx.x, kBins, sh);
-    if (tile == kBins) tile = last_of(here > 0.0, threadIdx.x, 0, sh);
-    __syncthreads();
-    if (int(threadIdx.x) == tile) sh.partd[0] = upto - here;
-    __syncthreads();
-    const double before = sh.partd[0];
-    const int i = tile * kTile + int(threadIdx.x) * kPer;
+    if (!by_slice) total = given_by(kThreads - 1, upto, sh.partd);
+    const double target = share * total - ahead;
+    int tile = first_of(here > 0.0 && upto > target, tid, kBins, sh);
+    if (tile == kBins) tile = last_of(here > 0.0, tid, 0, sh);
+    const double lead = given_by(tile, upto - here, sh.partd);
+    const int i = from + tile * kTile + tid * kPer;
     double w[kPer], mine = 0.0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) w[e] = 0.0;
-    if (i < vocab) {
+    if (i < to) {
         float l[kPer];
-        load_logits<DT>(row, i, vocab, l);
+        load_logits<DT, kPer>(row, i, to, l);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) w[e] = i + e < vocab ? kept(i + e, l[e]) : 0.0;
+        for (int e = 0; e < kPer; ++e) w[e] = i + e < to ? kept(i + e, l[e]) : 0.0;
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) mine += w[e];
-    double run = before + (scan(mine, sh) - mine);
-    int found = INT32_MAX, last = -1;
+    double run = lead + (scan(mine, sh) - mine);
+    int found = INT32_MAX, final = -1;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         run += w[e];
         if (w[e] > 0.0) {
             if (found == INT32_MAX && run > target) found = i + e;
-            last = i + e;
+            final = i + e;
         }
     }
     int token = first_of(found != INT32_MAX, found, INT32_MAX, sh);
-    if (token == INT32_MAX) token = last_of(last >= 0, last, 0, sh);
+    if (token == INT32_MAX) token = last_of(final >= 0, final, 0, sh);
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-        if (i + e == token) {
+        if (i + e == token && i + e < to) {
             p.tokens[r] = token;
-            p.logprobs[r] = static_cast<float>(log(w[e] / total));
+            p.logprobs[r] = static_cast<float>(log_once(w[e] / total));
         }
+}
+
+// Logits of a slice: the whole row (0) where 64 KiB of LDS hold it; otherwise 8192
+// while that makes no more than two rounds of workgroups, then 16384, and 32768,
+// the most that a histogram counts, where a row has more slices than are joined.
+int slice_step(int64_t m, int64_t vocab, int dtype) {
+    constexpr int64_t kCus = 256;
+    if (vocab <= (dtype == NANOVLLM_GEMM_F32 ? 2 * kTile : 4 * kTile)) return 0;
+    const int64_t tiles = (vocab + kTile - 1) / kTile;
+    if (tiles <= kMostSlices && m * tiles <= 4 * kCus) return kTile;
+    return (tiles + 1) / 2 <= kMostSlices ? 2 * kTile : kMostSlice;
+}
+
+template <int DT>
+int launch_typed(RowArgs a, int64_t m, hipStream_t s) {
+    constexpr int B = DT == NANOVLLM_GEMM_F32 ? 4 : 2, kMost = B == 4 ? 2 * kTile : 4 * kTile;
+    const dim3 rows(static_cast<uint32_t>(m)), block(kThreads);
+    a.step = slice_step(m, a.vocab, DT);
+    if (a.step == 0) {
+        hipLaunchKernelGGL((sample_row_kernel<DT, kMost>), rows, block, 0, s, a);
+        return check_launch("sample_logits");
+    }
+    a.slices = (a.vocab + a.step - 1) / a.step;
+    // Two workgroups to a CU, one of the largest slices.
+    const int64_t total = m * a.slices, room = a.step > 2 * kTile ? 256 : 512;
+    const dim3 grid(static_cast<uint32_t>(total < room ? total : room));
+    if (a.step == kTile) hipLaunchKernelGGL((sample_slices_kernel<DT, kTile>), grid, block, 0, s, a, m);
+    else if (a.step == 2 * kTile) hipLaunchKernelGGL((sample_slices_kernel<DT, 2 * kTile>), grid, block, 0, s, a, m);
+    else hipLaunchKernelGGL((sample_slices_kernel<DT, 4 * kTile>), grid, block, 0, s, a, m);
+    const int rc = check_launch("sample_logits");
+    if (rc != NANOVLLM_GEMM_OK) return rc;
+    hipLaunchKernelGGL((sample_row_kernel<DT, 0>), rows, block, 0, s, a);
+    return check_launch("sample_logits");
 }
 
 }  // namespace
 
-int64_t sample_logits_workspace(int64_t, int64_t, int) { return 0; }
+int64_t sample_logits_workspace(int64_t m, int64_t vocab, int dtype) {
+    const int step = slice_step(m, vocab, dtype);
+    if (step == 0) return 0;
+    const int64_t slices = (vocab + step - 1) / step;
+    return m * slices * record_bytes(step, static_cast<int>(slices));
+}
 
 int launch_sample_logits(const SampleLogitsArgs& p, hipStream_t s) {
     const RowArgs a{static_cast<const char*>(p.logits), p.temperatures, p.uniforms, p.top_k, p.top_p, p.min_p, p.tokens,
-                    p.logprobs, p.ld, static_cast<int32_t>(p.vocab)};
-    const dim3 grid(static_cast<uint32_t>(p.m)), block(kThreads);
-    if (p.dtype == NANOVLLM_GEMM_F32) hipLaunchKernelGGL(sample_row_kernel<NANOVLLM_GEMM_F32>, grid, block, 0, s, a);
-    else if (p.dtype == NANOVLLM_GEMM_F16) hipLaunchKernelGGL(sample_row_kernel<NANOVLLM_GEMM_F16>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(sample_row_kernel<NANOVLLM_GEMM_BF16>, grid, block, 0, s, a);
-    return check_launch("sample_logits");
+                    p.logprobs, p.ld, static_cast<int32_t>(p.vocab), p.workspace, 0, 0};
+    if (p.dtype == NANOVLLM_GEMM_F32) return launch_typed<NANOVLLM_GEMM_F32>(a, p.m, s);
+    if (p.dtype == NANOVLLM_GEMM_F16) return launch_typed<NANOVLLM_GEMM_F16>(a, p.m, s);
+    return launch_typed<NANOVLLM_GEMM_BF16>(a, p.m, s);
 }
 
 }  // namespace nvg
