@@ -243,7 +243,6 @@ struct Shared {
         struct { uint64_t list[kList], units[kList], front[kList]; uint32_t rank[kList]; };
         uint64_t few[kFew];    // listed members of a row of one slice, by index
         struct { uint32_t count[kBins]; uint64_t units[kBins]; } sub;
-        double tile[kBins];    // kept weight of the row's tiles
     };
     uint64_t part64[kThreads / 64];
     double partd[kThreads / 64];
@@ -383,23 +382,41 @@ __device__ __forceinline__ T given_by(int from, T v, T* part) {
     return part[0];
 }
 
-// Calls f(index, logit) for every logit of the row.
+// Calls f(index, logit) for the logits of the row from `low` to `high`.  Few are
+// expected: they are marked first, at four instructions a logit.
 template <int DT, typename F>
-__device__ __forceinline__ void each_logit(const char* row, int vocab, F f) {
+__device__ __forceinline__ void each_between(const char* row, int vocab, float low, float high, F f) {
     constexpr int kAhead = 2;   // loads in flight
     for (int base = threadIdx.x * kPer; base < vocab; base += kAhead * kTile) {
         float l[kAhead][kPer];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-            if (base + a * kTile < vocab) load_logits<DT, kPer>(row, base + a * kTile, vocab, l[a]);
-#pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            const int i = base + a * kTile;
+            if (a == 0 || base + a * kTile < vocab) {
+                load_logits<DT, kPer>(row, base + a * kTile, vocab, l[a]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (i + e < vocab) f(i + e, l[a][e]);
+                for (int e = 0; e < kPer; ++e) l[a][e] = __builtin_nanf("");
+            }
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) hits |= l[a][e] >= low && l[a][e] <= high ? 1u << (a * kPer + e) : 0u;
+#pragma unroll 1
+        for (; hits; hits &= hits - 1) {
+            const int at = __builtin_ctz(hits);
+            float v = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kAhead * kPer; ++e) v = at == e ? l[e / kPer][e % kPer] : v;
+            f(base + at / kPer * kTile + at % kPer, v);
         }
     }
+}
+
+// A key's logit as a bound; keys below that of -inf are of no logit.
+__device__ __forceinline__ float bound_of(uint32_t key) {
+    return key > 0x007FFFFFu ? logit_of(key) : -__builtin_inff();
 }
 
 // ---------------------------------------------------------------------------
@@ -460,7 +477,7 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
     const bool by_mass = mode == kByMass;
     // Keys of the members still in question, lo .. hi; need and want go down by
     // what lies above them.
-    uint32_t lo = key_floor(bin, sc), hi = key_ceiling(bin, sc);
+    uint32_t hi = key_ceiling(bin, sc), lo = sc.flat ? hi : key_floor(bin, sc);
     double above = 0.0;
     const bool whole = members <= uint32_t(kList);
     auto inside = [&](float l, uint32_t key) { return key >= lo && key <= hi && weigh(l, sc).bin == bin; };
@@ -476,7 +493,7 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
         sh.sub.count[threadIdx.x] = 0;
         sh.sub.units[threadIdx.x] = 0;
         __syncthreads();
-        each_logit<DT>(row, vocab, [&](int, float l) {
+        each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int, float l) {
             const uint32_t key = argmax_order(l);
             if (!inside(l, key)) return;
             const uint32_t b = (hi - key) / width;
@@ -546,7 +563,7 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
     __syncthreads();
     if (threadIdx.x == 0) sh.fill = 0;
     __syncthreads();
-    each_logit<DT>(row, vocab, [&](int i, float l) {
+    each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int i, float l) {
         const uint32_t key = argmax_order(l);
         if (inside(l, key)) sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place_of(key, i);
     });
@@ -758,10 +775,7 @@ __device__ __forceinline__ bool draws(float t, uint64_t best) {
 }
 
 // The least logit that may be in bin `last` or above.
-__device__ __forceinline__ float least_of(int last, const Scale& s) {
-    const uint32_t floor = key_floor(last, s);
-    return floor > 0 ? logit_of(floor) : -__builtin_inff();
-}
+__device__ __forceinline__ float least_of(int last, const Scale& s) { return bound_of(key_floor(last, s)); }
 
 // Workgroups take slice after slice, the logits of the next one on their way
 // while this one is binned.
@@ -874,7 +888,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     uint64_t units = 0;
     if (sc.flat) {
         // The holders of an infinity share the row.
-        each_logit<DT>(row, vocab, [&](int, float l) { count += l == sc.largest; });
+        each_between<DT>(row, vocab, sc.largest, sc.largest, [&](int, float) { ++count; });
         count = given_by(kThreads - 1, scan(count, sh), sh.part32);
         count = tid == 0 ? count : 0;
         units = uint64_t(count) << 36;
@@ -1080,10 +1094,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
                 if (at >= border) add(int(0xFFFFFFFFu - uint32_t(at)), weigh_once(logit_of(uint32_t(at >> 32)), sc));
             }
         } else if (border_bin < kRest) {
-            const uint32_t most = key_ceiling(border_bin, sc);
-            each_logit<DT>(row, vocab, [&](int i, float l) {
-                const uint32_t key = argmax_order(l);
-                if (key > most || place_of(key, i) < border) return;
+            const uint32_t least_key = uint32_t(border >> 32);
+            each_between<DT>(row, vocab, bound_of(least_key), bound_of(key_ceiling(border_bin, sc)), [&](int i, float l) {
+                if (place_of(argmax_order(l), i) < border) return;
                 const Weight w = weigh_once(l, sc);
                 if (w.bin == border_bin) add(i, w);
             });
@@ -1091,12 +1104,22 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         __syncthreads();
         const int wave = tid >> 6, lane = tid & 63;
         for (int s = wave; s < p.slices; s += kThreads / 64) {
-            const uint64_t* words = record_of(s)->words;
+            const Record* rec = record_of(s);
+            const int shift = sh.shift[s];
+            uint64_t words[kBins / 64];
+#pragma unroll
+            for (int e = 0; e < kBins / 64; ++e) {   // the whole bins that are kept
+                const int b = e * 64 + lane;
+                words[e] = b < kRest && b + shift < border_bin ? rec->words[b] : 0;
+            }
             double sum = 0.0;
-#pragma unroll 4
-            for (int b = lane; b < kRest; b += 64)   // the whole bins that are kept
-                if (b + sh.shift[s] < border_bin)
-                    sum += double(sum_of(words[b])) * kUnit * bin_scale(b + sh.shift[s]);
+#pragma unroll 1
+            for (int e = 0; e < kBins / 64; ++e) {
+                const uint64_t word = words[0];
+                if (word != 0) sum += double(sum_of(word)) * kUnit * bin_scale(e * 64 + lane + shift);
+#pragma unroll
+                for (int n = 1; n < kBins / 64; ++n) words[n - 1] = words[n];
+            }
 #pragma unroll
             for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
             if (border_bin < kRest) sum += double(sh.slice[s]) * kUnit * bin_scale(border_bin);
@@ -1112,59 +1135,40 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         from = s * p.step;
         to = from + p.step < vocab ? from + p.step : vocab;
     }
-    __syncthreads();
-    sh.tile[tid] = 0.0;
-    for (int base = from; base < to; base += kTile) {
-        const int i = base + tid * kPer;
-        double mine = 0.0;
-        if (i < to) {
-            float l[kPer];
-            load_logits<DT, kPer>(row, i, to, l);
+    // A run of logits a thread.
+    const int run = ((to - from + kThreads - 1) / kThreads + kPer - 1) / kPer * kPer;
+    const int begin = from + tid * run < to ? from + tid * run : to, end = to - begin < run ? to : begin + run;
+    double mine = 0.0;
+#pragma unroll 1
+    for (int i = begin; i < end; i += kPer) {
+        float l[kPer];
+        load_logits<DT, kPer>(row, i, end, l);
+#pragma unroll 1
+        for (int e = 0; e < kPer && i + e < end; ++e) {
+            mine += kept(i + e, l[0]);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (i + e < to) mine += kept(i + e, l[e]);
+            for (int n = 1; n < kPer; ++n) l[n - 1] = l[n];
         }
-        const double all = scan(mine, sh);
-        if (tid == kThreads - 1) sh.tile[(base - from) / kTile] = all;
     }
-    __syncthreads();
-    const double here = sh.tile[tid];
-    const double upto = scan(here, sh);
+    const double upto = scan(mine, sh);
     if (!by_slice) total = given_by(kThreads - 1, upto, sh.partd);
     const double target = share * total - ahead;
-    int tile = first_of(here > 0.0 && upto > target, tid, kBins, sh);
-    if (tile == kBins) tile = last_of(here > 0.0, tid, 0, sh);
-    const double lead = given_by(tile, upto - here, sh.partd);
-    const int i = from + tile * kTile + tid * kPer;
-    double w[kPer], mine = 0.0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) w[e] = 0.0;
-    if (i < to) {
-        float l[kPer];
-        load_logits<DT, kPer>(row, i, to, l);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) w[e] = i + e < to ? kept(i + e, l[e]) : 0.0;
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) mine += w[e];
-    double run = lead + (scan(mine, sh) - mine);
-    int found = INT32_MAX, final = -1;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        run += w[e];
-        if (w[e] > 0.0) {
-            if (found == INT32_MAX && run > target) found = i + e;
-            final = i + e;
+    int at = first_of(mine > 0.0 && upto > target, tid, kThreads, sh);
+    if (at == kThreads) at = last_of(mine > 0.0, tid, 0, sh);
+    if (tid != at) return;
+    double sum = upto - mine, its = 0.0;
+    int token = begin;
+#pragma unroll 1
+    for (int i = begin; i < end && !(its > 0.0 && sum > target); ++i) {
+        const double w = kept(i, logit_at<DT>(row, i));
+        sum += w;
+        if (w > 0.0) {
+            token = i;
+            its = w;
         }
     }
-    int token = first_of(found != INT32_MAX, found, INT32_MAX, sh);
-    if (token == INT32_MAX) token = last_of(final >= 0, final, 0, sh);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e)
-        if (i + e == token && i + e < to) {
-            p.tokens[r] = token;
-            p.logprobs[r] = static_cast<float>(log_once(w[e] / total));
-        }
+    p.tokens[r] = token;
+    p.logprobs[r] = static_cast<float>(log_once(its / total));
 }
 
 // Logits of a slice: the whole row (0) where 64 KiB of LDS hold it; otherwise 8192
