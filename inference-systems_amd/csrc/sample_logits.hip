@@ -32,6 +32,8 @@
 // largest weight down, which counts as 0.
 #include "int8_common.hpp"
 
+#include <type_traits>
+
 namespace nvg {
 namespace {
 
@@ -115,14 +117,16 @@ __device__ __forceinline__ Scale scale_of(float largest, float t) {
 // 2^(y / 16) - 1 in units of 2^-36: the linear term as a float and its remainder,
 // the others, to the 5th power, with the remainder (off by less than 2^-43).
 // A vector instruction in 64 bits takes as long as four in 32 here, and the
-// sum of both terms as integers takes the place of a wider type.
+// sum of both terms as integers takes the place of a wider type.  NEAR: all products
+// down to the last bin's are within kNear.
+template <bool NEAR = false>
 __device__ __forceinline__ Weight weigh_finite(float l, const Scale& s) {
 #pragma clang fp contract(off)
     constexpr double a = 0.69314718055994530942 / 16.0, unit = 0x1p36;
     constexpr float ah = float(a * unit), al = float(a * unit - double(float(a * unit)));
     const float hi = l * s.ch;
     float y, low, down;
-    if (__builtin_fabsf(hi) > kNear && !(hi < s.topf - 2048.0f)) {
+    if (!NEAR && __builtin_fabsf(hi) > kNear && !(hi < s.topf - 2048.0f)) {
         double rest;
         down = float(s.top - far_product(l, s, rest));
         y = float(rest);
@@ -181,6 +185,8 @@ __device__ __forceinline__ uint32_t key_ceiling(int first, const Scale& s) {
     const uint32_t key = argmax_order(float(l)) + 4;
     return key < most ? key : most;
 }
+
+__device__ __forceinline__ bool is_near(const Scale& s) { return __builtin_fabsf(s.topf) < kNear - 2.0f * kBins; }
 
 // 2^(-bin / 16), by the bits of bin.
 __device__ __forceinline__ double bin_scale(int bin) {
@@ -325,16 +331,21 @@ __device__ __attribute__((noinline)) T max_over(T v, T* part) {
     return from_lane(row_scan(part[lane & (kWaves - 1)], Max{}), kWaves - 1);
 }
 
-// Inclusive sums over the threads in order.
+// Inclusive sums over the threads in order, and the sum over all.
 template <typename T>
-__device__ __attribute__((noinline)) T scan_over(T v, T* part) {
+struct Sums {
+    T upto, all;
+    __device__ __forceinline__ operator T() const { return upto; }
+};
+template <typename T>
+__device__ __attribute__((noinline)) Sums<T> scan_over(T v, T* part) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     v = wave_scan(v, Add{});
     __syncthreads();
     if (lane == 63) part[wave] = v;
     __syncthreads();
     const T upto = row_scan(part[lane & (kWaves - 1)], Add{});
-    return wave > 0 ? from_lane(upto, wave - 1) + v : v;
+    return Sums<T>{wave > 0 ? from_lane(upto, wave - 1) + v : v, from_lane(upto, kWaves - 1)};
 }
 
 // The number of the first (or last) thread that says yes; `none` if none does.
@@ -360,11 +371,11 @@ template <typename S>
 __device__ __forceinline__ uint64_t max_all(uint64_t v, S& sh) { return max_over<uint64_t>(v, sh.part64); }
 template <typename S>
 __device__ __forceinline__ uint32_t max_all(uint32_t v, S& sh) { return max_over<uint32_t>(v, sh.part32); }
-__device__ __forceinline__ double scan(double v, Shared& sh) { return scan_over<double>(v, sh.partd); }
+__device__ __forceinline__ Sums<double> scan(double v, Shared& sh) { return scan_over<double>(v, sh.partd); }
 template <typename S>
-__device__ __forceinline__ uint32_t scan(uint32_t v, S& sh) { return scan_over<uint32_t>(v, sh.part32); }
+__device__ __forceinline__ Sums<uint32_t> scan(uint32_t v, S& sh) { return scan_over<uint32_t>(v, sh.part32); }
 template <typename S>
-__device__ __forceinline__ uint64_t scan(uint64_t v, S& sh) { return scan_over<uint64_t>(v, sh.part64); }
+__device__ __forceinline__ Sums<uint64_t> scan(uint64_t v, S& sh) { return scan_over<uint64_t>(v, sh.part64); }
 template <typename S>
 __device__ __forceinline__ int first_of(bool yes, int number, int none, S& sh) {
     return pick(yes, number, none, false, sh.part32, sh.some);
@@ -539,11 +550,8 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
             load_logits<DT, kPer>(row, i, vocab, l);
 #pragma unroll
             for (int e = 0; e < kPer; ++e) here += i + e < vocab && argmax_order(l[e]) == hi;
-            const uint32_t upto = scan(here, sh);
-            __syncthreads();
-            if (threadIdx.x == kThreads - 1) sh.part32[0] = upto;
-            __syncthreads();
-            const uint32_t all = sh.part32[0];
+            const Sums<uint32_t> sums = scan(here, sh);
+            const uint32_t upto = sums.upto, all = sums.all;
             if (seen + all >= c) {   // uniform
                 uint32_t k = seen + upto - here;
                 if (k < c && seen + upto >= c) {
@@ -701,35 +709,39 @@ struct Slice {
         else return logit_at<DT>(kept, i);
     }
 
+    template <bool NEAR, typename S>
+    __device__ __forceinline__ void bins_of(S& sh) {
+#pragma unroll 1
+        for (int i = int(threadIdx.x) * kPer; i < n; i += (i & 4) ? kTile - 4 : 4) {
+            float l[4];
+            if constexpr (B == 4) {
+                const u32x4_t v = chunk(i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[e] = element(v, e);
+            } else {
+                const u32x2_t v = *reinterpret_cast<const u32x2_t*>(kept + i * B);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[e] = half_to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
+            }
+            Weight w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = weigh_finite<NEAR>(l[e], sc);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (w[e].bin < kRest)
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.words[w[e].bin]),
+                              static_cast<unsigned long long>(packed(w[e].off)));
+        }
+    }
+
     // Its histogram in sh.words, four logits side by side.  A slice of infinities
     // leaves none.
     template <typename S>
     __device__ __forceinline__ void bins(S& sh) {
         sh.words[threadIdx.x] = 0;
         __syncthreads();
-        if (!sc.flat) {
-#pragma unroll 1
-            for (int i = int(threadIdx.x) * kPer; i < n; i += (i & 4) ? kTile - 4 : 4) {
-                float l[4];
-                if constexpr (B == 4) {
-                    const u32x4_t v = chunk(i);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) l[e] = element(v, e);
-                } else {
-                    const u32x2_t v = *reinterpret_cast<const u32x2_t*>(kept + i * B);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) l[e] = half_to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
-                }
-                Weight w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = weigh_finite(l[e], sc);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (w[e].bin < kRest)
-                        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.words[w[e].bin]),
-                                  static_cast<unsigned long long>(packed(w[e].off)));
-            }
-        }
+        if (is_near(sc) && !sc.flat) bins_of<true>(sh);
+        else if (!sc.flat) bins_of<false>(sh);
         __syncthreads();
     }
 
@@ -738,8 +750,9 @@ struct Slice {
     // one of its groups.
     template <typename S, typename F>
     __device__ __forceinline__ uint32_t list(float least, S& sh, F put) {
+        using Counts = std::conditional_t<(G > 2), uint64_t, uint32_t>;
         uint32_t hits = 0;   // bit 8 g + e: logit e of group g is listed
-        uint64_t mine = 0;
+        Counts mine = 0;
 #pragma unroll 1
         for (int g = 0; g < G; ++g) {
             if (first(g) >= n) break;
@@ -751,11 +764,10 @@ struct Slice {
                 for (int e = 0; e < E; ++e) here |= element(v, e) >= least ? 1u << (h * E + e) : 0u;
             }
             hits |= here << (kPer * g);
-            mine |= uint64_t(__builtin_popcount(here)) << (16 * g);
+            mine |= Counts(__builtin_popcount(here)) << (16 * g);
         }
-        const uint64_t upto = scan(mine, sh);
-        const uint64_t all = given_by(kThreads - 1, upto, sh.part64);
-        uint64_t at = upto - mine;   // by group, its groups' starts to come
+        const Sums<Counts> upto = scan(mine, sh);
+        const Counts at = upto.upto - mine;   // by group, its groups' starts to come
         uint32_t start = 0;
 #pragma unroll 1
         for (int g = 0; g < G; ++g) {
@@ -764,7 +776,7 @@ struct Slice {
                 const int i = first(g) + __builtin_ctz(here);
                 put(where++, begin + i, argmax_order(at_index(i)));
             }
-            start += uint32_t(all >> (16 * g) & 0xFFFFu);
+            start += uint32_t(upto.all >> (16 * g) & 0xFFFFu);
         }
         return start;
     }
@@ -889,7 +901,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     if (sc.flat) {
         // The holders of an infinity share the row.
         each_between<DT>(row, vocab, sc.largest, sc.largest, [&](int, float) { ++count; });
-        count = given_by(kThreads - 1, scan(count, sh), sh.part32);
+        count = scan(count, sh).all;
         count = tid == 0 ? count : 0;
         units = uint64_t(count) << 36;
         covered = -1;
@@ -1013,8 +1025,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         for (int e = 0; e < 2; ++e)
             w[e] = place[e] >= border && mine[e].bin <= last ? part_of(mine[e].off) * bin_scale(mine[e].bin) : 0.0;
         if (few) {
-            const double sum = scan(w[0] + w[1], sh);
-            total = given_by(kThreads - 1, sum, sh.partd);
+            const Sums<double> sums = scan(w[0] + w[1], sh);
+            const double sum = sums.upto;
+            total = sums.all;
             const double target = share * total;
             const int one = w[0] > 0.0 && sum - w[1] > target ? 0 : w[1] > 0.0 && sum > target ? 1 : -1;
             int at = first_of(one >= 0, 2 * tid + one, -1, sh);
@@ -1127,8 +1140,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         }
         __syncthreads();
         const double here = tid < p.slices ? sh.mass[tid] : 0.0;
-        const double upto = scan(here, sh);
-        total = given_by(kThreads - 1, upto, sh.partd);
+        const Sums<double> sums = scan(here, sh);
+        const double upto = sums.upto;
+        total = sums.all;
         int s = first_of(here > 0.0 && upto > share * total, tid, kBins, sh);
         if (s == kBins) s = last_of(here > 0.0, tid, 0, sh);
         ahead = given_by(s, upto - here, sh.partd);
@@ -1150,8 +1164,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             for (int n = 1; n < kPer; ++n) l[n - 1] = l[n];
         }
     }
-    const double upto = scan(mine, sh);
-    if (!by_slice) total = given_by(kThreads - 1, upto, sh.partd);
+    const Sums<double> sums = scan(mine, sh);
+    const double upto = sums.upto;
+    if (!by_slice) total = sums.all;
     const double target = share * total - ahead;
     int at = first_of(mine > 0.0 && upto > target, tid, kThreads, sh);
     if (at == kThreads) at = last_of(mine > 0.0, tid, 0, sh);
