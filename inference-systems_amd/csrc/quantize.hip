@@ -3,9 +3,14 @@
 //
 // Both are bound by memory: a row is read once, held in registers across the
 // reduction of its maximum, and written once as codes.  A row belongs to 16, 64
-// or 256 threads, whichever holds it in at most 8 chunks of 8 elements a thread,
-// so short rows share a wave, middle ones need no barrier, and only rows beyond
-// 16384 elements are read twice.
+// or 256 threads: short rows share a wave, those up to 2048 elements need no
+// barrier, and only rows beyond 16384 are read twice.  Longer rows go to more
+// threads, not to more chunks a thread: 8192 x 3584 fp16 takes 16.8 us with two
+// chunks of 8 elements in each of 256 threads, 22.1 us with eight in a wave's.
+//
+// Measured: 8192 x 3584 fp16 16.8 us (88 MB, 5.3 TB/s), with four instructions for
+// a code where its remainder proves it (22.5 us with the proof and its mend for each
+// one); behind the norm 4100 x 1024 bf16 7.1 us (29 MB, 4.1 TB/s).
 //
 // The norm's row is z * c with z = s * (1 + w) and c = rsqrt(mean s^2 + eps)
 // common to the row, so its codes are those of z and its scale is that of z
@@ -38,12 +43,12 @@ __device__ __forceinline__ float row_scale_of(uint32_t top, Scale& q) {
     return s;
 }
 
-// Code of x in the low byte: rint(x / s), exact.  The product with the
-// reciprocal is off by less than 2^-15 of a code, so rint of it is off by one at
-// most, next to a half; the remainder x - q s, which fp32 holds, tells.  The
-// sum with 1.5 * 2^23 rounds to a whole number whose low bits are the code.
+// Code of x: rint(x / s), exact.  The product with the reciprocal is off by less
+// than 2^-15 of a code, so rint of it is off by one at most, next to a half; the
+// remainder x - q s, which fp32 holds, tells.  The sum with 1.5 * 2^23 rounds to a
+// whole number whose low bits are the code.
+constexpr float kMagic = 12582912.0f;
 __device__ __forceinline__ uint32_t code_of(float x, const Scale& sc) {
-    constexpr float kMagic = 12582912.0f;
     x *= sc.lift;
     const float y = x * sc.r + kMagic;
     const float q = y - kMagic;
@@ -53,6 +58,30 @@ __device__ __forceinline__ uint32_t code_of(float x, const Scale& sc) {
     if (far > h || (far == h && (c & 1))) c += e > 0.0f ? 1 : -1;
     // A denormal scale may be so coarse that a quotient passes 127.
     return static_cast<uint32_t>(c < -127 ? -127 : c > 127 ? 127 : c);
+}
+
+// The codes of 8 elements, a byte each.  Four instructions an element where every
+// remainder is below half a step (one in 2^15 is not), which proves the codes; a
+// row of zeros or of NaN has s == 0 and never is.
+__device__ __forceinline__ u32x2_t codes_of(const float (&x)[8], const Scale& sc) {
+    uint32_t c[8];
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = x[i] * sc.r + kMagic;
+        far = __builtin_fmaxf(far, __builtin_fabsf(__builtin_fmaf(kMagic - y, sc.s, x[i])));
+        c[i] = __builtin_bit_cast(uint32_t, y);
+    }
+    if (!(far < 0.5f * sc.s) || sc.lift != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = sc.s == 0.0f ? 0u : code_of(x[i], sc);
+    }
+    u32x2_t v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        v[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0C0C0400u), 0x05040100u);
+    return v;
 }
 
 // 8 elements at p as fp32; those at and past `left` are 0.
@@ -85,20 +114,14 @@ __device__ __forceinline__ void load8(const char* p, int left, float (&x)[8]) {
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
 
 __device__ __forceinline__ void store_codes(int8_t* p, int left, const float (&x)[8], const Scale& sc) {
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = sc.s == 0.0f ? 0u : code_of(x[i], sc);
+    const u32x2_t v = codes_of(x, sc);
     if (left >= 8) {
-        u32x2_t v;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            v[i] = (c[4 * i] & 255u) | (c[4 * i + 1] & 255u) << 8 | (c[4 * i + 2] & 255u) << 16 | c[4 * i + 3] << 24;
         __builtin_memcpy(p, &v, 8);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (i < left) p[i] = static_cast<int8_t>(c[i]);
+        if (i < left) p[i] = static_cast<int8_t>(v[i >> 2] >> (8 * (i & 3)));
 }
 
 // Maximum and sum over the TPR threads of a row (the sum in a fixed order).
