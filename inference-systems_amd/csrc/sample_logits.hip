@@ -238,7 +238,6 @@ constexpr int kFew = 2 * kThreads;    // listed members that decide: two a threa
 struct Border {
     uint64_t place;   // the last member in front of the cut
     double mass;      // weight up to and with it, in parts
-    bool listed;      // sh.list holds the bin's members
 };
 
 struct Shared {
@@ -247,9 +246,10 @@ struct Shared {
     double mass[kBins];        // weight of the bins up to one
     union {
         struct { uint64_t list[kList], units[kList], front[kList]; uint32_t rank[kList]; };
-        uint64_t few[kFew];    // listed members of a row of one slice, by index
         struct { uint32_t count[kBins]; uint64_t units[kBins]; } sub;
+        double scale_of[kBins];   // of the bins' weights
     };
+    uint64_t few[kFew];    // listed members of a row of one slice, by index; a bin's members
     uint64_t part64[kThreads / 64];
     double partd[kThreads / 64];
     uint32_t part32[kThreads / 64];
@@ -431,17 +431,16 @@ __device__ __forceinline__ float bound_of(uint32_t key) {
 }
 
 // ---------------------------------------------------------------------------
-// The border within a bin, in sh.border: its need-th member (kByCount), the
-// member at which the running weight, in parts, reaches `want` (kByMass), or the
-// key `need` itself (kByKey, for the list of the bin's members).
+// The border within a bin, in sh.border: its need-th member (kByCount), or the
+// member at which the running weight, in parts, reaches `want` (kByMass).
 // ---------------------------------------------------------------------------
-enum { kByCount, kByMass, kByKey };
+enum { kByCount, kByMass };
 
 // The border among the `members` places in sh.list, which are of one bin.  The
 // threads of a member, 1024 / members of them, count the places in front of it
 // and sum their weights (whole numbers, in any order).
 __device__ __attribute__((noinline)) void border_of_list(int members, int mode, uint32_t need, double want, double above,
-                                                         bool whole, Shared& sh) {
+                                                         Shared& sh) {
     int size = 64;
     while (size < members) size *= 2;
     const int i = threadIdx.x & (size - 1), part = threadIdx.x / size, parts = kThreads / size;
@@ -453,7 +452,6 @@ __device__ __attribute__((noinline)) void border_of_list(int members, int mode, 
         sh.front[i] = 0;
         sh.rank[i] = 0;
     }
-    if (threadIdx.x == 0) sh.border = Border{uint64_t(need) << 32, above, whole};   // where all lie behind the cut
     __syncthreads();
     uint32_t rank = 0;
     uint64_t front = 0;
@@ -473,11 +471,9 @@ __device__ __attribute__((noinline)) void border_of_list(int members, int mode, 
     if (part == 0 && i < members) {
         rank = sh.rank[i];
         const double before = double(sh.front[i]) * kUnit, upto = double(sh.front[i] + units) * kUnit;
-        bool cut;
-        if (mode == kByMass) cut = (upto >= want || rank + 1 == uint32_t(members)) && (before < want || rank == 0);
-        else if (mode == kByCount) cut = rank + 1 == need;
-        else cut = false;
-        if (cut) sh.border = Border{place, above + upto, whole};
+        const bool cut = mode == kByMass ? (upto >= want || rank + 1 == uint32_t(members)) && (before < want || rank == 0)
+                                         : rank + 1 == need;
+        if (cut) sh.border = Border{place, above + upto};
     }
     __syncthreads();
 }
@@ -490,27 +486,48 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
     // what lies above them.
     uint32_t hi = key_ceiling(bin, sc), lo = sc.flat ? hi : key_floor(bin, sc);
     double above = 0.0;
-    const bool whole = members <= uint32_t(kList);
     auto inside = [&](float l, uint32_t key) { return key >= lo && key <= hi && weigh(l, sc).bin == bin; };
-    if (members > uint32_t(kList) && mode == kByKey) {
+    // The row is read once where sh.few holds the bin's members.
+    const uint32_t all = members;
+    const bool whole = all <= uint32_t(kFew);
+    if (whole) {
         __syncthreads();
-        if (threadIdx.x == 0) sh.border = Border{uint64_t(need) << 32, 0.0, false};
+        if (threadIdx.x == 0) sh.fill = 0;
         __syncthreads();
-        return;
+        each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int i, float l) {
+            const uint32_t key = argmax_order(l);
+            if (inside(l, key)) sh.few[atomicAdd(&sh.fill, 1) & (kFew - 1)] = place_of(key, i);
+        });
+        __syncthreads();
     }
-    while (members > uint32_t(kList) && lo < hi) {
+    auto each = [&](auto f) {
+        if (whole) {
+#pragma unroll 1
+            for (uint32_t j = threadIdx.x; j < all; j += kThreads) {
+                const uint64_t place = sh.few[j];
+                const uint32_t key = uint32_t(place >> 32);
+                if (key >= lo && key <= hi) f(place, key);
+            }
+        } else {
+            each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int i, float l) {
+                const uint32_t key = argmax_order(l);
+                if (inside(l, key)) f(place_of(key, i), key);
+            });
+        }
+    };
+    // Fewer are compared with each other (members^2 comparisons).
+    const uint32_t most = whole ? 64 : kList;
+    while (members > most && lo < hi) {
         const uint32_t width = (hi - lo) / kBins + 1;
         __syncthreads();
         sh.sub.count[threadIdx.x] = 0;
         sh.sub.units[threadIdx.x] = 0;
         __syncthreads();
-        each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int, float l) {
-            const uint32_t key = argmax_order(l);
-            if (!inside(l, key)) return;
+        each([&](uint64_t, uint32_t key) {
             const uint32_t b = (hi - key) / width;
             atomicAdd(&sh.sub.count[b], 1u);
             atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sub.units[b]),
-                      static_cast<unsigned long long>(units_of(weigh(l, sc).off)));
+                      static_cast<unsigned long long>(units_of(weigh_once(logit_of(key), sc).off)));
         });
         __syncthreads();
         const uint32_t n = sh.sub.count[threadIdx.x];
@@ -558,7 +575,7 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
 #pragma unroll
                     for (int e = 0; e < kPer; ++e)
                         if (i + e < vocab && argmax_order(l[e]) == hi && ++k == c)
-                            sh.border = Border{place_of(hi, i + e), above + double(c) * part, false};
+                            sh.border = Border{place_of(hi, i + e), above + double(c) * part};
                 }
                 __syncthreads();
                 return;
@@ -571,11 +588,8 @@ __device__ __forceinline__ void border_in(const char* row, int vocab, const Scal
     __syncthreads();
     if (threadIdx.x == 0) sh.fill = 0;
     __syncthreads();
-    each_between<DT>(row, vocab, bound_of(lo), bound_of(hi), [&](int i, float l) {
-        const uint32_t key = argmax_order(l);
-        if (inside(l, key)) sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place_of(key, i);
-    });
-    border_of_list(int(members), mode, need, want, above, whole, sh);
+    each([&](uint64_t place, uint32_t) { sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place; });
+    border_of_list(int(members), mode, need, want, above, sh);
 }
 
 struct RowArgs {
@@ -1014,7 +1028,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             for (int e = 0; e < 2; ++e)
                 if (mine[e].bin == b) sh.list[atomicAdd(&sh.fill, 1) & (kList - 1)] = place[e];
             border_of_list(n, mode, mode == kByMass ? 0u : uint32_t(k) - (b ? sh.count[b - 1] : 0u),
-                           (want - mass_before(b)) / bin_scale(b), 0.0, true, sh);
+                           (want - mass_before(b)) / bin_scale(b), 0.0, sh);
             const Border at = sh.border;
             if (mode == kByCount) total = mass_before(b) + at.mass * bin_scale(b);
             border = at.place > border ? at.place : border;
@@ -1044,10 +1058,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     // top-k's, the top-p's of what that keeps, the min-p's.
     uint64_t border = 0;   // places from here on are kept
     double total = whole;
-    bool listed = true;    // sh.list holds the members of the border's bin
+    bool listed = false;   // sh.few holds the members of the border's bin
     int border_bin = kRest;
 #pragma unroll 1
-    for (int mode = kByCount; mode <= kByKey; ++mode) {
+    for (int mode = kByCount; mode <= kByMass; ++mode) {
         int b = k_bin;
         double want = 0.0;
         uint32_t need = 0;
@@ -1055,25 +1069,26 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             // Without a top-p behind it a lower border than the min-p's is none.
             if (k_bin == kRest || (!(top_p < 1.0f) && least_bin < k_bin)) continue;
             need = uint32_t(k) - (b ? sh.count[b - 1] : 0u);
-        } else if (mode == kByMass) {
+        } else {
             if (!(top_p < 1.0f) || (k_bin == kRest && least_bin < p_bin)) continue;
             want = double(top_p) * total;
             b = first_of(sh.mass[tid] >= want, tid, kRest - 1, sh);
             if (b > border_bin) continue;   // rounding alone: the top-k's border stands
-        } else {
-            if (!(min_p > 0.0f) || least_bin > border_bin || least_bin == kRest) continue;
-            b = least_bin;
-            need = least;
         }
         border_in<DT>(row, vocab, sc, b, members(b), mode, need, (want - mass_before(b)) / bin_scale(b), sh);
         const Border at = sh.border;
-        // The list is of bin b now, where the border lies already or comes to lie.
-        listed = at.listed;
+        // sh.few is of bin b now, where the border lies already or comes to lie.
+        listed = members(b) <= uint32_t(kFew);
         if (at.place > border) {
             border = at.place;
             border_bin = b;
             if (mode == kByCount) total = mass_before(b) + at.mass * bin_scale(b);
         }
+    }
+    if (uint64_t(least) << 32 > border && least_bin < kRest) {
+        border = uint64_t(least) << 32;
+        border_bin = least_bin;
+        listed = false;
     }
     if (border > best || min_p > 1.0f) {
         border = best;
@@ -1081,12 +1096,6 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         listed = false;
     }
 
-    auto kept = [&](int i, float l) {
-        const uint32_t key = argmax_order(l);
-        if (place_of(key, i) < border) return 0.0;
-        const Weight w = weigh(l, sc);
-        return w.bin < kRest ? part_of(w.off) * bin_scale(w.bin) : 0.0;
-    };
     // Kept weight slice by slice, from the histograms and the members of the
     // border's bin; then the slice, and in it the tile, in which the running sum
     // passes u times the total.
@@ -1103,7 +1112,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         };
         if (border_bin < kRest && listed) {
             for (int i = tid; i < int(members(border_bin)); i += kThreads) {
-                const uint64_t at = sh.list[i];
+                const uint64_t at = sh.few[i];
                 if (at >= border) add(int(0xFFFFFFFFu - uint32_t(at)), weigh_once(logit_of(uint32_t(at >> 32)), sc));
             }
         } else if (border_bin < kRest) {
@@ -1125,14 +1134,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
                 const int b = e * 64 + lane;
                 words[e] = b < kRest && b + shift < border_bin ? rec->words[b] : 0;
             }
-            double sum = 0.0;
-#pragma unroll 1
-            for (int e = 0; e < kBins / 64; ++e) {
-                const uint64_t word = words[0];
-                if (word != 0) sum += double(sum_of(word)) * kUnit * bin_scale(e * 64 + lane + shift);
+            double sum = 0.0;   // 64 bins are four octaves
 #pragma unroll
-                for (int n = 1; n < kBins / 64; ++n) words[n - 1] = words[n];
-            }
+            for (int e = kBins / 64 - 1; e >= 0; --e) sum = __builtin_fma(sum, 0x1p-4, double(sum_of(words[e])));
+            sum *= kUnit * bin_scale(lane + shift);
 #pragma unroll
             for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
             if (border_bin < kRest) sum += double(sh.slice[s]) * kUnit * bin_scale(border_bin);
@@ -1149,19 +1154,34 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         from = s * p.step;
         to = from + p.step < vocab ? from + p.step : vocab;
     }
+    __syncthreads();
+    sh.scale_of[tid] = tid < kRest ? bin_scale(tid) : 0.0;
+    __syncthreads();
+    auto kept = [&](int i, float l) {
+        const uint32_t key = argmax_order(l);
+        if (place_of(key, i) < border) return 0.0;
+        const Weight w = weigh(l, sc);
+        return part_of(w.off) * sh.scale_of[w.bin];
+    };
     // A run of logits a thread.
     const int run = ((to - from + kThreads - 1) / kThreads + kPer - 1) / kPer * kPer;
     const int begin = from + tid * run < to ? from + tid * run : to, end = to - begin < run ? to : begin + run;
+    const float bound = bound_of(uint32_t(border >> 32));
     double mine = 0.0;
 #pragma unroll 1
     for (int i = begin; i < end; i += kPer) {
         float l[kPer];
         load_logits<DT, kPer>(row, i, end, l);
-#pragma unroll 1
-        for (int e = 0; e < kPer && i + e < end; ++e) {
-            mine += kept(i + e, l[0]);
+        uint32_t hits = 0;
 #pragma unroll
-            for (int n = 1; n < kPer; ++n) l[n - 1] = l[n];
+        for (int e = 0; e < kPer; ++e) hits |= l[e] >= bound ? 1u << e : 0u;
+#pragma unroll 1
+        for (; hits; hits &= hits - 1) {
+            const int at = __builtin_ctz(hits);
+            float v = l[0];
+#pragma unroll
+            for (int e = 1; e < kPer; ++e) v = at == e ? l[e] : v;
+            mine += kept(i + at, v);
         }
     }
     const Sums<double> sums = scan(mine, sh);
