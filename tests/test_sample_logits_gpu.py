@@ -228,3 +228,27 @@ def test_sample_logits_in_a_graph_and_on_a_side_stream(ops):
         graph.replay()
         want = ops.sample_logits(*new, k, p)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("filters", [dict(), dict(top_p=0.97), dict(min_p=1e-4), dict(top_k=9000, top_p=0.99),
+                                     dict(top_k=40, top_p=0.9)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_logits_slices_of_two_tiles(ops, dtype, filters):
+    """Rows enough that each workgroup takes several slices one after the other; tails of a slice of one to 8 logits."""
+    for m, vocab in ((150, 60000), (260, 32769 + 7)):
+        x, t, u = rows_of(m, vocab, m)
+        x[3, -1] = x[3].max() + 30      # alone in a tail
+        x[5] = float("nan")
+        x[7, ::2] = -INF
+        check(ops, x.to(dtype), t, u, **filters)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_logits_longest_rows(ops, dtype):
+    """Slices of four tiles: rows that two tiles a slice would cut into more than are joined."""
+    vocab = 256 * 16384 + 8193
+    x, t, u = rows_of(2, vocab, 21)
+    x[1, vocab - 2] = x[1].max() + 3
+    check(ops, x.to(dtype), t, u, top_k=torch.tensor([60, 100000], dtype=torch.int32), top_p=0.9)
+    check(ops, x.to(dtype), t, u, min_p=1e-3)
+    check(ops, x.to(dtype), t, u)
