@@ -186,7 +186,13 @@ int launch_rows(const Problem& p, hipStream_t s) {
         // it took 54.8-56.4 against 50.4-51.2 us for fp32 logits, 53.4-55.2
         // against 52.3-53.0 for the greedy head and 52.0-52.3 against
         // 50.8-51.2 for the sampled one, and was removed.
-        if constexpr (AROWS == 32) return launch_cfg<DT, DT_OUT, 32, 8, 4, 1, 4, EPI, PRO>(p, s);
+        // In 8 bits a line holds twice the K, and 32 W rows to 4 waves, small
+        // enough for many workgroups a CU, lead at each M (fp32 logits, N =
+        // 151936, K = 1024, W over three copies): M = 32 38.0 against 45.7 us of
+        // the 16-bit configuration, M = 16 26.9 against 30.1, M = 8 25.0 against
+        // 30.7; K = 2048 65.5 / 70.6, 51.0 / 52.4, 48.8 / 51.5.
+        if constexpr (DT == kI8) return launch_cfg<DT, DT_OUT, AROWS, 2, 4, 1, 4, EPI, PRO>(p, s);
+        else if constexpr (AROWS == 32) return launch_cfg<DT, DT_OUT, 32, 8, 4, 1, 4, EPI, PRO>(p, s);
         else if constexpr (AROWS == 16) return launch_cfg<DT, DT_OUT, 16, 2, 8, 1, 8, EPI, PRO>(p, s);
         else return launch_cfg<DT, DT_OUT, 8, 2, 8, 2, 8, EPI, PRO>(p, s);
     }

@@ -327,3 +327,20 @@ def test_int8_ops_have_no_backward(ops):
     if scales.requires_grad:
         with pytest.raises(RuntimeError):
             scales.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 65536, 16), (8, 65537, 144), (9, 70001, 272), (16, 65540, 528),
+                                   (17, 65550, 1040), (32, 65551, 992)])
+def test_gemm_int8_wide_heads(ops, dtype, m, n, k):
+    """Decode rows on the output widths of LM heads."""
+    a, sa, w, sw = operands(m, n, k, m + k, extreme=True)
+    check_product(ops.gemm_int8(*[t.to(DEV) for t in (a, sa, w, sw)], dtype), a, sa, w, sw, dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 32768, 160), (16, 33001, 272), (29, 32780, 1040)])
+def test_gemm_int8_silu_mul_wide(ops, m, n, k):
+    a, sa, w, sw = operands(m, 2 * n, k, m + k)
+    sw = sw * 3
+    for dtype in (BF16, F32):
+        check_silu(ops.gemm_int8_silu_mul(*[t.to(DEV) for t in (a, sa, w, sw)], dtype), a, sa, w, sw, dtype)
