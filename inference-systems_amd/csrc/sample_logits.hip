@@ -942,7 +942,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         }
         // The least of them, as the largest of what they are below kRest.
         covered = kRest - int(max_all(uint32_t(kRest - mine), sh));
-        constexpr int kBatch = 16;   // loads in flight
+        constexpr int kBatch = 24;   // loads in flight
         for (int first = 0; first < p.slices; first += kBatch) {
             uint64_t word[kBatch];
 #pragma unroll
