@@ -26,7 +26,7 @@
 // loops are left rolled and what a step shares with another is a call.
 //
 // Measured: 1 x 151936 bf16, top-k 50 and top-p 0.9: 25 us, of which the slices 8
-// and the join 15.  256 x 151936 fp32 (156 MB), top-p and min-p by row: 122 us; the
+// and the join 15.  256 x 151936 fp32 (156 MB), top-p and min-p by row: 120 us; the
 // slices 72 (2.2 TB/s; reading alone takes 25), the join 50, which is the time of
 // the rows that look their border up (others 15).  One workgroup a row for all of
 // it: 176 and 231 us.  Slices by 512 threads instead of 1024: 82 us for 78.
@@ -1103,8 +1103,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     }
 
     // Kept weight slice by slice, from the histograms and the members of the
-    // border's bin; then the slice, and in it the tile, in which the running sum
-    // passes u times the total.
+    // border's bin; then the slice, and in it the thread's run, in which the running
+    // sum passes u times the total.
     int from = 0, to = vocab;
     double ahead = 0.0;
     const bool by_slice = STEP == 0 && !sc.flat;
