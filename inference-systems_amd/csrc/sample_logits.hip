@@ -1161,13 +1161,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         to = from + p.step < vocab ? from + p.step : vocab;
     }
     __syncthreads();
-    sh.scale_of[tid] = tid < kRest ? bin_scale(tid) : 0.0;
+    sh.scale_of[tid] = bin_scale(tid);
     __syncthreads();
     auto kept = [&](int i, float l) {
         const uint32_t key = argmax_order(l);
         if (place_of(key, i) < border) return 0.0;
         const Weight w = weigh(l, sc);
-        return part_of(w.off) * sh.scale_of[w.bin];
+        return w.bin < kRest ? part_of(w.off) * sh.scale_of[w.bin] : 0.0;
     };
     // A run of logits a thread.
     const int run = ((to - from + kThreads - 1) / kThreads + kPer - 1) / kPer * kPer;
