@@ -904,13 +904,16 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         best = max_all(its_best, sh);
     }
     const uint32_t best_key = uint32_t(best >> 32);
-    if (!draws(t, best)) {
+    // The largest logit's token alone: a row that draws none, and what is left of
+    // one where no kept token should have weight, so that every token written is
+    // one of the row's.
+    auto take_best = [&] {
         if (tid == 0) {
             p.tokens[r] = int(0xFFFFFFFFu - uint32_t(best));
             p.logprobs[r] = best_key == kNanKey ? __builtin_nanf("") : 0.0f;
         }
-        return;
-    }
+    };
+    if (!draws(t, best)) return take_best();
     const Scale sc = scale_of(logit_of(best_key), t);
     if (tid == 0) sh.scale = sc;   // read behind the barriers of what follows
 
@@ -1051,7 +1054,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             const double target = share * total;
             const int one = w[0] > 0.0 && sum - w[1] > target ? 0 : w[1] > 0.0 && sum > target ? 1 : -1;
             int at = first_of(one >= 0, 2 * tid + one, -1, sh);
-            if (at < 0) at = last_of(w[0] + w[1] > 0.0, 2 * tid + (w[1] > 0.0), 0, sh);
+            if (at < 0) at = last_of(w[0] + w[1] > 0.0, 2 * tid + (w[1] > 0.0), -1, sh);
+            if (at < 0) return take_best();
             if (tid == at >> 1) {
                 p.tokens[r] = int64_t(0xFFFFFFFFu - uint32_t(place[at & 1]));
                 p.logprobs[r] = static_cast<float>(log_once(w[at & 1] / total));
@@ -1195,7 +1199,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     if (!by_slice) total = sums.all;
     const double target = share * total - ahead;
     int at = first_of(mine > 0.0 && upto > target, tid, kThreads, sh);
-    if (at == kThreads) at = last_of(mine > 0.0, tid, 0, sh);
+    if (at == kThreads) at = last_of(mine > 0.0, tid, -1, sh);
+    if (at < 0) return take_best();
     if (tid != at) return;
     double sum = upto - mine, its = 0.0;
     int token = begin;

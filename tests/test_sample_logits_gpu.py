@@ -252,3 +252,21 @@ def test_sample_logits_longest_rows(ops, dtype):
     check(ops, x.to(dtype), t, u, top_k=torch.tensor([60, 100000], dtype=torch.int32), top_p=0.9)
     check(ops, x.to(dtype), t, u, min_p=1e-3)
     check(ops, x.to(dtype), t, u)
+
+
+@pytest.mark.parametrize("filters", [dict(), dict(top_k=5), dict(top_p=0.9), dict(min_p=0.1), dict(top_k=3000, top_p=0.5)])
+@pytest.mark.parametrize("vocab", [1000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_logits_tokens_are_in_the_vocabulary(ops, dtype, vocab, filters):
+    """Whatever the temperature and the size of the logits, the token is one of the row's, and its logprob a number: rows of
+    one slice and of several, the largest logit in the last of them."""
+    g = torch.Generator().manual_seed(vocab)
+    t = torch.cat([10.0 ** (-10.5 + 5 * torch.rand(32, generator=g)), torch.tensor([1e-9, 1e-8, 1.5e-8, 3e-9]).repeat(8)])
+    x = torch.randn(64, vocab, generator=g)
+    x[torch.arange(64), vocab - 1 - torch.randint(0, 900, (64,), generator=g)] = 5 + 25 * torch.rand(64, generator=g)
+    x[::4] *= 10.0 ** torch.linspace(0, 37, 16)[:, None]
+    given = [torch.full((64,), v, dtype=torch.int32 if k == "top_k" else F32, device=DEV) if v else None
+             for k, v in ((k, filters.get(k)) for k in ("top_k", "top_p", "min_p"))]
+    tokens, logprobs = ops.sample_logits(x.to(dtype).to(DEV), t.to(DEV), torch.rand(64, generator=g).to(DEV), *given)
+    assert bool(((tokens >= 0) & (tokens < vocab)).all())
+    assert bool((logprobs <= 0).all())
