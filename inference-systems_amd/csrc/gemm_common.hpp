@@ -384,7 +384,7 @@ __device__ __forceinline__ float norm_scale(float ss, int64_t k, float eps) {
 // 0xFFFFFFFF - column in the low word, so the largest key is the largest
 // logit and, among equal logits, the first column (torch.argmax's rule).
 // Key 0 is below every real key.
-__device__ __forceinline__ uint32_t argmax_order(float v) {
+__host__ __device__ __forceinline__ uint32_t argmax_order(float v) {
     // -0 ranks equal to +0, and every NaN ranks above every number (as in
     // torch.argmax): both are canonicalised first.
     const uint32_t b = v != v ? 0x7FC00000u : (v == 0.0f ? 0u : __builtin_bit_cast(uint32_t, v));

@@ -270,3 +270,19 @@ def test_sample_logits_tokens_are_in_the_vocabulary(ops, dtype, vocab, filters):
     tokens, logprobs = ops.sample_logits(x.to(dtype).to(DEV), t.to(DEV), torch.rand(64, generator=g).to(DEV), *given)
     assert bool(((tokens >= 0) & (tokens < vocab)).all())
     assert bool((logprobs <= 0).all())
+
+
+@pytest.mark.parametrize("filters", [dict(), dict(top_k=7), dict(top_p=0.9), dict(min_p=0.2)])
+@pytest.mark.parametrize("vocab", [1000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_logits_small_temperatures(ops, dtype, vocab, filters):
+    """Temperatures down to the greedy ones and logits of any size, with l / T up to 1e47: equal, near and far logits at the
+    top, in a row's last slice."""
+    g = torch.Generator().manual_seed(vocab + 1)
+    t = torch.tensor([1.01e-10, 1e-9, 1e-9, 3e-9, 1e-8, 1.5e-8, 3e-8, 1e-6, 0.9, 40.0] * 3)
+    top = torch.cat([5 + 25 * torch.rand(10, generator=g), 10.0 ** torch.linspace(-9, 0, 10), 10.0 ** torch.linspace(9, 37, 10)])
+    x = torch.randn(30, vocab, generator=g) * top[:, None] / 10
+    at = vocab - 1 - torch.randint(0, 900, (30, 6), generator=g)
+    # Some at the top within a few weights of each other, some equal.
+    x.scatter_(1, at, top[:, None] - t[:, None] * torch.tensor([0.0, 0.0, 0.3, 1.0, 2.5, 7.0]))
+    check(ops, x.to(dtype), t, torch.rand(30, generator=g), **filters)
