@@ -831,6 +831,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     __syncthreads();
     auto members = [&](int b) { return b ? sh.count[b] - sh.count[b - 1] : sh.count[0]; };
     auto mass_before = [&](int b) { return b ? sh.mass[b - 1] : 0.0; };
+    // The first bin with members at which the running mass reaches `want`; the last
+    // one where rounding leaves the whole a little short.  A bin without members is
+    // none: its sum is that of the bins before it in another order, which may pass
+    // `want` in the last bit alone.
+    const bool some = members(tid) > 0;
+    auto bin_reaching = [&](double want) {
+        const int b = first_of(some && sh.mass[tid] >= want, tid, -1, sh);
+        return b >= 0 ? b : last_of(some, tid, 0, sh);
+    };
 
     // The least logit whose weight is min_p or more, as a key.
     uint32_t least = 0;
@@ -849,7 +858,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     // Where everything up to the border is listed, and not too many, the listed
     // members decide.  With a top-k in front of the top-p its whole bin is needed.
     int last = k_bin;
-    if (top_p < 1.0f && k_bin == kRest) last = first_of(sh.mass[tid] >= double(top_p) * whole, tid, kRest - 1, sh);
+    if (top_p < 1.0f && k_bin == kRest) last = bin_reaching(double(top_p) * whole);
     const int p_bin = last;   // of the top-p where there is no top-k
     if (!(top_p < 1.0f && k_bin < kRest)) last = least_bin < last ? least_bin : last;
     if (last >= kRest) last = kRest - 1;
@@ -888,7 +897,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             } else {
                 if (!(top_p < 1.0f)) continue;
                 want = double(top_p) * total;
-                b = first_of(sh.mass[tid] >= want, tid, kRest - 1, sh);
+                b = bin_reaching(want);
                 if (b > last) continue;
             }
             const int n = int(members(b));
@@ -948,7 +957,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
         } else {
             if (!(top_p < 1.0f) || (k_bin == kRest && least_bin < p_bin)) continue;
             want = double(top_p) * total;
-            b = first_of(sh.mass[tid] >= want, tid, kRest - 1, sh);
+            b = bin_reaching(want);
             if (b > border_bin) continue;   // rounding alone: the top-k's border stands
         }
         border_in<DT>(row, vocab, sc, b, members(b), mode, need, (want - mass_before(b)) / bin_scale(b), sh);

@@ -286,3 +286,28 @@ def test_sample_logits_small_temperatures(ops, dtype, vocab, filters):
     # Some at the top within a few weights of each other, some equal.
     x.scatter_(1, at, top[:, None] - t[:, None] * torch.tensor([0.0, 0.0, 0.3, 1.0, 2.5, 7.0]))
     check(ops, x.to(dtype), t, torch.rand(30, generator=g), **filters)
+
+
+# Half of this row's weight lies in its first six tokens, to the last bit: the running sum at the bin of the sixth is a
+# little below half, at the empty bins behind it, summed in another order, a little above.
+HALF = """0x0.0p+0 -0x1.b15cea0000000p-6 -0x1.a7d9e60000000p-4 -0x1.8a2a920000000p-3 -0x1.be3d9c0000000p-3
+-0x1.2ecf300000000p-2 -0x1.5480720000000p+0 -0x1.1e13040000000p+1 -0x1.506a400000000p+0 -0x1.ffabb40000000p-1
+-0x1.0427820000000p+1 -0x1.8ffe680000000p+0 -0x1.1c52c20000000p+1 -0x1.2975820000000p+0 -0x1.5204e40000000p+0
+-0x1.1c8cac0000000p+1 -0x1.ac29a20000000p+0 -0x1.abd5760000000p+0 -0x1.29c9020000000p+0 -0x1.7e316a0000000p-1
+-0x1.3ca3e80000000p+1 -0x1.c2d1c20000000p-1 -0x1.2764000000000p+1 -0x1.692b340000000p+0 -0x1.40ec7e0000000p+1
+-0x1.785a100000000p+0 -0x1.3d6a2c0000000p+1 -0x1.c3caa00000000p+0 -0x1.2baea20000000p+0 -0x1.0e7b240000000p+1
+-0x1.2f0a620000000p+1 -0x1.3a3ae40000000p+2 -0x1.27b4b20000000p+3 -0x1.9727b80000000p+3 -0x1.1bac220000000p+4
+-0x1.7f12a60000000p+4"""
+
+
+@pytest.mark.parametrize("vocab", [36, 36 + 20000])
+def test_sample_logits_border_behind_an_empty_bin(ops, vocab):
+    """A top-p whose weight falls between two running sums of the same tokens: one token more or less, no other set."""
+    x = torch.full((1, vocab), -INF)
+    x[0, :36] = torch.tensor([float.fromhex(v) for v in HALF.split()])
+    order = torch.sort(x[0, :36].double(), descending=True).values.exp()
+    one = torch.ones(1, device=DEV)
+    token, logprob = ops.sample_logits(x.to(DEV), one, 0 * one, None, 0.5 * one)
+    assert token.item() == 0
+    wanted = [-order[:n].sum().log().item() for n in (6, 7)]
+    assert any(abs(logprob.item() - w) <= abs(w) * 2.0 ** -24 + 1e-11 for w in wanted), (logprob.item(), wanted)
