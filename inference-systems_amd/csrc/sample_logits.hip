@@ -845,7 +845,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     uint32_t least = 0;
     int least_bin = kRest;   // no member of a lower one has that weight
     if (min_p > 0.0f) {
-        const double l = min_p >= 1.0f ? double(sc.largest) : double(sc.largest) + double(t) * log_once(double(min_p));
+        // At T = inf every finite logit weighs 1 (and the logarithm's product is no number).
+        double l = double(sc.largest);
+        if (t == __builtin_inff() && min_p <= 1.0f && !sc.flat) l = -__builtin_inf();
+        else if (min_p < 1.0f) l += double(t) * log_once(double(min_p));
         const float near = float(l);
         least = argmax_order(near) + (double(near) < l ? 1u : 0u);
         if (min_p > 1.0f || least > best_key) least = best_key;

@@ -311,3 +311,16 @@ def test_sample_logits_border_behind_an_empty_bin(ops, vocab):
     assert token.item() == 0
     wanted = [-order[:n].sum().log().item() for n in (6, 7)]
     assert any(abs(logprob.item() - w) <= abs(w) * 2.0 ** -24 + 1e-11 for w in wanted), (logprob.item(), wanted)
+
+
+@pytest.mark.parametrize("vocab", [300, 40000])
+def test_sample_logits_infinite_temperature(ops, vocab):
+    """Every finite logit weighs 1, so each min-p up to 1 keeps them all; infinities as at any temperature."""
+    x, _, u = rows_of(6, vocab, 31)
+    x[1, ::2] = -INF
+    x[2] = -INF
+    x[3, 5], x[3, vocab - 9] = INF, INF
+    x[4] = 2.0
+    for filters in (dict(), dict(min_p=1.0), dict(min_p=0.5), dict(min_p=1.0, top_k=vocab // 2), dict(min_p=1.0, top_p=0.3),
+                    dict(min_p=2.0), dict(min_p=1.0 + 2.0 ** -23)):
+        check(ops, x, INF, u, **filters)
