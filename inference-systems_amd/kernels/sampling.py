@@ -113,8 +113,6 @@ def torch_sample_logits(logits: torch.Tensor, temperatures: torch.Tensor, unifor
                         min_p: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """sample_logits in torch operations, on finite and infinite logits: a sort a row, weights in 64 bits."""
     shape, vocab = logits.shape[:-1], logits.shape[-1]
-
-
     x = logits.reshape(-1, vocab).float()
     t = temperatures.reshape(-1, 1)
     greedy = ~(t > GREEDY_TEMPERATURE)
@@ -123,7 +121,8 @@ def torch_sample_logits(logits: torch.Tensor, temperatures: torch.Tensor, unifor
     top = ordered[:, :1].double()
     weight = torch.where(ordered.double() == top, 1.0,
                          ((ordered.double() - top) / torch.where(greedy, 1.0, t).double()).exp())
-    weight = torch.where((ordered == -float("inf")) & (top > -float("inf")), 0.0, weight)
+    # Below an infinite logit nothing has weight, nor has -inf below a finite one (at T = inf both are NaN so far).
+    weight = torch.where((ordered.double() < top) & (top.isinf() | ordered.isinf()), 0.0, weight)
     rank = torch.arange(vocab, device=logits.device)
     kept = torch.ones_like(weight, dtype=torch.bool)
     if top_k is not None:

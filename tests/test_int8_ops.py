@@ -273,3 +273,19 @@ def test_step_in_8_bits_on_the_torch_backend():
     for call in (lambda: head.greedy(out), lambda: head.sample(out, t, 0, 0)):
         with pytest.raises(RuntimeError, match="8 bits"):
             call()
+
+
+def test_torch_sample_logits_at_infinite_temperatures():
+    """Every finite logit weighs 1; below an infinite one nothing has weight."""
+    inf = float("inf")
+    x = torch.randn(6, 40, generator=torch.Generator().manual_seed(5))
+    x[1, ::3] = -inf
+    x[2] = -inf
+    x[3, 7], x[3, 20], x[3, 30] = inf, inf, -inf
+    x[4] = inf
+    t, u = torch.full((6,), inf), torch.linspace(0, 0.99, 6)
+    for p, q in ((None, None), (0.5, None), (None, 1.0), (0.5, 0.5), (None, 2.0)):
+        tokens, shares = K.torch_sample_logits(x, t, u, None, *(None if v is None else torch.full((6,), v) for v in (p, q)))
+        for i in range(6):
+            token, share = orc.sample(x[i].double().numpy(), inf, float(u[i]), None, p, q)
+            assert tokens[i] == token and abs(shares[i].item() - share) <= abs(share) * U + 1e-11, (i, p, q)
