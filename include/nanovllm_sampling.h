@@ -38,8 +38,9 @@ extern "C" {
  * tokens that hold it.  A row with a NaN takes its first NaN, with logprob NaN.
  * u below 0 or NaN counts as 0, u of 1 or more takes the last kept token.
  *
- * Weights are off by less than 2^-34 of themselves, their sums are held in 64
- * bits, and no sum depends on the order in which workgroups run.  Workspace: nanovllm_sample_logits_workspace_bytes()
+ * Weights are off by less than 2^-32 of themselves (2^-25 where T is above
+ * 2^100), their sums are held in 64 bits, and no sum depends on the order in
+ * which workgroups run.  Workspace: nanovllm_sample_logits_workspace_bytes()
  * bytes, 16-byte aligned scratch.  vocab is at most 2^23.
  */
 int nanovllm_sample_logits(const void* logits, const float* temperatures, const float* uniforms,

@@ -32,8 +32,8 @@
 // it: 176 and 231 us.  Slices by 512 threads instead of 1024: 82 us for 78.
 //
 // Numerics: l c is held as a product and its remainder; a weight within its bin
-// is a whole number of 2^-36, off by two of them at most, and summed as one, in
-// one 64-bit word with the count.  Sums over bins are in 64 bits and do not depend
+// is a whole number of 2^-36, off by less than 8 of them (sample_weights.hpp), and
+// summed as one, in one 64-bit word with the count.  Sums over bins are in 64 bits and do not depend
 // on the order of atomics.  The last bin holds everything from 2^-63.9 of the
 // largest weight down, which counts as 0.
 #include "int8_common.hpp"

@@ -76,11 +76,19 @@ __host__ __device__ __forceinline__ Scale scale_of(float largest, float t) {
     return s;
 }
 
-// Of a row whose largest logit is finite.  Near 0 the product is a sum of two
-// floats whose error is below 2^-24 of its last place, 2^-36 of a weight at a
-// product of 2^13 and less below; y, the product less the whole number, is exact.
-// 2^(y / 16) - 1 in units of 2^-36: the linear term as a float and its remainder,
-// the others, to the 5th power, with the remainder (off by less than 2^-43).
+// Of a row whose largest logit is finite.  y, the product in 32 bits less its whole
+// number, is exact; low is what that product leaves of l c.  2^(y / 16) - 1 in units
+// of 2^-36: the linear term of y as a float and its remainder, the others, to the
+// 5th power, with the remainder.
+//
+// Off by less than 8 units, at a product up to 2^14: less than 1 each for the cuts of
+// both terms to whole numbers; 0.17 for low's rounding and 0.25 for its term's; 1 for
+// that of the sum r, which may pass 2^24; of the square term, up to 1.7e7 units, 0.5
+// each from its coefficient and the polynomial q, 1 from z * z and 1.95 from z; 0.02
+// for the 6th power.  4.4 is the most in 4e7 random products.  A weight is 0.978 of its bin's
+// or more, so as a share of the largest logit's it is good to 2^-32 (above T = 2^100,
+// where cl is denormal, to 2^-25).
+//
 // A vector instruction in 64 bits takes as long as four in 32 here, and the
 // sum of both terms as integers takes the place of a wider type.  NEAR: all products
 // down to the last bin's are within kNear.

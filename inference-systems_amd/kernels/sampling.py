@@ -20,9 +20,9 @@ nanovllm/layers/sampler.py:8-21, which knows the temperature alone).
         int32; one entry a row.  A row whose largest logit is an infinity draws
         among its holders; one with a NaN takes its first NaN, logprob NaN.
 
-The result depends on the inputs alone: weights are good to
-2^-34, and no sum depends on the order in which workgroups run.  ``sample_rows`` adds
-the ``torch | hip | auto`` switch.
+The result depends on the inputs alone: weights are good to 2^-32 of themselves
+(2^-25 where T is above 2^100), and no sum depends on the order in which
+workgroups run.  ``sample_rows`` adds the ``torch | hip | auto`` switch.
 """
 from __future__ import annotations
 

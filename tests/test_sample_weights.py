@@ -116,3 +116,29 @@ def test_bins_do_not_fall_with_the_logit(weigh):
             y = np.sort(below(g, np.full(20000, x), np.full(20000, t, np.float32)))[::-1]
             bins, _ = weigh(y, x, np.float32(t))
             assert (np.diff(bins) >= 0).all(), (t, top)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_weights_are_good_to_2_to_the_minus_32(weigh, seed):
+    """Weights as shares of the largest logit's.  Within its bin each is off by less than 8 units of 2^-36: one for each of
+    the two terms' cuts to a whole number; from the remainder up to 2^-9 of the product 0.25 for its term's rounding and
+    0.17 for its own; 1 for the sum's rounding at 2^24 units; from the square term, up to 1.7e7 units, 0.5 each for the
+    coefficient and the polynomial, 1 for the square and 1.95 for twice its argument's rounding; 0.02 for the 6th power.
+    A weight is 0.978 of its bin's at least, so two of them are off by less than 2 * 8 * 2^-36 = 2^-32 (7.4 / 0.978 is
+    below 8).  Above T = 2^100 the second float of c is denormal, off by up to 2^-150; times the 2^129 that two logits may
+    lie apart, times ln 2 / 16, that is 2^-25.5 more."""
+    g = np.random.default_rng(200 + seed)
+    n = 300000
+    x, t = logits(g, n), temperatures(g, n)
+    if seed % 2:   # ordinary rows, where products are in 32 bits; next to half a bin, where most is off
+        x, t = g.uniform(-40, 40, n).astype(np.float32), g.uniform(0.1, 3.0, n).astype(np.float32)
+    y = below(g, x, t)
+    bins, offs = weigh(y, x, t)
+    _, top_offs = weigh(x, x, t)
+    ld = np.longdouble
+    part = (ld(1) + offs.astype(ld) * ld(2.0) ** -36) / (ld(1) + top_offs.astype(ld) * ld(2.0) ** -36)
+    down = octaves16(x, y, t)
+    has = bins < REST
+    most = np.where(t[has] <= 2.0 ** 100, ld(2.0) ** -32, ld(2.0) ** -25)
+    error = np.abs(part[has] * np.exp2((down[has] - bins[has]) / ld(16)) - 1)
+    assert has.mean() > 0.3 and (error < most).all(), float((error / most).max())
