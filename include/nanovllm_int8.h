@@ -41,7 +41,9 @@ int nanovllm_quantize_rows(const void* x, int8_t* codes, float* scales,
  *     s * (1 + w) * rsqrt(mean(s^2) + eps)
  * in 8 bits as above, from fp32 (it is rounded to no other type).  h, r, w and
  * residual_out are of dtype (f16 or bf16); h and r have row strides ldh and
- * ldr; codes and residual_out are contiguous [m, k].
+ * ldr; codes and residual_out are contiguous [m, k].  residual_out must not
+ * overlap the span of h or of r (refused); nor may any output of these entry
+ * points overlap an input.
  */
 int nanovllm_add_rmsnorm_quantize(const void* h, const void* r, const void* w, float eps,
                                   int8_t* codes, float* scales, void* residual_out,

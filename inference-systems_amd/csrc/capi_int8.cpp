@@ -38,6 +38,15 @@ int check_pointer(const char* op, const char* name, const void* p, int bytes) {
     return NANOVLLM_GEMM_OK;
 }
 
+// Whether the contiguous [m, k] at `out` shares bytes with the span of m rows of k
+// elements at `in`, `ld` apart (positive sizes; all elements of `bytes`).
+bool overlaps(const void* out, const void* in, int64_t m, int64_t k, int64_t ld, int bytes) {
+    const auto begin = static_cast<__int128>(reinterpret_cast<uintptr_t>(out));
+    const auto other = static_cast<__int128>(reinterpret_cast<uintptr_t>(in));
+    return begin < other + (static_cast<__int128>(m - 1) * ld + k) * bytes &&
+           other < begin + static_cast<__int128>(m) * k * bytes;
+}
+
 // Which rows splitk_decode takes, in the units of the bf16 GEMM of the same
 // bytes (nanovllm_gemm_select and nanovllm_gemm_silu_mul_select): the weights
 // are streamed once up to M = 32, and up to 64 where larger tiles would leave
@@ -89,6 +98,8 @@ int nanovllm_add_rmsnorm_quantize(const void* h, const void* r, const void* w, f
     if (rc == NANOVLLM_GEMM_OK) rc = check_pointer(op, "codes", codes, 1);
     if (rc == NANOVLLM_GEMM_OK) rc = check_pointer(op, "scales", scales, 4);
     if (rc != NANOVLLM_GEMM_OK) return rc;
+    if (overlaps(residual_out, h, m, k, ldh, 2) || overlaps(residual_out, r, m, k, ldr, 2))
+        return set_error(NANOVLLM_GEMM_EINVAL, "%s: residual_out must not overlap h or r", op);
     return launch_add_rmsnorm_quantize(h, ldh, r, ldr, w, eps, codes, scales, residual_out, m, k, dtype,
                                        static_cast<hipStream_t>(stream));
 }

@@ -4,7 +4,8 @@
 // Both are bound by memory: a row is read once, held in registers across the
 // reduction of its maximum, and written once as codes.  A row belongs to 16, 64
 // or 256 threads: short rows share a wave, those up to 2048 elements need no
-// barrier, and only rows beyond 16384 are read twice.  Longer rows go to more
+// barrier, and only rows beyond 16384 are read twice (the sum is stored the second
+// time).  Longer rows go to more
 // threads, not to more chunks a thread: 8192 x 3584 fp16 takes 16.8 us with two
 // chunks of 8 elements in each of 256 threads, 22.1 us with eight in a wave's.
 //
@@ -162,7 +163,7 @@ struct RowArgs {
     int32_t m, k;
 };
 
-template <int DT, int NORM>
+template <int DT, int NORM, int STORE>
 __device__ __forceinline__ void row_values(const char* __restrict__ x, const char* __restrict__ res_in,
                                            const char* __restrict__ weight, char* __restrict__ res, int c, int k,
                                            float (&z)[8], float& ss) {
@@ -180,6 +181,7 @@ __device__ __forceinline__ void row_values(const char* __restrict__ x, const cha
             r[i] = s;
             z[i] = s * (1.0f + w[i]);
         }
+        if constexpr (!STORE) return;
         uint16_t* out = reinterpret_cast<uint16_t*>(res) + c;
         if (left >= 8) {
             const u32x4_t v{pack2<DT>(r[0], r[1]), pack2<DT>(r[2], r[3]), pack2<DT>(r[4], r[5]), pack2<DT>(r[6], r[7])};
@@ -221,13 +223,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(
             const int c = 8 * (t + TPR * j);
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[j][i] = 0.0f;
-            if (c < k) row_values<DT, NORM>(x, res_in, weight, res, c, k, z[j], ss);
+            if (c < k) row_values<DT, NORM, 1>(x, res_in, weight, res, c, k, z[j], ss);
         }
 #pragma unroll
         for (int j = 0; j < CH; ++j) higher(z[j]);
     } else {
         for (int c = 8 * t; c < k; c += 8 * TPR) {
-            row_values<DT, NORM>(x, res_in, weight, res, c, k, z[0], ss);
+            row_values<DT, NORM, 0>(x, res_in, weight, res, c, k, z[0], ss);
             higher(z[0]);
         }
     }
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(
     } else {
         float ignored = 0.0f;
         for (int c = 8 * t; c < k; c += 8 * TPR) {
-            row_values<DT, NORM>(x, res_in, weight, res, c, k, z[0], ignored);
+            row_values<DT, NORM, 1>(x, res_in, weight, res, c, k, z[0], ignored);
             store_codes(codes + c, k - c, z[0], sc);
         }
     }

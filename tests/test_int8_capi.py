@@ -122,6 +122,18 @@ def test_sampler_workspace_is_checked():
         assert _sample(workspace=P + 8) == L.EINVAL
 
 
+K20 = 20000 * 2    # bytes of a row of 20000
+
+
+@pytest.mark.parametrize("changes", [dict(h=P), dict(r=P), dict(h=P - 2), dict(r=P + 3 * K20 - 2),
+                                     dict(h=P - (2 * 20008 + 19999) * 2, ldh=20008), dict(r=P + 40, ldr=2 ** 40)])
+def test_the_sum_does_not_replace_its_terms(changes):
+    """residual_out in place of h or r, or next to them by an element: rows too long for the registers are read twice."""
+    a = dict(h=P + 100 * K20, r=P + 200 * K20, residual_out=P, m=3, k=20000, ldh=20000, ldr=20000)
+    assert _norm(**(a | changes)) == L.EINVAL
+    assert "must not overlap" in L.last_error()
+
+
 CHILD = r"""
 import sys
 import pytest
