@@ -29,7 +29,8 @@ Same conventions as ``nanovllm::gemm``: ``nanovllm`` namespace, fixed
 RuntimeError messages, fake implementations, launch on the current stream, no
 fallback inside the op.  ``int8_linear``, ``int8_silu_mul_linear`` and
 ``int8_add_rmsnorm_linear`` add the ``torch | hip | auto`` switch with the same
-arithmetic in torch operations as the ``torch`` backend.
+arithmetic in torch operations as the ``torch`` backend.  None of these has a
+backward: asking for one raises, on either backend.
 """
 from __future__ import annotations
 
@@ -296,6 +297,25 @@ def _weights_reason(x, w, w_scales, out_dtype, silu_mul) -> Optional[str]:
     return None
 
 
+class _NoBackward(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, y, name, *inputs):
+        ctx.name = name
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError(f"{ctx.name} has no backward: the layers in 8 bits serve")
+
+
+def _refuse_backward(name: str, y: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
+    """y with the ops' refusal of a backward: codes have no gradient, and that of the scales alone is no row's."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        return _NoBackward.apply(y, name, *inputs)
+    return y
+
+
 def _hip(backend: Optional[str], reason) -> bool:
     backend = validate_gemm_backend(backend) if backend is not None else default_backend()
     return backend == "hip" or (backend == "auto" and reason() is None)
@@ -312,9 +332,12 @@ def _int8_linear(x, w, w_scales, out_dtype, backend, silu_mul):
 
     if _hip(backend, lambda: reason(x, w, w_scales)):
         return run_hip(op, reason, x, w, w_scales)
-    if silu_mul:
-        return _torch_silu_mul(torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, torch.float32), out_dtype)
-    return torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, out_dtype)
+    with torch.no_grad():
+        if silu_mul:
+            y = _torch_silu_mul(torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, torch.float32), out_dtype)
+        else:
+            y = torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, out_dtype)
+    return _refuse_backward("int8_silu_mul_linear" if silu_mul else "int8_linear", y, x, w_scales)
 
 
 def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None,
@@ -348,7 +371,11 @@ def int8_add_rmsnorm_linear(h: torch.Tensor, residual: torch.Tensor, norm_weight
     args = (h, residual, norm_weight, w, w_scales)
     if _hip(backend, lambda: reason(*args)):
         return run_hip(op, reason, *args)
-    summed = h.float() + residual.float()
-    normed = summed * torch.rsqrt(summed.pow(2).mean(-1, keepdim=True) + eps) * (1.0 + norm_weight.float())
-    y = torch_gemm_int8(*torch_quantize_rows(normed), w, w_scales, torch.float32)
-    return (_torch_silu_mul(y, h.dtype) if silu_mul else y.to(h.dtype)), summed.to(h.dtype)
+    with torch.no_grad():
+        summed = h.float() + residual.float()
+        normed = summed * torch.rsqrt(summed.pow(2).mean(-1, keepdim=True) + eps) * (1.0 + norm_weight.float())
+        y = torch_gemm_int8(*torch_quantize_rows(normed), w, w_scales, torch.float32)
+        y = _torch_silu_mul(y, h.dtype) if silu_mul else y.to(h.dtype)
+    given = (h, residual, norm_weight, w_scales)
+    return (_refuse_backward("int8_add_rmsnorm_linear", y, *given),
+            _refuse_backward("int8_add_rmsnorm_linear", summed.to(h.dtype), *given))

@@ -289,3 +289,31 @@ def test_torch_sample_logits_at_infinite_temperatures():
         for i in range(6):
             token, share = orc.sample(x[i].double().numpy(), inf, float(u[i]), None, p, q)
             assert tokens[i] == token and abs(shares[i].item() - share) <= abs(share) * U + 1e-11, (i, p, q)
+
+
+NO_BACKWARD = {
+    "int8_linear": lambda x, r, n, w, s: [K.int8_linear(x, w, s, backend="torch")],
+    "int8_silu_mul_linear": lambda x, r, n, w, s: [K.int8_silu_mul_linear(x, w, s, backend="torch")],
+    "int8_add_rmsnorm_linear": lambda x, r, n, w, s: K.int8_add_rmsnorm_linear(x, r, n, 1e-6, w, s, backend="torch"),
+}
+
+
+@pytest.mark.parametrize("name", NO_BACKWARD)
+def test_the_torch_backend_has_no_backward_either(name):
+    """What is differentiable of a row in 8 bits is its scale alone: refused, as the ops refuse it."""
+    g = torch.Generator().manual_seed(6)
+    x, r, n = torch.randn(3, 16, generator=g), torch.randn(3, 16, generator=g), torch.randn(16, generator=g)
+    w, s = K.torch_quantize_rows(torch.randn(8, 16, generator=g))
+    want = NO_BACKWARD[name](x, r, n, w, s)
+    assert not any(y.requires_grad for y in want)
+    for leaf in (x, n) if "norm" in name else (x,):
+        leaf.requires_grad_()
+        with torch.no_grad():
+            assert not any(y.requires_grad for y in NO_BACKWARD[name](x, r, n, w, s))
+        for i, y in enumerate(want):
+            out = NO_BACKWARD[name](x, r, n, w, s)[i]
+            assert torch.equal(out, y) and out.requires_grad
+            with pytest.raises(RuntimeError, match=f"{name} has no backward"):
+                out.sum().backward()
+        assert leaf.grad is None
+        leaf.requires_grad_(False)
