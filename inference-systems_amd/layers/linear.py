@@ -48,7 +48,8 @@ def _tp_rank_size() -> tuple[int, int]:
 
 class Int8Weight(nn.Module):
     """A module whose ``weight`` [N, K] can be kept in 8 bits: ``weight_codes`` (int8) and ``weight_scales`` (float32,
-    a scale for each row) in its place, both in the state dict."""
+    a scale for each row) in its place, both in the state dict.  A 16-bit module that loads such a state dict keeps its
+    weight in 8 bits from then on; a 16-bit weight is loaded before ``quantize_int8``, not after."""
 
     weight_codes: Optional[torch.Tensor]
     weight_scales: Optional[torch.Tensor]
@@ -70,6 +71,22 @@ class Int8Weight(nn.Module):
         weight = self.weight.detach()
         self.weight_codes, self.weight_scales = quantize_rows(weight) if weight.is_cuda else torch_quantize_rows(weight)
         self.weight = None
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        codes, scales = (state_dict.get(prefix + name) for name in ("weight_codes", "weight_scales"))
+        if not self.is_int8 and codes is not None and scales is not None:
+            shape = self.weight.shape
+            if codes.shape == shape and scales.shape == shape[:1]:
+                self.weight_codes = torch.empty_like(self.weight, dtype=torch.int8, requires_grad=False)
+                self.weight_scales = self.weight.new_empty(shape[:1], dtype=torch.float32, requires_grad=False)
+                self.weight = None
+            else:
+                error_msgs.append(f"size mismatch for {prefix}weight_codes and {prefix}weight_scales: {tuple(codes.shape)} "
+                                  f"and {tuple(scales.shape)} in the state dict, the weight has {tuple(shape)}.")
+        elif self.is_int8 and prefix + "weight" in state_dict:
+            error_msgs.append(f"{prefix}weight: this layer keeps its weight in 8 bits; load a 16-bit weight before "
+                              "quantize_int8().")
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
 
 def quantize_int8(module: nn.Module) -> nn.Module:

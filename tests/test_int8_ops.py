@@ -317,3 +317,64 @@ def test_the_torch_backend_has_no_backward_either(name):
                 out.sum().backward()
         assert leaf.grad is None
         leaf.requires_grad_(False)
+
+
+LAYERS = {
+    "column": lambda: Lyr.ColumnParallelLinear(48, 40, bias=True),
+    "merged": lambda: Lyr.MergedColumnParallelLinear(48, [24, 16]),
+    "row": lambda: Lyr.RowParallelLinear(48, 40),
+    "gdn": lambda: Lyr.GdnInputProjection(48, 2, 4, 8, 8),
+    "head": lambda: Lyr.ParallelLMHead(200, 48),
+    "mlp": lambda: Lyr.Qwen35MLP(48, 32),
+}
+
+
+def _made(name, seed, int8):
+    layer = LAYERS[name]()
+    g = torch.Generator().manual_seed(seed)
+    for p in layer.parameters():
+        p.data = torch.randn(p.shape, generator=g)
+    for part in layer.modules():
+        if hasattr(part, "gemm_backend"):
+            part.gemm_backend = "torch"
+    return Lyr.quantize_int8(layer) if int8 else layer
+
+
+def _same(x, y):
+    return all(torch.equal(a, b) for a, b in zip(*(v if isinstance(v, tuple) else (v,) for v in (x, y))))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("strict", [True, False])
+@pytest.mark.parametrize("assign", [False, True])
+@pytest.mark.parametrize("name", LAYERS)
+def test_a_state_dict_in_8_bits_is_loaded(name, assign, strict):
+    """Into a 16-bit layer, which keeps its weight in 8 bits from then on, and into one in 8 bits."""
+    x = torch.randn(5, 48, generator=torch.Generator().manual_seed(9))
+    saved = _made(name, 1, True)
+    want, state = saved(x), {k: v.clone() for k, v in saved.state_dict().items()}
+    for int8 in (False, True):
+        layer = _made(name, 2, int8)
+        out = layer.load_state_dict(state, strict=strict, assign=assign)
+        assert not out.missing_keys and not out.unexpected_keys
+        assert all(part.is_int8 for part in layer.modules() if isinstance(part, Lyr.Int8Weight))
+        assert _same(layer(x), want)
+        again = layer.state_dict()
+        assert set(again) == set(state) and all(again[k].dtype == state[k].dtype for k in state)
+
+
+@pytest.mark.parametrize("strict", [True, False])
+def test_state_dicts_that_do_not_fit_are_refused(strict):
+    layer, full = _made("row", 3, False), _made("row", 4, True)
+    short = {"weight_codes": full.weight_codes[:39], "weight_scales": full.weight_scales[:39]}
+    with pytest.raises(RuntimeError, match="size mismatch for weight_codes"):
+        layer.load_state_dict(short, strict=strict)
+    assert not layer.is_int8 and layer.weight is not None
+    with pytest.raises(RuntimeError, match="keeps its weight in 8 bits"):
+        full.load_state_dict(layer.state_dict(), strict=strict)
+    assert full.is_int8
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        full.load_state_dict(short, strict=strict)
+    if strict:
+        with pytest.raises(RuntimeError, match="weight_codes"):
+            layer.load_state_dict({"weight_codes": full.weight_codes})
