@@ -53,6 +53,7 @@ class Int8Weight(nn.Module):
 
     weight_codes: Optional[torch.Tensor]
     weight_scales: Optional[torch.Tensor]
+    gemm_backend: Optional[str]
 
     def __init__(self):
         super().__init__()
@@ -62,6 +63,12 @@ class Int8Weight(nn.Module):
     @property
     def is_int8(self) -> bool:
         return self.weight_codes is not None
+
+    def matmul(self, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+        if self.is_int8:
+            y = int8_linear(x, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
+            return y if bias is None else y + bias.to(y.dtype)
+        return gemm_linear(x, self.weight, bias, backend=self.gemm_backend)
 
     @torch.no_grad()
     def quantize_int8(self) -> None:
@@ -111,12 +118,6 @@ class LinearBase(Int8Weight):
         else:
             self.register_parameter("bias", None)
         self.gemm_backend: Optional[str] = None   # None: NANOVLLM_GEMM_BACKEND
-
-    def matmul(self, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
-        if self.is_int8:
-            y = int8_linear(x, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
-            return y if bias is None else y + bias.to(y.dtype)
-        return gemm_linear(x, self.weight, bias, backend=self.gemm_backend)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
@@ -372,7 +373,7 @@ class ParallelLMHead(Int8Weight):
         return torch.stack(all_tokens, 0).gather(0, best).squeeze(0), stacked.gather(0, best).squeeze(0)
 
 
-class GemmLinear(nn.Linear):
+class GemmLinear(nn.Linear, Int8Weight):
     """``nn.Linear`` whose matmul goes through the backend switch; drop-in for
     the plain nn.Linear projections of nanovllm/layers/gated_delta_net.py:60-63,
     90 and nanovllm/models/qwen3_5_mtp.py:41."""
@@ -380,4 +381,4 @@ class GemmLinear(nn.Linear):
     gemm_backend: Optional[str] = None
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return gemm_linear(x, self.weight, self.bias, backend=self.gemm_backend)
+        return self.matmul(x, self.bias)

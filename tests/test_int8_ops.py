@@ -378,3 +378,23 @@ def test_state_dicts_that_do_not_fit_are_refused(strict):
     if strict:
         with pytest.raises(RuntimeError, match="weight_codes"):
             layer.load_state_dict({"weight_codes": full.weight_codes})
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("bias", [False, True])
+def test_every_linear_layer_goes_to_8_bits(bias):
+    """GemmLinear, the drop-in for nn.Linear, among them: its rows go through the 8-bit product, and its state dict loads."""
+    g = torch.Generator().manual_seed(8)
+    model = torch.nn.ModuleDict({"plain": Lyr.GemmLinear(48, 40, bias=bias), "row": Lyr.RowParallelLinear(40, 48)})
+    plain = model["plain"]
+    plain.gemm_backend = "auto"
+    for p in model.parameters():
+        p.data = torch.randn(p.shape, generator=g)
+    x, w, b = torch.randn(5, 48, generator=g), plain.weight.clone(), plain.bias
+    exact = F.linear(x.double(), w.double(), None if b is None else b.double())
+    assert Lyr.quantize_int8(model) is model
+    assert plain.is_int8 and plain.weight is None and model["row"].is_int8
+    assert bool(((plain(x).double() - exact).abs() <= int8_error(x, w) + 1e-4).all())
+    fresh = Lyr.GemmLinear(48, 40, bias=bias)
+    fresh.load_state_dict(plain.state_dict())
+    assert fresh.is_int8 and torch.equal(fresh(x), plain(x))
