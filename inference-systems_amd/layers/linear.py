@@ -222,11 +222,14 @@ class RowParallelLinear(LinearBase):
         in front of the GEMM."""
         if self.is_int8:
             backend = validate_gemm_backend(self.gemm_backend) if self.gemm_backend is not None else default_backend()
-            one = x.new_empty((1, x[0].numel())) if backend == "auto" else None
-            if backend == "hip" or (backend == "auto" and gated_contract_reason(x, gate, one) is None):
+            rows = x.reshape(x.shape[0], self.weight_codes.shape[1])
+            # The gate's contract is the gated GEMM's; the rows themselves stand in for its weight.
+            if rows.shape[0] == 0:
+                gated = rows
+            elif backend == "hip" or (backend == "auto" and gated_contract_reason(x, gate, rows) is None):
                 gated = sigmoid_gate(x, gate)
             else:
-                gated = (x.reshape(gate.shape) * torch.sigmoid(gate)).reshape(x.shape[0], -1)
+                gated = (x.reshape(gate.shape) * torch.sigmoid(gate)).reshape(rows.shape)
             y = int8_linear(gated, self.weight_codes, self.weight_scales, backend=self.gemm_backend)
         else:
             y = gated_linear(x, gate, self.weight, backend=self.gemm_backend)

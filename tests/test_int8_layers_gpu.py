@@ -103,3 +103,18 @@ def test_float_scales_are_refused_once_converted(pkg):
     mlp.gemm_backend = "hip"
     with pytest.raises(RuntimeError, match="float32"):
         mlp(torch.zeros(2, HIDDEN, dtype=BF16, device=DEV))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("name", ["hip", "auto"])
+def test_gated_rows_in_8_bits(pkg, name):
+    """On the gate's kernel, and without rows."""
+    layer = build(pkg, 3)["o_proj"]
+    layer.gemm_backend = name
+    g = torch.Generator().manual_seed(4)
+    for m in (0, 1, 5):
+        x, gate = (torch.randn(m, 4, 128, generator=g).to(BF16).to(DEV) for _ in range(2))
+        out = layer.forward_gated(x, gate)
+        assert out.shape == (m, HIDDEN) and out.dtype == BF16
+        if m:
+            assert torch.equal(out, layer(pkg.kernels.sigmoid_gate(x, gate)))

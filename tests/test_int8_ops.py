@@ -398,3 +398,19 @@ def test_every_linear_layer_goes_to_8_bits(bias):
     fresh = Lyr.GemmLinear(48, 40, bias=bias)
     fresh.load_state_dict(plain.state_dict())
     assert fresh.is_int8 and torch.equal(fresh(x), plain(x))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("backend", ["torch", "auto"])
+@pytest.mark.parametrize("shapes", [((4, 8), (4, 8)), ((32,), (32,)), ((32,), (4, 8)), ((4, 8), (32,))])
+def test_gated_rows_in_8_bits(backend, shapes):
+    """The heads and their gate in either layout, without rows too."""
+    g = torch.Generator().manual_seed(12)
+    row = Lyr.RowParallelLinear(32, 24)
+    row.weight.data = torch.randn(24, 32, generator=g)
+    row.gemm_backend = backend
+    row.quantize_int8()
+    for m in (0, 1, 5):
+        x, gate = (torch.randn(m, *s, generator=g) for s in shapes)
+        want = row((x.reshape(m, 32) * torch.sigmoid(gate.reshape(m, 32))))
+        assert torch.equal(row.forward_gated(x, gate), want) and want.shape == (m, 24)
