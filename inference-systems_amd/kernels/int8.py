@@ -321,6 +321,13 @@ def _hip(backend: Optional[str], reason) -> bool:
     return backend == "hip" or (backend == "auto" and reason() is None)
 
 
+def _check_types(name: str, w: torch.Tensor, w_scales: torch.Tensor) -> None:
+    """The torch backend takes the ops' types alone: scales rounded to 16 bits, of a module that was converted after its
+    weights went to 8 bits, are refused and not used."""
+    if w.dtype != torch.int8 or w_scales.dtype != torch.float32:
+        raise RuntimeError(f"{name}: w must be int8 and w_scales float32, got {w.dtype} and {w_scales.dtype}")
+
+
 def _int8_linear(x, w, w_scales, out_dtype, backend, silu_mul):
     out_dtype = x.dtype if out_dtype is None else out_dtype
 
@@ -332,12 +339,14 @@ def _int8_linear(x, w, w_scales, out_dtype, backend, silu_mul):
 
     if _hip(backend, lambda: reason(x, w, w_scales)):
         return run_hip(op, reason, x, w, w_scales)
+    name = "int8_silu_mul_linear" if silu_mul else "int8_linear"
+    _check_types(name, w, w_scales)
     with torch.no_grad():
         if silu_mul:
             y = _torch_silu_mul(torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, torch.float32), out_dtype)
         else:
             y = torch_gemm_int8(*torch_quantize_rows(x), w, w_scales, out_dtype)
-    return _refuse_backward("int8_silu_mul_linear" if silu_mul else "int8_linear", y, x, w_scales)
+    return _refuse_backward(name, y, x, w_scales)
 
 
 def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None,
@@ -371,6 +380,7 @@ def int8_add_rmsnorm_linear(h: torch.Tensor, residual: torch.Tensor, norm_weight
     args = (h, residual, norm_weight, w, w_scales)
     if _hip(backend, lambda: reason(*args)):
         return run_hip(op, reason, *args)
+    _check_types("int8_add_rmsnorm_linear", w, w_scales)
     with torch.no_grad():
         summed = h.float() + residual.float()
         normed = summed * torch.rsqrt(summed.pow(2).mean(-1, keepdim=True) + eps) * (1.0 + norm_weight.float())

@@ -414,3 +414,15 @@ def test_gated_rows_in_8_bits(backend, shapes):
         x, gate = (torch.randn(m, *s, generator=g) for s in shapes)
         want = row((x.reshape(m, 32) * torch.sigmoid(gate.reshape(m, 32))))
         assert torch.equal(row.forward_gated(x, gate), want) and want.shape == (m, 24)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("backend", ["torch", "auto"])
+def test_scales_of_a_converted_module_are_refused(backend):
+    """As on the HIP backend: scales rounded to 16 bits are not used in silence."""
+    mlp, norm = _made("mlp", 1, True).to(BF16), Lyr.Qwen35RMSNorm(48).to(BF16)
+    mlp.gemm_backend = backend
+    x = torch.zeros(2, 48, dtype=BF16)
+    for call in (lambda: mlp(x), lambda: mlp.forward_add_norm(x, x, norm), lambda: mlp.down_proj(x[:, :32])):
+        with pytest.raises(RuntimeError, match="w must be int8 and w_scales float32"):
+            call()
