@@ -39,7 +39,8 @@ int nanovllm_quantize_rows(const void* x, int8_t* codes, float* scales,
  * Residual add and zero-centred RMSNorm with the result in 8 bits: with
  * s = h + r in fp32, residual_out = round(s), and the row
  *     s * (1 + w) * rsqrt(mean(s^2) + eps)
- * in 8 bits as above, from fp32 (it is rounded to no other type).  h, r, w and
+ * in 8 bits as above, from fp32 (it is rounded to no other type; where the sum
+ * of squares passes fp32 it is a row of zeros).  h, r, w and
  * residual_out are of dtype (f16 or bf16); h and r have row strides ldh and
  * ldr; codes and residual_out are contiguous [m, k].  residual_out must not
  * overlap the span of h or of r (refused); nor may any output of these entry

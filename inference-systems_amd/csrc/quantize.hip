@@ -236,7 +236,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(
     reduce_row<TPR>(top, ss);
     Scale sc;
     float scale = row_scale_of(top, sc);
-    if constexpr (NORM) scale *= norm_scale(ss, k, eps);
+    if constexpr (NORM) {
+        // Codes 0 with a scale of 0 (a sum of squares beyond fp32) or of no number
+        // (one that rounds to 0, at eps = 0), as in rows that are so themselves.
+        scale *= norm_scale(ss, k, eps);
+        if (!(scale < __builtin_inff())) scale = __builtin_nanf("");
+        if (!(scale > 0.0f)) sc.s = 0.0f;
+    }
     if (t == 0) scales[row] = scale;
     if constexpr (CH > 0) {
 #pragma unroll

@@ -344,3 +344,20 @@ def test_gemm_int8_silu_mul_wide(ops, m, n, k):
     sw = sw * 3
     for dtype in (BF16, F32):
         check_silu(ops.gemm_int8_silu_mul(*[t.to(DEV) for t in (a, sa, w, sw)], dtype), a, sa, w, sw, dtype)
+
+
+def test_add_rmsnorm_quantize_sums_beyond_float32(ops):
+    """Squares that overflow make a row of zeros, squares that vanish at eps = 0 one of no number, both with codes 0, as the
+    formula in float32 does."""
+    h = torch.zeros(4, 96, dtype=BF16)
+    h[0] = torch.linspace(1e20, 3e20, 96)
+    h[1] = torch.linspace(-1e-25, 1e-25, 96)
+    h[2] = torch.linspace(-2, 2, 96)
+    w = torch.linspace(-0.5, 0.5, 96).to(BF16)
+    codes, scales, residual = (t.cpu() for t in ops.add_rmsnorm_quantize(h.to(DEV), 0 * h.to(DEV), w.to(DEV), 0.0))
+    assert scales[0] == 0 and scales[1].isnan() and scales[3].isnan()
+    assert bool((codes[[0, 1, 3]] == 0).all()) and torch.equal(residual, h)
+    check_norm(h[2:3], 0 * h[2:3], w, 0.0, codes[2:3], scales[2:3], residual[2:3])
+    codes, scales, _ = (t.cpu() for t in ops.add_rmsnorm_quantize(h.to(DEV), 0 * h.to(DEV), w.to(DEV), 1e-6))
+    assert scales[0] == 0 and scales[3] == 0 and bool((codes[[0, 3]] == 0).all())
+    check_norm(h[1:3], 0 * h[1:3], w, 1e-6, codes[1:3], scales[1:3], torch.empty_like(h[1:3]).copy_(h[1:3]))
