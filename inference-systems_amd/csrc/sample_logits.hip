@@ -930,7 +930,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
             const double sum = sums.upto;
             total = sums.all;
             const double target = share * total;
-            const int one = w[0] > 0.0 && sum - w[1] > target ? 0 : w[1] > 0.0 && sum > target ? 1 : -1;
+            // At u = 0 the first weight decides, also one that is lost in the sum with the other.
+            const bool first = sum - w[1] > target || !(target > 0.0);
+            const int one = w[0] > 0.0 && first ? 0 : w[1] > 0.0 && sum > target ? 1 : -1;
             int at = first_of(one >= 0, 2 * tid + one, -1, sh);
             if (at < 0) at = last_of(w[0] + w[1] > 0.0, 2 * tid + (w[1] > 0.0), -1, sh);
             if (at < 0) return take_best();

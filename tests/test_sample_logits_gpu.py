@@ -324,3 +324,15 @@ def test_sample_logits_infinite_temperature(ops, vocab):
     for filters in (dict(), dict(min_p=1.0), dict(min_p=0.5), dict(min_p=1.0, top_k=vocab // 2), dict(min_p=1.0, top_p=0.3),
                     dict(min_p=2.0), dict(min_p=1.0 + 2.0 ** -23)):
         check(ops, x, INF, u, **filters)
+
+
+@pytest.mark.parametrize("filters", [dict(), dict(top_k=30), dict(top_p=1 - 2.0 ** -24)])
+@pytest.mark.parametrize("vocab", [50, 30000])
+def test_sample_logits_first_token_of_small_weight(ops, vocab, filters):
+    """u = 0 takes the first kept token, whatever its weight is beside its neighbours'."""
+    x = torch.full((10, vocab), -INF)
+    for i, down in enumerate((1.0, 20.0, 36.0, 36.8, 37.0, 38.0, 40.0, 41.0, 42.0, 43.0)):
+        at = i * (vocab // 11)
+        x[i, at], x[i, at + 1], x[i, at + 2] = 5.0 - down, 5.0, 5.0 - down
+    for u in (0.0, -1.0, float("nan"), 2.0 ** -24):
+        check(ops, x, 1.0, torch.tensor(u), **filters)
