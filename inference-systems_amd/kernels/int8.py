@@ -257,10 +257,11 @@ def gemm_int8_silu_mul(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor,
 # Backend switch and the same arithmetic in torch operations
 # ---------------------------------------------------------------------------
 def torch_quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """quantize_rows in torch operations (the quotient in 64 bits)."""
+    """quantize_rows in torch operations (the quotients in 64 bits; a division by a plain number in 32 is a product with its
+    reciprocal on a GPU)."""
     top = x.float().abs().amax(-1)
     good = top < float("inf")      # false for a NaN too
-    scale = torch.where(good, top / 127, float("nan"))
+    scale = torch.where(good, (top.double() / 127).float(), float("nan"))
     safe = torch.where(good & (scale > 0), scale, 1.0).double().unsqueeze(-1)
     codes = torch.where((good & (scale > 0)).unsqueeze(-1), (x.double() / safe).round().clamp(-127, 127), 0.0)
     return codes.to(torch.int8), scale

@@ -361,3 +361,14 @@ def test_add_rmsnorm_quantize_sums_beyond_float32(ops):
     codes, scales, _ = (t.cpu() for t in ops.add_rmsnorm_quantize(h.to(DEV), 0 * h.to(DEV), w.to(DEV), 1e-6))
     assert scales[0] == 0 and scales[3] == 0 and bool((codes[[0, 3]] == 0).all())
     check_norm(h[1:3], 0 * h[1:3], w, 1e-6, codes[1:3], scales[1:3], torch.empty_like(h[1:3]).copy_(h[1:3]))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_torch_quantize_rows_on_the_gpu(ops, dtype):
+    """The torch backend's codes and scales are the ops', to the last bit, and the oracle's."""
+    x = (torch.randn(4096, 64, generator=gen(21)) * 3).to(dtype)
+    x[1] = 0
+    x[2] *= 1e-3
+    x[3, 5] = float("nan")
+    codes, scales = ops.torch_quantize_rows(x.to(DEV))
+    check_rows(x, codes, scales)
