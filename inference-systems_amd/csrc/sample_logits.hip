@@ -856,7 +856,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(RowArgs p) {
     }
     const int k_bin = k > 0 && k < vocab ? first_of(sh.count[tid] >= uint32_t(k), tid, kRest, sh) : kRest;
     const double whole = sh.mass[kRest];
-    const double share = u > 0.0f ? double(u) : 0.0;
+    // From 1 on no running sum is above it, whose last bits may pass the total's.
+    const double share = u >= 1.0f ? __builtin_inf() : u > 0.0f ? double(u) : 0.0;
 
     // Where everything up to the border is listed, and not too many, the listed
     // members decide.  With a top-k in front of the top-p its whole bin is needed.

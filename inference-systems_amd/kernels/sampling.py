@@ -140,7 +140,8 @@ def torch_sample_logits(logits: torch.Tensor, temperatures: torch.Tensor, unifor
     running = by_index.cumsum(1)
     total = running[:, -1:]
     u = uniforms.reshape(-1, 1).double()
-    target = torch.where(u > 0, u, 0.0) * total
+    # From 1 on no running sum is above it, whose last bits may pass the total's.
+    target = torch.where(u >= 1, float("inf"), torch.where(u > 0, u, 0.0)) * total
     above = (running > target) & (by_index > 0)
     last = vocab - 1 - (by_index > 0).flip(1).to(torch.int8).argmax(1, keepdim=True)
     token = torch.where(above.any(1, keepdim=True), above.to(torch.int8).argmax(1, keepdim=True), last)

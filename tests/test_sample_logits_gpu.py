@@ -336,3 +336,20 @@ def test_sample_logits_first_token_of_small_weight(ops, vocab, filters):
         x[i, at], x[i, at + 1], x[i, at + 2] = 5.0 - down, 5.0, 5.0 - down
     for u in (0.0, -1.0, float("nan"), 2.0 ** -24):
         check(ops, x, 1.0, torch.tensor(u), **filters)
+
+
+@pytest.mark.parametrize("backend", ["hip", "torch"])
+@pytest.mark.parametrize("filters", [dict(), dict(top_k=900), dict(top_p=0.999)])
+@pytest.mark.parametrize("m,vocab", [(600, 1500), (20, 40000)])
+def test_sample_logits_last_token(ops, m, vocab, filters, backend):
+    """u of 1 or more takes the last kept token: no running sum passes the total by its last bit."""
+    # Weights down to 2^-60, so that many sums are the total but for its last bit.
+    g = torch.Generator().manual_seed(41)
+    t = 0.5 + torch.rand(m, generator=g)
+    x = -41.5 * t[:, None] * torch.rand(m, vocab, generator=g)
+    k, p = filters.get("top_k"), filters.get("top_p")
+    given = [None if v is None else torch.full((m,), v, dtype=d, device=DEV) for v, d in ((k, torch.int32), (p, F32))]
+    for u in (1.0, 1.5, INF):
+        tokens, _ = ops.sample_rows(x.to(DEV), t.to(DEV), torch.full((m,), u, device=DEV), *given, backend=backend)
+        for i in range(m):
+            assert tokens[i] == orc.sample(x[i].double().numpy(), float(t[i]), u, k, p)[0], (i, u)
