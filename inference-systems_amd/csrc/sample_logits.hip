@@ -21,13 +21,13 @@
 // running sum passes u times the total, which it reads again.
 //
 // What bounds it: with many rows the instructions of a weight (23 a logit, 33 with
-// its bin; the histogram's atomics run beside them for nothing), and of a slice's
-// list; with few the join, a chain of short steps whose code is fetched as it runs:
+// its bin, half of the slices' time; the histogram's atomics run beside them for
+// nothing), a slice's list (a fifth) and its fixed steps; with few the join, a chain of short steps whose code is fetched as it runs:
 // loops are left rolled and what a step shares with another is a call.
 //
 // Measured: 1 x 151936 bf16, top-k 50 and top-p 0.9: 25 us, of which the slices 8
 // and the join 15.  256 x 151936 fp32 (156 MB), top-p and min-p by row: 120 us; the
-// slices 72 (2.2 TB/s; reading alone takes 25), the join 50, which is the time of
+// slices 71 (2.2 TB/s; reading alone takes 25), the join 50, which is the time of
 // the rows that look their border up (others 15).  One workgroup a row for all of
 // it: 176 and 231 us.  Slices by 512 threads instead of 1024: 82 us for 78.
 //
